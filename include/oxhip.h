@@ -322,6 +322,100 @@ int oxhip_dev_experts(oxhip_ctx* ctx, oxhip_moe* m, const float* x, size_t t, co
 int oxhip_dev_moe_routed(oxhip_ctx* ctx, oxhip_moe* m, const float* x, size_t t, const float* logits, size_t logit_stride, size_t k,
                          const float* expert_scale, uint32_t* sel, float* y, int add, void* stream);
 
+/* ---- attention over an 8-bit cache (between the q / k / v linears and the output projection: what the reference's graph
+ * runs as Op::QkRope and Op::Attend, src/gpu_decode.rs) ---------------------------------------------------------------
+ * The cache: pages of `page_tokens` tokens (a power of two, 32 at least), cut into blocks of 32. A block holds, for one key head, 32 d
+ * codes of keys (and of values) and one f32 scale for each; a code u stands for (u - 128) * scale. d is a multiple of 32, 256 at most.
+ * All arrays are the caller's, on the device, and start out as they like; k and v begin at multiples of 16 bytes. Codes of block
+ * [page][head][block of the page], a byte each: the key of token t, channel c at c / 32 * 1024 + c % 32 / 8 * 256 + t % 16 * 16 +
+ * t / 16 * 8 + c % 8, its value at c / 32 * 1024 + t % 16 / 4 * 256 + c % 16 * 16 + c % 32 / 16 * 8 + t / 16 * 4 + t % 4: a matrix
+ * instruction's operands in the order in which a wave reads them. */
+typedef struct {
+    uint8_t* k;       /* [n_pages, n_kv, page_tokens / 32, 32 d] */
+    uint8_t* v;       /* the same */
+    float* k_scale;   /* [n_pages, n_kv, page_tokens / 32] */
+    float* v_scale;   /* the same */
+    size_t n_pages, page_tokens, n_kv, d;
+} oxhip_kv_cache;
+
+/* The sequences of a call and their rows (query rows, or new tokens). Sequence s has the rows row_start[s] .. row_start[s + 1] - 1 and
+ * holds kv_len[s] tokens, these rows among them: its last row is token kv_len[s] - 1. Token p lies in page pages[s][p / page_tokens]. All three
+ * arrays are on the device, so that a recorded plan's replays find the lengths of their step there; the calls read no more of them
+ * than the sizes here say. Rows behind the last sequence are left as they are; a sequence may have no rows. */
+typedef struct {
+    size_t n_seqs, rows;
+    const int32_t* row_start; /* [n_seqs + 1], ascending; or NULL: one row per sequence (rows == n_seqs) */
+    const int32_t* kv_len;    /* [n_seqs] */
+    const int32_t* pages;     /* [n_seqs, max_pages]; entries that no token needs may hold anything */
+    size_t max_pages;
+} oxhip_kv_batch;
+
+/* Rotation by a table of angles [n_pos, n_rot / 2] of f32 pairs (cos, sin), at a multiple of 8 bytes: the first n_rot channels of a head, in pairs
+ * (i, i + n_rot / 2), or (2 i, 2 i + 1) if `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin), formed in f64. */
+typedef struct {
+    const float* table;
+    size_t n_pos, n_rot;
+    int interleaved;
+} oxhip_rope;
+
+/* The rows' keys (rotated by the angles of their positions) and values go into the cache, and their queries (optional: q, q_out NULL, n_q 0)
+ * are rotated into q_out (q itself, or apart from it). k, v [rows, n_kv, d], q [rows, n_q, d] of `dtype` (OXHIP_F32, OXHIP_BF16), rows
+ * *_stride values apart (0 = dense); rope NULL: no rotation. A block's scale is the largest magnitude of its values over 127 where all its
+ * tokens come in one call. Tokens that come later and do not fit double it until they do, and the codes that are there are rounded to the new scale:
+ * none is further than a scale from its value, however many calls fill a block (half a scale where it did not grow). Scales stay within 2^-60 and
+ * 2^61, larger values are cut to 127 * 2^60; NaN is stored as 0. A row whose position the table does not hold: q NaN, the key's rotated
+ * channels 0. A page number outside the cache: that token is not stored. A page that a call appends to belongs to one sequence of it; pages
+ * that are only read may be shared. */
+int oxhip_dev_kv_append(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* k, size_t k_stride, const void* v, size_t v_stride,
+                        const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream);
+/* The values that the last `count` tokens of every sequence stand for, k_out / v_out [n_seqs, count, n_kv, d] of `dtype` (either may be NULL);
+ * places before a sequence's first token are zeros, tokens of a page outside the cache NaN. */
+int oxhip_dev_kv_read(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, size_t count, void* k_out, void* v_out, int dtype, void* stream);
+
+/* What a row at position p sees of its sequence: the keys j with j < prefix[s], and those with first[row] <= j <= p and j > p - window. Their
+ * scores: cap * tanh(score / cap), then less slopes[head] * |p - j|. A NULL (or 0) field sets no such rule. */
+typedef struct {
+    float cap;
+    const float* slopes;   /* [n_q] */
+    size_t window;
+    const int32_t* prefix; /* [n_seqs]: keys that every row of the sequence sees, whatever the other rules */
+    const int32_t* first;  /* [rows]: the first key of the row's document */
+} oxhip_attend_rules;
+/* out [rows, n_q, d] = softmax(scale * q K^T, as the rules have it) V over the cache, query head h reading key head h * n_kv / n_q (n_q a
+ * multiple of n_kv); q and out of `dtype`, rows *_stride values apart (0 = dense). Scores, weights' sums and results are formed in
+ * f32; f32 rows enter as two f16 values each (22 bits), bf16 rows as one. A row that sees no key gives zeros; one that would see a token of a page
+ * outside the cache NaN. The stream's scratch (as oxhip_dev_decode_batch's) is made with the first call on it. */
+int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* q, size_t q_stride, size_t n_q, int dtype, float scale,
+                     const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
+
+/* ---- the logits' rules (behind the head's linear) ------------------------------------------------------------------
+ * In this order, for every row; a NULL array sets no such rule. All arrays are on the device.
+ *   history: ids of the row's tokens so far, the first prompt_len[row] of them its prompt. An id that occurs: l > 0 ? l / repetition[row] : l *
+ *            repetition[row]; one that occurs n > 0 times behind the prompt: l - frequency[row] * n - presence[row]. Ids outside the vocabulary
+ *            count for nothing.
+ *   bias:    entries bias_start[row] .. bias_start[row + 1] - 1 of bias_id / bias are added; of an id that is named twice, the last.
+ *   allowed: bit id % 32 of word id / 32 of mask allowed_row[row] (NULL: mask `row`; -1: no mask): where it is 0 the logit becomes -infinity. A mask
+ *            number of n_allowed or more allows nothing. */
+typedef struct {
+    const int32_t* history;     /* [rows], history_stride ids apart */
+    size_t history_stride;
+    const int32_t* history_len; /* [rows] */
+    const int32_t* prompt_len;  /* [rows]; NULL: no prompt */
+    const float *repetition, *presence, *frequency; /* [rows] each, not zero the first */
+    const int32_t* bias_start;  /* [rows + 1] */
+    const int32_t* bias_id;     /* [n_bias] */
+    const float* bias;
+    size_t n_bias;
+    const uint32_t* allowed;    /* [n_allowed], allowed_stride words apart (at least (vocab + 31) / 32) */
+    size_t n_allowed, allowed_stride;
+    const int32_t* allowed_row; /* [rows] */
+} oxhip_logit_rules;
+/* logits [rows, vocab] of `dtype`, rows `stride` values apart (0 = dense), to `out` (the same buffer, one apart from it, or NULL), and the id of
+ * each row's largest resulting logit to `next` (or NULL): the lowest of equal ones, NaN passed over, -1 where all are -infinity. With `next`, the rows are
+ * 16384 at most; scratch as oxhip_dev_attend's. */
+int oxhip_dev_logits(oxhip_ctx* ctx, const void* logits, size_t stride, void* out, size_t out_stride, size_t rows, size_t vocab, int dtype,
+                     const oxhip_logit_rules* rules, int32_t* next, void* stream);
+
 /* ---- a recorded chain of device-pointer ops, replayed with one call ---------------------------------------------
  * The matmul side of DecodePlan::step (src/gpu_decode.rs:572-587; CUDA's per-graph launch list, src/cuda_decode.rs:1044-1049):
  * a token's ops (norm + quantize, linears, route, experts, ...) are issued once between oxhip_plan_begin and

@@ -266,6 +266,27 @@ hipError_t launch_moe_bf16_gate(const WeightView& w, const WeightView& down, con
                                 uint32_t act_kind, float act_param, void* frag, hipStream_t s);
 hipError_t launch_moe_bf16_down(const WeightView& w, const GroupView& g, uint32_t max_chunks, uint32_t chunks, const void* frag, float* out, hipStream_t s);
 
+// The 8-bit key / value cache and the attention over it (kv_cache.hip, attend.hip), the logits' rules (logits.hip)
+struct KvView;
+struct KvBatchView;
+struct RopeView;
+hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
+                            size_t q_stride, void* q_out, size_t q_out_stride, uint32_t n_q, bool bf16, hipStream_t s);
+hipError_t launch_kv_read(const KvView& kv, const KvBatchView& b, size_t count, void* k_out, void* v_out, bool bf16, hipStream_t s);
+struct AttendCall {
+    const void* q;
+    void* out;
+    size_t q_stride, out_stride;
+    const float* slopes;
+    const int32_t *prefix, *first;
+    float scale, cap;
+    uint32_t n_q, window;
+    bool bf16;
+};
+hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
+struct LogitArgs;
+hipError_t launch_logits(const LogitArgs& a, bool bf16, hipStream_t s);
+
 hipError_t launch_fill_zero(uint32_t* p, size_t n, hipStream_t s);  // n dwords, by a kernel on `s`
 
 void set_error(const std::string& msg);

@@ -1,0 +1,31 @@
+// The arguments of the logits' launch (logits.hip).
+#pragma once
+#include "internal.hpp"
+
+namespace oxhip {
+
+struct LogitArgs {
+    const void* x;
+    void* out;      // or none
+    int32_t* next;  // or none
+    size_t x_stride, out_stride;
+    uint32_t rows, vocab;
+    const int32_t *history, *history_len, *prompt_len;
+    size_t history_stride;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_start, *bias_id;
+    const float* bias;
+    uint32_t n_bias, n_allowed;
+    const uint32_t* allowed;
+    size_t allowed_stride;  // words
+    const int32_t* allowed_row;
+    uint64_t* best;      // one per row and slice
+    uint32_t* counters;  // one per row, zero between launches
+    uint32_t slices, vec;
+};
+
+// Workgroups that share a row's vocabulary.
+constexpr uint32_t LOGIT_SLICE = 4096;
+inline size_t logit_slices(size_t vocab) { return (vocab + LOGIT_SLICE - 1) / LOGIT_SLICE; }
+
+}  // namespace oxhip

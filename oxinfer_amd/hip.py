@@ -5,6 +5,7 @@ conventions (False / None = declined, nothing written), plus the device-pointer 
 Device buffers are torch tensors (torch is plumbing for memory and streams only).
 """
 import ctypes as C
+import math
 import os
 
 import numpy as np
@@ -48,6 +49,31 @@ class RowsJob(C.Structure):
 class QActC(C.Structure):
     _fields_ = [("q", C.c_void_p), ("scales", C.c_void_p), ("sums", C.c_void_p), ("fsums", C.c_void_p),
                 ("hsums", C.c_void_p), ("sums16", C.c_void_p), ("t", C.c_size_t), ("n_in", C.c_size_t)]
+
+
+class KvCacheC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n_pages", C.c_size_t),
+                ("page_tokens", C.c_size_t), ("n_kv", C.c_size_t), ("d", C.c_size_t)]
+
+
+class KvBatchC(C.Structure):
+    _fields_ = [("n_seqs", C.c_size_t), ("rows", C.c_size_t), ("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p),
+                ("max_pages", C.c_size_t)]
+
+
+class RopeC(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("n_pos", C.c_size_t), ("n_rot", C.c_size_t), ("interleaved", C.c_int)]
+
+
+class AttendRulesC(C.Structure):
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("window", C.c_size_t), ("prefix", C.c_void_p), ("first", C.c_void_p)]
+
+
+class LogitRulesC(C.Structure):
+    _fields_ = [("history", C.c_void_p), ("history_stride", C.c_size_t), ("history_len", C.c_void_p), ("prompt_len", C.c_void_p),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_start", C.c_void_p),
+                ("bias_id", C.c_void_p), ("bias", C.c_void_p), ("n_bias", C.c_size_t), ("allowed", C.c_void_p), ("n_allowed", C.c_size_t),
+                ("allowed_stride", C.c_size_t), ("allowed_row", C.c_void_p)]
 
 
 _lib = None
@@ -113,6 +139,10 @@ def load_library():
         "oxhip_dev_route": (C.c_int, [vp, vp, vp, vp, sz, sz, sz, sz, vp, vp, vp, vp]),
         "oxhip_dev_experts": (C.c_int, [vp, vp, vp, sz, vp, sz, vp, C.c_int, vp]),
         "oxhip_dev_moe_routed": (C.c_int, [vp, vp, vp, sz, vp, sz, sz, vp, vp, vp, C.c_int, vp]),
+        "oxhip_dev_kv_append": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), vp, sz, vp, sz, vp, sz, vp, sz, sz, C.c_int, C.POINTER(RopeC), vp]),
+        "oxhip_dev_kv_read": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), sz, vp, vp, C.c_int, vp]),
+        "oxhip_dev_attend": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
+        "oxhip_dev_logits": (C.c_int, [vp, vp, sz, vp, sz, sz, sz, C.c_int, C.POINTER(LogitRulesC), vp, vp]),
         "oxhip_plan_begin": (vp, [vp, vp]),
         "oxhip_plan_end": (C.c_int, [vp]),
         "oxhip_plan_launches": (sz, [vp]),
@@ -220,6 +250,82 @@ class QAct:
         self.sums16 = torch.empty((t, n_in // 16), dtype=torch.int32, device=device)
         self.c = QActC(self.q.data_ptr(), self.scales.data_ptr(), self.sums.data_ptr(), self.fsums.data_ptr(),
                        self.hsums.data_ptr(), self.sums16.data_ptr(), t, n_in)
+
+
+def _array(name, t, dtypes, device=None, shape=None):
+    """Checks a dense device tensor that the library gets by its pointer; returns the pointer (None for None)."""
+    if t is None:
+        return None
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype}, wanted {' or '.join(map(str, dtypes))}")
+    if not t.is_cuda or (device is not None and t.device.index != device):
+        raise ValueError(f"{name}: on {t.device}, wanted cuda:{device if device is not None else '*'}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _rows(name, t, width, rows, dtypes, device):
+    """Checks rows [rows, ...] of `width` dense values each, which may lie further apart; returns (pointer, stride in values)."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype}, wanted {' or '.join(map(str, dtypes))}")
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name}: on {t.device}, wanted cuda:{device}")
+    if t.dim() < 2 or t.shape[0] < rows or math.prod(t.shape[1:]) != width:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted at least {rows} rows of {width} values")
+    dense = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and stride != dense:
+            raise ValueError(f"{name}: a row's values are not dense")
+        dense *= size
+    stride = t.stride(0) if t.shape[0] > 1 else width
+    if stride < width:
+        raise ValueError(f"{name}: rows overlap")
+    return t.data_ptr(), stride
+
+
+class KvCache:
+    """`oxhip_kv_cache`: an 8-bit key / value cache in torch tensors, codes uint8 [n_pages, n_kv, page_tokens / 32, 32 d] and f32 scales
+    [n_pages, n_kv, page_tokens / 32] each. `HipBackend.kv_cache` makes a new one."""
+
+    def __init__(self, k, v, k_scale, v_scale, page_tokens, d):
+        import torch
+        n_pages, n_kv = k.shape[:2]
+        per = page_tokens // 32
+        dev = k.device.index if k.is_cuda else None
+        p = [_array(n, t, (torch.uint8,), dev, (n_pages, n_kv, per, 32 * d)) for n, t in (("k", k), ("v", v))]
+        p += [_array(n, t, (torch.float32,), dev, (n_pages, n_kv, per)) for n, t in (("k_scale", k_scale), ("v_scale", v_scale))]
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.page_tokens, self.n_kv, self.d, self.device = page_tokens, n_kv, d, dev
+        self.c = KvCacheC(*p, n_pages, page_tokens, n_kv, d)
+
+
+class KvBatch:
+    """`oxhip_kv_batch`: kv_len int32 [n_seqs], pages int32 [n_seqs, max_pages], row_start int32 [n_seqs + 1] or None (one row each). Their
+    contents may change between calls (and between a recorded plan's replays)."""
+
+    def __init__(self, kv_len, pages, rows=None, row_start=None):
+        import torch
+        n, dev = kv_len.numel(), kv_len.device.index if kv_len.is_cuda else None
+        p = _array("kv_len", kv_len, (torch.int32,), dev, (n,)), _array("pages", pages, (torch.int32,), dev, (n, pages.shape[-1]))
+        start = _array("row_start", row_start, (torch.int32,), dev, (n + 1,))
+        if rows is None and row_start is not None:
+            raise ValueError("rows: how many the batch has in all is the host's to know")
+        self.kv_len, self.pages, self.row_start = kv_len, pages, row_start
+        self.rows, self.n_seqs, self.device = n if rows is None else rows, n, dev
+        self.c = KvBatchC(n, self.rows, start, *p, pages.shape[1])
+
+
+class Rope:
+    """`oxhip_rope`: a table of angles f32 [n_pos, n_rot / 2, 2] of (cos, sin)."""
+
+    def __init__(self, table, interleaved=False):
+        import torch
+        p = _array("table", table, (torch.float32,), table.device.index, (table.shape[0], table.shape[1], 2))
+        self.table = table
+        self.c = RopeC(p, table.shape[0], 2 * table.shape[1], int(interleaved))
 
 
 class HipBackend:
@@ -515,6 +621,137 @@ class HipBackend:
         if not ok:
             raise RuntimeError(self.last_error())
         return sel
+
+    # ---- attention over an 8-bit cache, the logits' rules ---------------------------------------------------------
+    def _stream_here(self):
+        """The current torch stream of this backend's device, which need not be the current device."""
+        import torch
+        if torch._C._cuda_getDevice() == self.device:
+            return self._stream()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _float_rows(self, name, t, width, rows):
+        import torch
+        p, stride = _rows(name, t, width, rows, (torch.float32, torch.bfloat16), self.device)
+        return p, stride, 1 if t.dtype == torch.bfloat16 else 0
+
+    def _held(self, cache, batch):
+        if cache.device != self.device or batch.device != self.device:
+            raise ValueError(f"the cache and the batch are wanted on cuda:{self.device}")
+
+    def kv_cache(self, n_pages, n_kv, d, page_tokens=64):
+        """A new 8-bit cache of n_pages pages of page_tokens tokens (a power of two, 32 at least), d a multiple of 32 up to 256."""
+        import torch
+        dev, per = f"cuda:{self.device}", page_tokens // 32
+        codes = [torch.full((n_pages, n_kv, per, 32 * d), 128, dtype=torch.uint8, device=dev) for _ in range(2)]
+        scales = [torch.zeros((n_pages, n_kv, per), dtype=torch.float32, device=dev) for _ in range(2)]
+        return KvCache(*codes, *scales, page_tokens, d)
+
+    def kv_append(self, cache, batch, k, v, q=None, rope=None, q_out=None):
+        """The rows' keys and values [rows, n_kv * d] (f32 or bf16; any row stride) into the cache; the keys, and the queries [rows, n_q * d],
+        rotated by `rope`. Returns the rotated queries (`q_out`, which may be q) or None."""
+        import torch
+        self._held(cache, batch)
+        width = cache.n_kv * cache.d
+        kp, ks, kd = self._float_rows("k", k, width, batch.rows)
+        vp, vs, vd = self._float_rows("v", v, width, batch.rows)
+        qp = op = None
+        qs = os_ = n_q = 0
+        if q is not None:
+            n_q = math.prod(q.shape[1:]) // cache.d
+            qp, qs, qd = self._float_rows("q", q, n_q * cache.d, batch.rows)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            op, os_, od = self._float_rows("q_out", q_out, n_q * cache.d, batch.rows)
+            if qd != kd or od != kd:
+                raise ValueError("q, q_out, k and v have one type")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if kd != vd:
+            raise ValueError("q, q_out, k and v have one type")
+        if batch.rows and not self.lib.oxhip_dev_kv_append(self.ctx, C.byref(cache.c), C.byref(batch.c), kp, ks, vp, vs, qp, qs, op, os_, n_q, kd,
+                                            C.byref(rope.c) if rope is not None else None, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return q_out
+
+    def kv_read(self, cache, batch, count, dtype=None):
+        """The values that the last `count` tokens of every sequence stand for: (k, v), each [n_seqs, count, n_kv, d] f32 (or bf16)."""
+        import torch
+        self._held(cache, batch)
+        dtype = dtype or torch.float32
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"dtype: {dtype}")
+        k, v = (torch.empty((batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype, device=cache.k.device) for _ in range(2))
+        if count and not self.lib.oxhip_dev_kv_read(self.ctx, C.byref(cache.c), C.byref(batch.c), count, k.data_ptr(), v.data_ptr(),
+                                                    int(dtype == torch.bfloat16), self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return k, v
+
+    def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
+        """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of
+        `oxhip_attend_rules`. Returns out, of q's shape and type."""
+        import torch
+        self._held(cache, batch)
+        n_q = math.prod(q.shape[1:]) // cache.d
+        qp, qs, qd = self._float_rows("q", q, n_q * cache.d, batch.rows)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        op, os_, od = self._float_rows("out", out, n_q * cache.d, batch.rows)
+        if qd != od:
+            raise ValueError("q and out have one type")
+        rules = None
+        if cap or window or slopes is not None or prefix is not None or first is not None:
+            if window < 0:
+                raise ValueError("window: at least 0")
+            if first is not None and first.numel() < batch.rows:
+                raise ValueError("first: one for each row")
+            rules = C.byref(AttendRulesC(cap, _array("slopes", slopes, (torch.float32,), self.device, (n_q,)), window,
+                                         _array("prefix", prefix, (torch.int32,), self.device, (batch.n_seqs,)),
+                                         _array("first", first, (torch.int32,), self.device)))
+        if batch.rows and not self.lib.oxhip_dev_attend(self.ctx, C.byref(cache.c), C.byref(batch.c), qp, qs, n_q, qd, cache.d**-0.5 if scale is None else scale, rules,
+                                         op, os_, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out
+
+    def adjust_logits(self, logits, out=None, want_out=True, want_next=True, history=None, history_len=None, prompt_len=None, repetition=None,
+                      presence=None, frequency=None, bias_start=None, bias_id=None, bias=None, allowed=None, allowed_row=None):
+        """The rules of `oxhip_logit_rules` on rows of logits [rows, vocab] (f32 or bf16; any row stride): (out, next), the adjusted logits (`out`
+        may be `logits`) and the best token of each row, int32. history int32 [rows, most], allowed int32 words [masks, (vocab + 31) / 32]."""
+        import torch
+        t, vocab = logits.shape
+        lp, ls, ld = self._float_rows("logits", logits, vocab, t)
+        op, os_ = None, 0
+        if out is not None or want_out:
+            if out is None:
+                out = torch.empty((t, vocab), dtype=logits.dtype, device=logits.device)
+            op, os_, od = self._float_rows("out", out, vocab, t)
+            if od != ld:
+                raise ValueError("logits and out have one type")
+        best = torch.empty(t, dtype=torch.int32, device=logits.device) if want_next else None
+        ints, floats = (torch.int32,), (torch.float32,)
+
+        def array(name, v, dtypes, *shape):
+            return _array(name, v, dtypes, self.device, shape)
+
+        for name, v, n in (("history", history, t), ("allowed", allowed, 1)):
+            if v is not None and (v.dim() != 2 or v.shape[0] < n):
+                raise ValueError(f"{name}: shape {tuple(v.shape)}")
+        rules = None
+        if history is not None or bias_start is not None or allowed is not None:
+            rules = C.byref(LogitRulesC(
+                array("history", history, ints, t, history.shape[1]) if history is not None else None, history.shape[1] if history is not None else 0,
+                array("history_len", history_len, ints, t), array("prompt_len", prompt_len, ints, t), array("repetition", repetition, floats, t),
+                array("presence", presence, floats, t), array("frequency", frequency, floats, t), array("bias_start", bias_start, ints, t + 1),
+                _array("bias_id", bias_id, ints, self.device), _array("bias", bias, floats, self.device, bias_id.shape if bias_id is not None else None),
+                bias_id.numel() if bias_id is not None else 0, _array("allowed", allowed, ints, self.device), allowed.shape[0] if allowed is not None else 0,
+                allowed.shape[1] if allowed is not None else 0, array("allowed_row", allowed_row, ints, t)))
+        elif any(v is not None for v in (history_len, prompt_len, repetition, presence, frequency, bias_id, bias, allowed_row)):
+            raise ValueError("penalties need a history, biases bias_start, allowed_row masks")
+        if op is None and best is None:
+            raise ValueError("neither the adjusted logits nor the best tokens are wanted")
+        if t and not self.lib.oxhip_dev_logits(self.ctx, lp, ls, op, os_, t, vocab, ld, rules, best.data_ptr() if want_next else None, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out, best
 
     def plan_record(self, chain):
         """Records chain() (device-pointer calls on the current torch stream, which must not be the null stream) and

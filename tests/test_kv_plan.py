@@ -1,0 +1,211 @@
+"""The index arithmetic of the key / value cache (csrc/kv_plan.hpp) compiled for the CPU, and what its entry points refuse (no device needed)."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from tests import kv_ref
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oxinfer_amd", "csrc")
+
+PROGRAM = r"""
+#include "kv_plan.hpp"
+#include <cstdio>
+#include <cstring>
+#include <vector>
+using namespace oxhip;
+int main() {
+    char what[16];
+    while (std::scanf("%15s", what) == 1) {
+        if (!std::strcmp(what, "offsets")) {
+            unsigned d;
+            if (std::scanf("%u", &d) != 1) return 1;
+            for (unsigned t = 0; t < KV_BLOCK; t++)
+                for (unsigned c = 0; c < d; c++) std::printf("%u %u\n", kv_key_offset(t, c), kv_value_offset(t, c));
+        } else if (!std::strcmp(what, "place")) {
+            unsigned long long start, s;
+            unsigned unit, more;
+            if (std::scanf("%llu %llu %u %u", &start, &s, &unit, &more) != 4) return 1;
+            std::printf("%llu %llu\n", (unsigned long long)kv_first_place(start, s, unit, more), (unsigned long long)kv_places(start, s, unit, more));
+        } else if (!std::strcmp(what, "span")) {
+            long long pre, lo, hi;
+            if (std::scanf("%lld %lld %lld", &pre, &lo, &hi) != 3) return 1;
+            const KvSpan s = kv_span(pre, lo, hi);
+            for (unsigned i = 0; i < s.count; i++) std::printf("%u ", kv_span_block(s, i));
+            std::printf("\n");
+        } else if (!std::strcmp(what, "part")) {
+            int s, r0, r1, len;
+            unsigned rows, pages, shift;
+            if (std::scanf("%d %d %d %d %u %u %u", &s, &r0, &r1, &len, &rows, &pages, &shift) != 7) return 1;
+            const KvSeq q = kv_part(s, r0, r1, len, rows, pages, shift);
+            std::printf("%d %d %d %d\n", q.s, q.row0, q.n, q.len);
+        } else {
+            int id;
+            unsigned most, n_pages, block, shift;
+            if (std::scanf("%d %u %u %u %u", &id, &most, &n_pages, &block, &shift) != 5) return 1;
+            std::vector<int32_t> table(most, id);
+            std::printf("%d\n", kv_page_of(table.data(), most, n_pages, block, shift));
+        }
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    d = tmp_path_factory.mktemp("kv_plan")
+    (d / "main.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", CSRC, str(d / "main.cpp"), "-o", str(d / "main")], check=True)
+
+    def ask(lines):
+        r = subprocess.run([str(d / "main")], input="\n".join(lines), capture_output=True, text=True, check=True)
+        return [list(map(int, line.split())) for line in r.stdout.splitlines()]
+    return ask
+
+
+@pytest.mark.parametrize("d", range(32, 257, 32))
+def test_a_blocks_bytes(ask, d):
+    """Every token's channel has a byte of its own, where the reference layout has it."""
+    got = np.array(ask([f"offsets {d}"])).reshape(32, d, 2)
+    for i, want in enumerate(kv_ref.offsets(d)):
+        assert np.array_equal(got[..., i], want)
+        assert np.array_equal(np.sort(got[..., i].reshape(-1)), np.arange(32 * d))
+
+
+def test_places_of_ragged_sequences(ask):
+    """Every sequence has room for its tiles (of 16 entries, g to a row) and for the blocks that its tokens touch, and the launch covers all."""
+    rng = np.random.default_rng(1)
+    for _ in range(30):
+        n = rng.integers(0, rng.choice([2, 5, 40, 300]), rng.integers(1, 70))
+        start = np.concatenate([[0], np.cumsum(n)])
+        for g in (1, 3, 16, 17):
+            got = np.array(ask([f"place {v * g} {s} 16 1" for s, v in enumerate(start)]))
+            assert (np.diff(got[:, 0]) >= -(-(n * g) // 16)).all() and got[-1, 1] >= got[-1, 0]
+        got = np.array(ask([f"place {v} {s} 32 2" for s, v in enumerate(start)]))
+        for at in range(32):  # wherever the first token lies in its block
+            assert (np.diff(got[:, 0]) >= np.where(n > 0, (at + n + 31) // 32, 0)).all()
+        assert (np.diff(got[:, 0]) > 0).all()
+
+
+def test_spans_of_blocks(ask):
+    """The blocks of [0, prefix) and [lo, hi), each once, in order."""
+    rng = np.random.default_rng(2)
+    cases = [(0, 0, 0), (0, 5, 5), (0, 2**31 - 1, 0), (0, 0, 1), (32, 0, 32), (33, 40, 70), (7, 100, 101), (200, 10, 90), (1, 31, 33), (64, 64, 65)]
+    cases += [tuple(int(v) for v in rng.integers(0, 400, 3)) for _ in range(200)]
+    for (pre, lo, hi), got in zip(cases, ask([f"span {p} {a} {b}" for p, a, b in cases])):
+        want = set(range(-(-pre // 32))) | (set(range(lo // 32, -(-hi // 32))) if hi > lo else set())
+        assert got == sorted(want), (pre, lo, hi)
+
+
+def test_unsound_sequences_and_pages(ask):
+    """Rows outside the batch, lengths outside the table and pages outside the cache are cut off before anything is read with them."""
+    parts = [("0 0 4 7 4 2 0", [0, 0, 4, 7]), ("1 -5 3 7 4 2 0", [1, 0, 3, 7]), ("1 2 9 7 4 2 0", [1, 2, 2, 7]), ("1 9 2 7 4 2 0", [1, 9, 0, 7]), ("2 5 9 7 4 2 0", [2, 5, 0, 7]),
+             ("0 0 1 -3 4 2 0", [0, 0, 1, 0]), ("0 0 1 65 4 2 0", [0, 0, 1, 64]), ("0 0 1 2147483647 4 2 3", [0, 0, 1, 512]), ("0 0 1 2147483647 1 67108862 0", [0, 0, 1, 2147483584])]
+    assert ask([f"part {p}" for p, _ in parts]) == [w for _, w in parts]
+    pages = [("3 2 4 0 0", 3), ("4 2 4 0 0", -1), ("-1 2 4 0 0", -1), ("-2147483648 2 4 0 0", -1), ("2147483647 2 4 0 0", -1), ("3 2 4 2 0", -1), ("3 2 4 15 3", 3), ("3 2 4 16 3", -1)]
+    assert ask([f"page {p}" for p, _ in pages]) == [[w] for _, w in pages]
+
+
+# ---- refusals: every check comes before the context is looked at, so that valid arguments without one are told from invalid ones ----------
+
+P = 4096  # stands for a device pointer: nothing on this side reads it
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from oxinfer_amd import build, hip
+    if not os.path.exists(hip.library_path()):
+        build.build()
+    return hip.load_library()
+
+
+def structs(hip, kv=(), b=()):
+    c = dict(k=P, v=P, k_scale=P, v_scale=P, n_pages=9, page_tokens=64, n_kv=2, d=64, **{})
+    bb = dict(n_seqs=3, rows=3, row_start=None, kv_len=P, pages=P, max_pages=4)
+    c.update(kv)
+    bb.update(b)
+    return hip.KvCacheC(**c), hip.KvBatchC(**bb)
+
+
+def said(lib, ok):
+    assert ok == 0
+    return lib.oxhip_last_error().decode()
+
+
+BAD_KV = [dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=P + 8), dict(v=P + 1), dict(k_scale=P + 2), dict(d=0), dict(d=48), dict(d=288), dict(page_tokens=16), dict(page_tokens=0),
+          dict(page_tokens=96), dict(page_tokens=2**31), dict(n_kv=0), dict(n_kv=20000), dict(n_pages=0), dict(n_pages=2**31)]
+BAD_B = [dict(kv_len=None), dict(pages=None), dict(kv_len=P + 1), dict(row_start=P + 2), dict(n_seqs=0), dict(n_seqs=2**25, rows=2**25), dict(max_pages=0), dict(max_pages=2**31), dict(max_pages=2**26), dict(rows=4),
+         dict(rows=2**29, row_start=P)]
+OF_KV = [(a, ()) for a in BAD_KV] + [((), a) for a in BAD_B]
+
+
+@pytest.mark.parametrize("kv,b", OF_KV)
+def test_caches_and_batches_that_are_refused(lib, kv, b):
+    from oxinfer_amd import hip
+    good, bad = structs(hip), structs(hip, kv, b)
+    for cache, batch, null in ((*good, True), (*bad, False)):
+        for ok in (lambda: lib.oxhip_dev_attend(None, C.byref(cache), C.byref(batch), P, 0, 4, 0, 1.0, None, P, 0, None),
+                   lambda: lib.oxhip_dev_kv_append(None, C.byref(cache), C.byref(batch), P, 0, P, 0, None, 0, None, 0, 0, 0, None, None),
+                   lambda: lib.oxhip_dev_kv_read(None, C.byref(cache), C.byref(batch), 5, P, P, 0, None)):
+            assert ("null context" in said(lib, ok())) == null
+
+
+def test_rows_and_rules_that_are_refused(lib):
+    from oxinfer_amd import hip
+    cache, batch = (C.byref(s) for s in structs(hip))
+
+    def attend(q=P, qs=0, n_q=4, dtype=0, scale=0.5, rules=None, out=P, os=0):
+        return said(lib, lib.oxhip_dev_attend(None, cache, batch, q, qs, n_q, dtype, scale, C.byref(hip.AttendRulesC(**rules)) if rules is not None else None, out, os, None))
+
+    for good in (dict(), dict(dtype=1, q=P + 2, out=P + 2), dict(qs=256, os=300), dict(scale=-2.0), dict(scale=0.0), dict(rules=dict(cap=30.0, slopes=P, window=2**40, prefix=P, first=P))):
+        assert "null context" in attend(**good), good
+    for bad in (dict(q=None), dict(out=None), dict(q=P + 2), dict(out=P + 1, dtype=1), dict(n_q=0), dict(n_q=3), dict(n_q=2**17), dict(dtype=2), dict(dtype=-1), dict(scale=float("inf")), dict(scale=float("nan")),
+                dict(qs=255), dict(os=1), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=float("nan"))), dict(rules=dict(cap=float("inf"))), dict(rules=dict(slopes=P + 1)), dict(rules=dict(first=P + 2))):
+        assert "null context" not in attend(**bad), bad
+
+    def append(k=P, ks=0, v=P, vs=0, q=P, qs=0, out=P, os=0, n_q=4, dtype=0, rope=None):
+        return said(lib, lib.oxhip_dev_kv_append(None, cache, batch, k, ks, v, vs, q, qs, out, os, n_q, dtype, C.byref(hip.RopeC(*rope)) if rope else None, None))
+
+    for good in (dict(), dict(q=None, out=None, n_q=0), dict(rope=(P, 9, 64, 0)), dict(rope=(P, 1, 2, 1)), dict(qs=300, os=300), dict(qs=300, out=2 * P, os=301)):
+        assert "null context" in append(**good), good
+    for bad in (dict(k=None), dict(v=None), dict(q=None), dict(out=None), dict(n_q=0), dict(n_q=40000), dict(k=P + 2), dict(dtype=5), dict(ks=127), dict(vs=1), dict(qs=255), dict(os=255), dict(qs=256, os=300),
+                dict(rope=(None, 9, 64, 0)), dict(rope=(P + 4, 9, 64, 0)), dict(rope=(P, 0, 64, 0)), dict(rope=(P, 9, 63, 0)), dict(rope=(P, 9, 0, 0)), dict(rope=(P, 9, 66, 0))):
+        assert "null context" not in append(**bad), bad
+    read = lambda *a: said(lib, lib.oxhip_dev_kv_read(None, cache, batch, *a, None))  # noqa: E731
+    assert "null context" in read(5, P, None, 1)
+    for bad in ((5, None, None, 0), (5, P, P, 2), (5, P + 2, P, 0), (2**31, P, P, 0)):
+        assert "null context" not in read(*bad), bad
+
+
+def test_logits_rules_that_are_refused(lib):
+    from oxinfer_amd import hip
+
+    def logits(x=P, s=0, out=P, os=0, rows=3, vocab=1000, dtype=0, next=P, **rules):
+        return said(lib, lib.oxhip_dev_logits(None, x, s, out, os, rows, vocab, dtype, C.byref(hip.LogitRulesC(**rules)) if rules else None, next, None))
+
+    hist = dict(history=P, history_stride=7, history_len=P)
+    bias = dict(bias_start=P, bias_id=P, bias=P, n_bias=4)
+    mask = dict(allowed=P, allowed_stride=32, n_allowed=3)
+    for good in (dict(), dict(out=None), dict(next=None), dict(s=1001, os=1001), dict(s=1001, out=2 * P, os=1000), hist, dict(hist, repetition=P, prompt_len=P), bias, mask, dict(mask, n_allowed=1, allowed_row=P)):
+        assert "null context" in logits(**good), good
+    for bad in (dict(x=None), dict(out=None, next=None), dict(dtype=3), dict(vocab=0), dict(vocab=2**31), dict(rows=2**25), dict(x=P + 2), dict(next=P + 2), dict(s=999), dict(os=999), dict(s=1001),
+                dict(history=P), dict(hist, history_stride=0), dict(hist, history_len=None), dict(repetition=P), dict(prompt_len=P), dict(bias, bias=None), dict(bias, bias_start=None), dict(bias, n_bias=2**31),
+                dict(mask, allowed_stride=31), dict(mask, n_allowed=0), dict(mask, n_allowed=2), dict(allowed_row=P), dict(mask, allowed=P + 2)):
+        assert "null context" not in logits(**bad), bad
+
+
+def test_the_bindings_own_checks():
+    """What the binding tells from shapes, types and devices before the library is called."""
+    import torch
+    from oxinfer_amd import hip
+    z = lambda *s, t=torch.uint8: torch.zeros(s, dtype=t)  # noqa: E731
+    with pytest.raises(ValueError, match="wanted cuda"):
+        hip.KvCache(z(3, 2, 2, 2048), z(3, 2, 2, 2048), z(3, 2, 2, t=torch.float32), z(3, 2, 2, t=torch.float32), 64, 64)
+    with pytest.raises(ValueError, match="int8"):
+        hip.KvCache(z(3, 2, 2, 2048, t=torch.int8), z(3, 2, 2, 2048), z(3, 2, 2, t=torch.float32), z(3, 2, 2, t=torch.float32), 64, 64)
+    with pytest.raises(ValueError, match="wanted"):
+        hip.KvBatch(z(3), z(3, 4, t=torch.int32))
+    with pytest.raises(ValueError, match="wanted"):
+        hip.Rope(z(3, 4, 2, t=torch.float64))

@@ -12,6 +12,8 @@
 // hardly ever behind a wave's first blocks): of weights rounded to f16, small ones keep as many bits as there are.
 // f32 rows: q and p' go in as two f16 values each (value and residual, 22 bits), twice the matrix instructions, which the reads hide.
 // bf16 rows: as one (11 bits, where the rows and results have 8); the rows are scaled by a power of two each, so that nothing overflows.
+#include <type_traits>
+
 #include "kv.hpp"
 
 namespace oxhip {
@@ -31,11 +33,12 @@ struct AttendArgs {
     float* partial;
     uint32_t* counters;
     float scale, cap;
-    uint32_t n_q, g, window, splits, cols, vec;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
+    uint32_t n_q, g, window, cols, vec, quantum;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from it that 2^(NO_MAX - score) is 0
+constexpr uint32_t MOST_SPLITS = 256;  // workgroups of a launch, and so of a tile
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
 
 // Eight codes as f16 values, exactly.
@@ -49,14 +52,48 @@ __device__ __forceinline__ half8 code_values(uint32_t a, uint32_t b) {
     return o.v;
 }
 __device__ __forceinline__ f32x4 mma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-// The largest over the four lanes that hold an entry's scores.
+// Over the four lanes that hold an entry's scores, 16 apart: the largest, and the sum.
+template <class F>
+__device__ __forceinline__ float entry_fold(float v, F f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float entry_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    return entry_fold(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float entry_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    return entry_fold(v, [](float a, float b) { return a + b; });
+}
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int32_t lanes_of(int32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+// Over the 16 entries (the lanes of a row of 16), as a scalar.
+template <class F>
+__device__ __forceinline__ int32_t tile_fold(int32_t v, F f) {
+    v = f(v, lanes_of<0x128>(v));  // row_ror:8, 4, 2, 1
+    v = f(v, lanes_of<0x124>(v));
+    v = f(v, lanes_of<0x122>(v));
+    v = f(v, lanes_of<0x121>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int32_t tile_min(int32_t v) {
+    return tile_fold(v, [](int32_t a, int32_t b) { return min(a, b); });
+}
+__device__ __forceinline__ int32_t tile_max(int32_t v) {
+    return tile_fold(v, [](int32_t a, int32_t b) { return max(a, b); });
+}
+// The sum of a wave's lanes up to one's own.
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+    v += (uint32_t)lanes_of<0x111>((int32_t)v);  // row_shr:1, 2, 4, 8
+    v += (uint32_t)lanes_of<0x112>((int32_t)v);
+    v += (uint32_t)lanes_of<0x114>((int32_t)v);
+    v += (uint32_t)lanes_of<0x118>((int32_t)v);
+    v += (uint32_t)lanes_of<0x142, 0xA>((int32_t)v);  // row_bcast:15, then :31
+    v += (uint32_t)lanes_of<0x143, 0xC>((int32_t)v);
+    return v;
 }
 // tanh: by its series below 1/4 (the next term is 2^-27 of the value), where 1 - 2 / (e^2x + 1) cancels, and by that above.
 __device__ __forceinline__ float tanh_of(float x) {
@@ -66,29 +103,100 @@ __device__ __forceinline__ float tanh_of(float x) {
     return a < 0.25f ? series : copysignf(1.0f - 2.0f / (e + 1.0f), x);
 }
 
+// A value that all lanes hold alike, as a scalar.
+__device__ __forceinline__ uint32_t scalar(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// Waves of a workgroup: as many as its registers leave room for on a CU, where a workgroup is alone.
+constexpr int split_waves(int kd) { return kd <= 4 ? 16 : 8; }
+
 // KD = d / 32; F32: f32 rows; RULES: capped or biased scores, or a factor outside the range that the plain path takes.
 template <int KD, bool F32, bool RULES>
-__global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
-    constexpr int NW = 8, PLANES = F32 ? 2 : 1, CHUNK = KD >= 2 ? 64 : 32;  // channels whose sums the waves exchange at a time
-    __shared__ float red[NW][16][CHUNK + 1];
+__global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(AttendArgs a) {
+    constexpr int NW = split_waves(KD), PLANES = F32 ? 2 : 1, CHUNK = KD >= 2 ? 64 : 32;  // channels whose sums the waves exchange at a time
+    constexpr int RED = NW * 16 * (CHUNK + 1) > NW * 4 * (KD * 32 + 1) ? NW * 16 * (CHUNK + 1) : NW * 4 * (KD * 32 + 1), JOIN = 16 * MOST_SPLITS + NW * 128;
+    __shared__ __align__(16) float lds[RED > JOIN ? RED : JOIN];
     __shared__ float m_s[NW][16], l_s[NW][16];
     __shared__ uint32_t last_s;
+    __shared__ half8 q_s[PLANES][KD][64];
+    __shared__ float top_s[KD][16];
     constexpr uint32_t d = KD * 32;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, grp = lane >> 4;
-    const uint32_t split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits, kvh = pair % a.kv.n_kv, place = pair / a.kv.n_kv, g = a.g;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = a.g;
+    uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, grp = lane >> 4;
+    // The compiler takes the thread's number as new: the addresses that it makes of it for one part of a tile's work would otherwise stay in
+    // registers through all the others.
+    auto anew = [&]() {
+        asm volatile("" : "+v"(tid));
+        lane = tid & 63;
+        n = lane & 15;
+        grp = lane >> 4;
+    };
 
-    int32_t s, tile;
-    if (a.b.row_start) {
-        s = kv_find(a.b, place, g, 16, 1);
-        tile = (int32_t)(place - (uint32_t)kv_first_place((uint64_t)(uint32_t)max(a.b.row_start[s], 0) * g, s, 16, 1));
-    } else {
-        const uint32_t per = (g + 15) / 16;
-        s = (int32_t)(place / per);
-        tile = (int32_t)(place % per);
+    // This workgroup's share: all tiles' weights (kv_weight) lie one after the other, sequence by sequence, tile by tile, a tile's key heads
+    // together; every workgroup takes as much of them. A wave adds them up, a lane a sequence, 64 sequences at a time, for the others too: what
+    // decides how many barriers a wave passes is read once.
+    __shared__ int32_t seq_s[4][64];
+    __shared__ uint32_t upto_s[64];
+    KvSeq mine{};              // the lane's sequence of the 64 from s0 on
+    uint32_t mine_blocks, mine_upto, s0 = 0;  // its tiles' weight each; the weights of the lanes up to it
+    auto load = [&](uint32_t from) {
+        s0 = from;
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t all = 0;
+            mine_blocks = 1;
+            if (s0 + lane < a.b.n_seqs) {
+                mine = kv_seq(a.b, (int32_t)(s0 + lane), a.kv.shift);
+                mine_blocks = kv_weight(mine, a.window, a.window && a.prefix ? a.prefix[s0 + lane] : 0, a.quantum);
+                all = kv_tiles(mine, g) * a.kv.n_kv * mine_blocks;
+            }
+            seq_s[0][lane] = mine.row0;
+            seq_s[1][lane] = mine.n;
+            seq_s[2][lane] = mine.len;
+            seq_s[3][lane] = (int32_t)mine_blocks;
+            upto_s[lane] = lanes_upto(all);
+        }
+        __syncthreads();
+        mine.row0 = seq_s[0][lane];
+        mine.n = seq_s[1][lane];
+        mine.len = seq_s[2][lane];
+        mine_blocks = (uint32_t)seq_s[3][lane];
+        mine_upto = upto_s[lane];
+        return (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, 63);
+    };
+    uint32_t total = 0;
+    for (uint32_t from = 0; from < a.b.n_seqs; from += 64) total += load(from);
+    const uint32_t size = max((total + gridDim.x - 1) / gridDim.x, 1u), share0 = blockIdx.x * size, share1 = min(share0 + size, total);
+    if (share0 >= share1 || total <= share0) return;
+    uint32_t s_at = 0;  // where the weights of the 64 sequences in the lanes begin
+    if (a.b.n_seqs > 64) {
+        uint32_t here = load(0);
+        while (s_at + here <= share0) {
+            if (s0 + 64 >= a.b.n_seqs) return;
+            s_at += here;
+            here = load(s0 + 64);
+        }
     }
-    const KvSeq seq = kv_seq(a.b, s, a.kv.shift);
+  for (uint32_t place = share0; place < share1;) {
+    uint64_t behind = __ballot(s_at + mine_upto > place);  // sequences that end behind the place
+    while (!behind) {
+        if (s0 + 64 >= a.b.n_seqs) return;
+        s_at += (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, 63);
+        load(s0 + 64);
+        behind = __ballot(s_at + mine_upto > place);
+    }
+    const uint32_t from = (uint32_t)__builtin_ctzll(behind), s = s0 + from;
+    const KvSeq seq{(int32_t)s, __builtin_amdgcn_readlane(mine.row0, from), __builtin_amdgcn_readlane(mine.n, from), __builtin_amdgcn_readlane(mine.len, from)};
+    const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane((int)mine_blocks, from);
+    const uint32_t seq_at = s_at + (from ? (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, from - 1) : 0u);
+    const uint32_t unit = (place - seq_at) / blocks, unit_at = seq_at + unit * blocks;
+    const uint32_t x0 = place - unit_at, x1 = min(blocks, share1 - unit_at);
+    const int32_t tile = (int32_t)(unit / a.kv.n_kv);
+    const uint32_t kvh = unit - (uint32_t)tile * a.kv.n_kv;
+    place = unit_at + x1;
+    const uint32_t first_wg = x0 ? unit_at / size : blockIdx.x, active = (unit_at + blocks - 1) / size - first_wg + 1;  // workgroups that share this tile
+    __syncthreads();  // (what the tile before left in LDS has been read)
+    anew();
     const int64_t entries = (int64_t)seq.n * g;
-    if (tile < 0 || (int64_t)tile * 16 >= entries) return;
     const uint32_t e = (uint32_t)tile * 16 + n, cols = (uint32_t)min((int64_t)16, entries - (int64_t)tile * 16);
     const bool live = n < cols;
     const uint32_t i = live ? e / g : 0u, head = kvh * g + (live ? e % g : 0u);
@@ -104,131 +212,146 @@ __global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
         if (hi <= lo) lo = hi = 0;
         if (a.prefix) pre = min(max(a.prefix[s], 0), seq.len);
     }
-    int32_t lo_min = hi > lo ? lo : INT32_MAX, hi_max = hi, lo_max = live ? lo : 0, hi_min = live ? hi : INT32_MAX, pre_max = pre;
-#pragma unroll
-    for (int m = 8; m; m >>= 1) {
-        lo_min = min(lo_min, __shfl_xor(lo_min, m));
-        hi_max = max(hi_max, __shfl_xor(hi_max, m));
-        lo_max = max(lo_max, __shfl_xor(lo_max, m));
-        hi_min = min(hi_min, __shfl_xor(hi_min, m));
-        pre_max = max(pre_max, __shfl_xor(pre_max, m));
-    }
-    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
-    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-    pre_max = __builtin_amdgcn_readfirstlane(pre_max);
+    const int32_t lo_min = tile_min(hi > lo ? lo : INT32_MAX), hi_max = tile_max(hi), lo_max = tile_max(live ? lo : 0), hi_min = tile_min(live ? hi : INT32_MAX);
+    const int32_t pre_max = tile_max(pre);
     const KvSpan span = kv_span(pre_max, lo_min, hi_max);
-    // the splits' shares: equal, and at least a block for each wave
-    const uint32_t share = max((uint32_t)NW, (span.count + a.splits - 1) / a.splits), active = max(1u, (span.count + share - 1) / share);
-    if (split >= active) return;
-    const uint32_t b0 = split * share, b1 = min(b0 + share, span.count);
+    const uint32_t b0 = x0 ? (uint32_t)((uint64_t)span.count * x0 / blocks) : 0u, b1 = x1 < blocks ? (uint32_t)((uint64_t)span.count * x1 / blocks) : span.count;
 
-    // the entry's query as operands, scaled to 2^14 at most
-    half8 qh[KD], ql[PLANES == 2 ? KD : 1];
-    float factor;  // of a score, with the key scale: natural units where RULES, else times log2 e
-    {
-        float v[KD][8], top = 0.0f;
+    // The entry's query as operands: in LDS, where all waves read it for each block (kept in registers, it would cost a wave in two its place on
+    // the CU). Wave ks brings the channels 32 ks .. 32 ks + 31. What depends on memory goes in an order that keeps the chain short: queries and
+    // page numbers are asked for together, the first keys and the scales before the queries are converted.
+    float v[8];
+    if (wave < KD) {
+        const size_t at = row * a.q_stride + (size_t)head * d + wave * 32 + grp * 8;
+        if (!live) {
 #pragma unroll
-        for (int ks = 0; ks < KD; ks++) {
-            const size_t at = row * a.q_stride + (size_t)head * d + ks * 32 + grp * 8;
-            if (!live) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[ks][j] = 0.0f;
-            } else if constexpr (F32) {
-                const float* p = static_cast<const float*>(a.q) + at;
-                if (a.vec & 1) {
-                    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-                    v[ks][0] = x.x; v[ks][1] = x.y; v[ks][2] = x.z; v[ks][3] = x.w;
-                    v[ks][4] = y.x; v[ks][5] = y.y; v[ks][6] = y.z; v[ks][7] = y.w;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[ks][j] = p[j];
-                }
+            for (int j = 0; j < 8; j++) v[j] = 0.0f;
+        } else if constexpr (F32) {
+            const float* p = static_cast<const float*>(a.q) + at;
+            if (a.vec & 1) {
+                const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
             } else {
-                const uint16_t* p = static_cast<const uint16_t*>(a.q) + at;
-                if (a.vec & 1) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(p);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[ks][j] = __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[ks][j] = bf16_bits_to_f32(p[j]);
-                }
+                for (int j = 0; j < 8; j++) v[j] = p[j];
             }
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(a.q) + at;
+            if (a.vec & 1) {
+                const uint4 u = *reinterpret_cast<const uint4*>(p);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[ks][j]));
+                for (int j = 0; j < 8; j++) v[j] = __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = bf16_bits_to_f32(p[j]);
+            }
         }
-        top = entry_max(top);
-        const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);
-        const float up = ldexpf(1.0f, 14 - ex);
-#pragma unroll
-        for (int ks = 0; ks < KD; ks++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float x = v[ks][j] * up;
-                qh[ks][j] = (_Float16)x;
-                if constexpr (F32) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
-            }
-        factor = ldexpf(RULES ? a.scale : a.scale * LOG2E, ex - 14);
     }
     const float slope = RULES && a.slopes && live ? a.slopes[head] : 0.0f;
+    const uint32_t steps = b1 > b0 + wave ? (b1 - b0 - wave + NW - 1) / NW : 0;  // of this wave: blocks b0 + wave, + NW, ...
+    // Where the wave's blocks lie, and their scales: for 64 of them at a time, a lane a block. A block's number and scales as scalars, one
+    // block ahead of its use; a block of no page reads the cache's first (nothing is made of it).
+    int32_t at = -1;
+    float ksc = 0.0f, lvs = 0.0f;
+    auto page_of = [&](uint32_t t) { return t + lane < steps ? kv_page(a.b, a.kv, (int32_t)s, kv_span_block(span, b0 + wave + (t + lane) * NW)) : -1; };
+    auto scales_of = [&](uint32_t t, int32_t page) {
+        float vsc = 1.0f;
+        at = -1;
+        if (page >= 0) {
+            at = (int32_t)kv_block_index(a.kv, page, kvh, kv_span_block(span, b0 + wave + (t + lane) * NW));
+            ksc = a.kv.k_scale[at];
+            vsc = a.kv.v_scale[at];
+        }
+        return vsc;
+    };
+    auto locate = [&](uint32_t t, int32_t& where, float& ks_b, float& lv) {
+        if ((t & 63) == 0) lvs = __builtin_amdgcn_logf(scales_of(t, page_of(t)));  // (log2)
+        const uint32_t from = t & 63;
+        where = __builtin_amdgcn_readlane(at, from);
+        ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), from));
+        lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), from));
+    };
+    auto request = [&](const uint8_t* codes, int32_t where, uint4* to) {
+        const gbytes p = as_global(codes + (size_t)(uint32_t)max(where, 0) * (KV_BLOCK * d)) + lane * 16;
+#pragma unroll
+        for (int x = 0; x < KD; x++) to[x] = gload<uint4>(p + x * 1024);
+    };
+    const int32_t page0 = page_of(0);
+    if (wave < KD) {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[j]));
+        top = entry_max(top);
+        if (lane < 16) top_s[wave][lane] = top;
+    }
+    __syncthreads();
+    uint4 kq[KD], vq[KD];
+    const float vsc0 = scales_of(0, page0);
+    int32_t where = __builtin_amdgcn_readlane(at, 0);
+    request(a.kv.k, where, kq);
+    float top = top_s[0][n];
+#pragma unroll
+    for (int ks = 1; ks < KD; ks++) top = fmaxf(top, top_s[ks][n]);
+    const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);  // (scaled to 2^14 at most)
+    const float factor = ldexpf(RULES ? a.scale : a.scale * LOG2E, ex - 14);     // of a score, with the key scale: natural units where RULES, else times log2 e
+    if (wave < KD) {
+        const float up = ldexpf(1.0f, 14 - ex);
+        half8 hi8, lo8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float x = v[j] * up;
+            hi8[j] = (_Float16)x;
+            if constexpr (F32) lo8[j] = (_Float16)(x - (float)hi8[j]);
+        }
+        q_s[0][wave][lane] = hi8;
+        if constexpr (F32) q_s[PLANES - 1][wave][lane] = lo8;
+    }
+    __syncthreads();
 
     f32x4 acc[2 * KD];
 #pragma unroll
     for (int t = 0; t < 2 * KD; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = NO_MAX, l = 0.0f;
-    const uint32_t steps = b1 > b0 + wave ? (b1 - b0 - wave + NW - 1) / NW : 0;  // of this wave: blocks b0 + wave, + NW, ...
-    for (uint32_t t0 = 0; t0 < steps; t0 += 64) {
-        // where the next 64 blocks lie, and their scales: one request each, a lane a block
-        int64_t at = -1;
-        float ksc = 0.0f, vsc = 0.0f;
-        if (t0 + lane < steps) {
-            const uint32_t blk = kv_span_block(span, b0 + wave + (t0 + lane) * NW);
-            const int32_t page = kv_page(a.b, a.kv, s, blk);
-            if (page >= 0) {
-                at = (int64_t)kv_block_index(a.kv, page, kvh, blk);
-                ksc = a.kv.k_scale[at];
-                vsc = a.kv.v_scale[at];
-            }
-        }
-        const float lvs = __builtin_amdgcn_logf(vsc);  // (log2)
-        const uint32_t many = min(steps - t0, 64u);
-        for (uint32_t t = 0; t < many; t++) {
-            const uint32_t blk = kv_span_block(span, b0 + wave + (t0 + t) * NW);
+    // keys are on request from the block before, values from before the scores
+    if (steps) {
+        lvs = __builtin_amdgcn_logf(vsc0);
+        int32_t where_next;
+        float ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), 0)), lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), 0)), ks_next, lv_next;
+        for (uint32_t t = 0; t < steps; t++) {
+            const uint32_t blk = kv_span_block(span, b0 + wave + t * NW);
             const int32_t k0 = (int32_t)(blk * KV_BLOCK);
-            const int64_t where = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), t) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)at, t));
-            if (where < 0) {  // no page of the cache: rows that would see it come out as NaN
-                if ((k0 < hi && k0 + (int32_t)KV_BLOCK > lo) || k0 < pre) l = __builtin_nanf("");
-                continue;
-            }
-            const float ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), t)), lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), t));
-            const gbytes kp = as_global(a.kv.k + (size_t)where * (KV_BLOCK * d)) + lane * 16, vp = as_global(a.kv.v + (size_t)where * (KV_BLOCK * d)) + lane * 16;
-            uint4 kq[KD], vq[KD];
-#pragma unroll
-            for (int x = 0; x < KD; x++) kq[x] = gload<uint4>(kp + x * 1024);
-#pragma unroll
-            for (int x = 0; x < KD; x++) vq[x] = gload<uint4>(vp + x * 1024);
+            request(a.kv.v, where, vq);
+            asm volatile("" ::: "memory");  // (the queries are to be read anew, not kept)
             f32x4 sc[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int x = 0; x < KD; x++) {
                 const half8 k_lo = code_values(kq[x].x, kq[x].y), k_hi = code_values(kq[x].z, kq[x].w);
-                sc[0] = mma(k_lo, qh[x], sc[0]);
-                sc[1] = mma(k_hi, qh[x], sc[1]);
-                if constexpr (F32) {
-                    sc[0] = mma(k_lo, ql[x], sc[0]);
-                    sc[1] = mma(k_hi, ql[x], sc[1]);
+#pragma unroll
+                for (int plane = 0; plane < PLANES; plane++) {
+                    const half8 q = q_s[plane][x][lane];
+                    sc[0] = mma(k_lo, q, sc[0]);
+                    sc[1] = mma(k_hi, q, sc[1]);
                 }
             }
+            const bool none = where < 0;
+            where_next = where;
+            ks_next = ks_b;
+            lv_next = lv;
+            if (t + 1 < steps) locate(t + 1, where_next, ks_next, lv_next);
+            request(a.kv.k, where_next, kq);
+            // no page of the cache: rows that would see it come out as NaN
+            l = none && ((k0 < hi && k0 + (int32_t)KV_BLOCK > lo) || k0 < pre) ? __builtin_nanf("") : l;
             // scores: of keys k0 + 4 grp + r and k0 + 16 + 4 grp + r
             const float f = factor * ks_b;
-            float x[8];
+            float x[8];  // scores times log2 e; without rules, what the products gave: their factor is above 0 and joins the exponent
             const int32_t own = k0 + 4 * (int32_t)grp;
 #pragma unroll
             for (int r = 0; r < 8; r++) {
-                x[r] = sc[r >> 2][r & 3] * f;
+                x[r] = sc[r >> 2][r & 3];
                 if constexpr (RULES) {
+                    x[r] *= f;
                     if (a.cap > 0.0f) x[r] = a.cap * tanh_of(x[r] / a.cap);
                     x[r] -= slope * fabsf((float)(pos - (own + 16 * (r >> 2) + (r & 3))));
                     x[r] *= LOG2E;
@@ -243,6 +366,7 @@ __global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
                 }
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if constexpr (!RULES) top *= f;
             if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM))) {
                 const float to = fmaxf(m, entry_max(top) + lv), down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
@@ -255,7 +379,7 @@ __global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
             float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 8; r++) {
-                const float p = __builtin_amdgcn_exp2f(x[r] + shift);
+                const float p = __builtin_amdgcn_exp2f(RULES ? x[r] + shift : fmaf(x[r], f, shift));
                 sum += p;
                 ph[r] = (_Float16)p;
                 if constexpr (F32) pl[r] = (_Float16)(p - (float)ph[r]);
@@ -271,9 +395,13 @@ __global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
                     acc[2 * c + 1] = mma(v_hi, pl, acc[2 * c + 1]);
                 }
             }
+            where = where_next;
+            ks_b = ks_next;
+            lv = lv_next;
         }
     }
     // the waves' parts meet
+    anew();
     l = entry_sum(l);
     if (lane < 16) {
         m_s[wave][lane] = m;
@@ -292,82 +420,140 @@ __global__ __launch_bounds__(512) void attend_split_kernel(AttendArgs a) {
         if constexpr (F32) static_cast<float*>(a.out)[to] = x;
         else static_cast<uint16_t*>(a.out)[to] = f32_to_bf16_bits(x);
     };
+    // [cols][d], then the maxima, then the sums: a workgroup's part of a tile that it begins (slot 1) or goes on with (slot 0)
     const size_t stride = (size_t)a.cols * (d + 2);
-    float* mine = a.partial + ((size_t)pair * a.splits + split) * stride;  // [cols][d], then the maxima, then the sums
+    float* mine_part = a.partial + ((size_t)blockIdx.x * 2 + (x0 == 0)) * stride;
     {
         float top, sum;
         meet(n, top, sum);
-        const float down = __builtin_amdgcn_exp2f(m - top);
+        const float whole = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees nothing: zeros)
+        const float down = __builtin_amdgcn_exp2f(m - top) * (active == 1 ? whole : 1.0f);
 #pragma unroll
         for (int c = 0; c < 2 * KD; c++) acc[c] *= down;
         if (active > 1 && wave == 0 && lane < cols) {
-            __hip_atomic_store(mine + (size_t)a.cols * d + lane, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(mine + (size_t)a.cols * (d + 1) + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(mine_part + (size_t)a.cols * d + lane, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(mine_part + (size_t)a.cols * (d + 1) + lane, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
+    auto exchange = [&](auto rows, auto channels) {  // so many entries and channels at a time
+        constexpr uint32_t ROWS = decltype(rows)::value, C = decltype(channels)::value;
+        float* r = lds;  // [NW][ROWS][C + 1]
 #pragma unroll
-    for (uint32_t c0 = 0; c0 < d; c0 += CHUNK) {
+        for (uint32_t c0 = 0; c0 < d; c0 += C) {
+            if (c0) __syncthreads();
+            if (n < ROWS) {
 #pragma unroll
-        for (uint32_t c = 0; c < CHUNK / 16; c++)
-            if (c0 / 16 + c < 2 * KD)
+                for (uint32_t c = 0; c < C / 16; c++)
+                    if (c0 / 16 + c < 2 * KD)
 #pragma unroll
-                for (int r = 0; r < 4; r++) red[wave][n][c * 16 + grp * 4 + r] = acc[c0 / 16 + c < 2 * KD ? c0 / 16 + c : 0][r];
-        __syncthreads();
-        for (uint32_t idx = tid; idx < cols * CHUNK; idx += NW * 64) {
-            const uint32_t entry = idx / CHUNK, c = idx % CHUNK;
-            if (c0 + c < d) {
+                        for (int x = 0; x < 4; x++) r[(wave * ROWS + n) * (C + 1) + c * 16 + grp * 4 + x] = acc[c0 / 16 + c < 2 * KD ? c0 / 16 + c : 0][x];
+            }
+            __syncthreads();
+            for (uint32_t idx = tid; idx < cols * C; idx += NW * 64) {
+                const uint32_t entry = idx / C, c = idx % C;
+                if (c0 + c >= d) continue;
                 float x = 0.0f;
-                for (int w = 0; w < NW; w++) x += red[w][entry][c];
-                if (active > 1) {
-                    __hip_atomic_store(mine + (size_t)entry * d + c0 + c, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                } else {
-                    float top, sum;
-                    meet(entry, top, sum);
-                    store(entry, c0 + c, sum == 0.0f ? 0.0f : x / sum);  // (a row that sees nothing: zeros)
-                }
+#pragma unroll
+                for (int w = 0; w < NW; w++) x += r[(w * ROWS + entry) * (C + 1) + c];
+                if (active > 1) __hip_atomic_store(mine_part + (size_t)entry * d + c0 + c, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                else store(entry, c0 + c, x);
             }
         }
-        __syncthreads();
-    }
-    if (active == 1) return;
-    // The splits' parts meet through memory: the last workgroup to arrive adds them, in their order; the counter returns to zero for the next
+    };
+    if (cols <= 4) exchange(std::integral_constant<uint32_t, 4>{}, std::integral_constant<uint32_t, d>{});
+    else exchange(std::integral_constant<uint32_t, 16>{}, std::integral_constant<uint32_t, CHUNK>{});
+    if (active == 1) continue;
+    // The parts meet through memory: the last workgroup to arrive adds them, in their order; the counter returns to zero for the next
     // launch. (Device-scope accesses throughout and a wait for this thread's stores before the arrival: no cache is written back or emptied.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-        const uint32_t seen = __hip_atomic_fetch_add(&a.counters[(size_t)pair * CTR_STRIDE], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t seen = __hip_atomic_fetch_add(&a.counters[(size_t)first_wg * CTR_STRIDE], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         last_s = seen == active - 1;
-        if (seen == active - 1) __hip_atomic_store(&a.counters[(size_t)pair * CTR_STRIDE], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (seen == active - 1) __hip_atomic_store(&a.counters[(size_t)first_wg * CTR_STRIDE], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!last_s) return;
-    const float* all = a.partial + (size_t)pair * a.splits * stride;
-    auto get = [&](size_t at) { return __hip_atomic_load(all + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    for (uint32_t idx = tid; idx < cols * d; idx += NW * 64) {
-        const uint32_t entry = idx / d;
-        float top = NO_MAX;
-        for (uint32_t z = 0; z < active; z++) top = fmaxf(top, get(z * stride + (size_t)a.cols * d + entry));
-        float x = 0.0f, sum = 0.0f;
-        for (uint32_t z = 0; z < active; z++) {
-            const float w = __builtin_amdgcn_exp2f(get(z * stride + (size_t)a.cols * d + entry) - top);
-            sum += w * get(z * stride + (size_t)a.cols * (d + 1) + entry);
-            x += w * get(z * stride + idx);
+    if (!last_s) continue;
+    anew();
+    const float* all = a.partial + (size_t)first_wg * 2 * stride;  // part z: 2 z strides from here, the first one's one further
+    float* weight = lds;                        // [16][MOST_SPLITS]: what a split's part counts
+    float* sums = lds + 16 * MOST_SPLITS;       // [512][2]
+    for (uint32_t entry = wave; entry < cols; entry += NW) {  // an entry a wave, a split a lane
+        float mz[MOST_SPLITS / 64], lz[MOST_SPLITS / 64], top = NO_MAX, sum = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < MOST_SPLITS / 64; i++) {
+            const uint32_t z = min(lane + 64 * i, active - 1);
+            const size_t part = (size_t)(z ? 2 * z : 1) * stride;
+            mz[i] = __hip_atomic_load(all + part + (size_t)a.cols * d + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            lz[i] = __hip_atomic_load(all + part + (size_t)a.cols * (d + 1) + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        store(entry, idx % d, sum == 0.0f ? 0.0f : x / sum);
+#pragma unroll
+        for (uint32_t i = 0; i < MOST_SPLITS / 64; i++) top = fmaxf(top, mz[i]);
+#pragma unroll
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+#pragma unroll
+        for (uint32_t i = 0; i < MOST_SPLITS / 64; i++) {
+            mz[i] = __builtin_amdgcn_exp2f(mz[i] - top);
+            sum += lane + 64 * i < active ? mz[i] * lz[i] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+#pragma unroll
+        for (uint32_t i = 0; i < MOST_SPLITS / 64; i++)
+            if (lane + 64 * i < active) weight[entry * MOST_SPLITS + lane + 64 * i] = sum == 0.0f ? 0.0f : mz[i] / sum;
     }
+    __syncthreads();
+    // two channels a thread, and the splits in as many groups as there are threads for
+    const uint32_t twos = cols * d / 2, groups = max(1u, (uint32_t)(NW * 64) / twos);
+    for (uint32_t i0 = 0; i0 < twos; i0 += NW * 64) {
+        const uint32_t idx = groups > 1 ? tid % twos : i0 + tid, group = groups > 1 ? tid / twos : 0u, entry = idx * 2 / d;
+        float y0 = 0.0f, y1 = 0.0f;
+        if (idx < twos && group < groups) {
+            const uint32_t z0 = active * group / groups, z1 = active * (group + 1) / groups;
+            const uint64_t* p = reinterpret_cast<const uint64_t*>(all) + idx;  // (a part begins at a multiple of 8 bytes)
+            for (uint32_t z = z0; z < z1; z += 8) {
+                uint64_t v[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    const uint32_t zi = min(z + i, z1 - 1);
+                    v[i] = __hip_atomic_load(p + (size_t)(zi ? 2 * zi : 1) * (stride / 2), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    const float w = z + i < z1 ? weight[entry * MOST_SPLITS + min(z + i, z1 - 1)] : 0.0f;
+                    y0 = fmaf(w, __uint_as_float((uint32_t)v[i]), y0);
+                    y1 = fmaf(w, __uint_as_float((uint32_t)(v[i] >> 32)), y1);
+                }
+            }
+        }
+        if (groups > 1) {
+            sums[2 * tid] = y0;
+            sums[2 * tid + 1] = y1;
+            __syncthreads();
+            for (uint32_t j = 1; j < groups && tid < twos; j++) {
+                y0 += sums[2 * (tid + j * twos)];
+                y1 += sums[2 * (tid + j * twos) + 1];
+            }
+        }
+        if (idx < twos && group == 0) {
+            store(entry, idx * 2 % d, y0);
+            store(entry, idx * 2 % d + 1, y1);
+        }
+    }
+  }
 }
 
 template <bool F32, bool RULES>
 static hipError_t launch_split(const AttendArgs& a, dim3 grid, hipStream_t s) {
     switch (a.kv.d / 32) {
-        case 1: attend_split_kernel<1, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 2: attend_split_kernel<2, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 3: attend_split_kernel<3, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 4: attend_split_kernel<4, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 5: attend_split_kernel<5, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 6: attend_split_kernel<6, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        case 7: attend_split_kernel<7, F32, RULES><<<grid, 512, 0, s>>>(a); break;
-        default: attend_split_kernel<8, F32, RULES><<<grid, 512, 0, s>>>(a); break;
+        case 1: attend_split_kernel<1, F32, RULES><<<grid, 64 * split_waves(1), 0, s>>>(a); break;
+        case 2: attend_split_kernel<2, F32, RULES><<<grid, 64 * split_waves(2), 0, s>>>(a); break;
+        case 3: attend_split_kernel<3, F32, RULES><<<grid, 64 * split_waves(3), 0, s>>>(a); break;
+        case 4: attend_split_kernel<4, F32, RULES><<<grid, 64 * split_waves(4), 0, s>>>(a); break;
+        case 5: attend_split_kernel<5, F32, RULES><<<grid, 64 * split_waves(5), 0, s>>>(a); break;
+        case 6: attend_split_kernel<6, F32, RULES><<<grid, 64 * split_waves(6), 0, s>>>(a); break;
+        case 7: attend_split_kernel<7, F32, RULES><<<grid, 64 * split_waves(7), 0, s>>>(a); break;
+        default: attend_split_kernel<8, F32, RULES><<<grid, 64 * split_waves(8), 0, s>>>(a); break;
     }
     return hipGetLastError();
 }
@@ -392,19 +578,17 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.window = call.window;
     const size_t size = call.bf16 ? 2 : 4;
     a.vec = reinterpret_cast<uintptr_t>(call.q) % 16 == 0 && call.q_stride * size % 16 == 0 ? 1u : 0u;
-    const uint64_t tiles = b.row_start ? kv_places((uint64_t)b.rows * a.g, b.n_seqs, 16, 1) : (uint64_t)b.n_seqs * ((a.g + 15) / 16);
     a.cols = b.row_start ? 16u : min(16u, a.g);
-    // splits of a tile's keys: enough workgroups for the chip, as far as a table's longest sequence gives each wave a block and the scratch
-    // holds their parts
-    const uint64_t pairs = tiles * kv.n_kv, most = ((uint64_t)b.max_pages << kv.shift) / 8;
-    uint64_t splits = 1024 / pairs;
-    splits = splits < most ? splits : most;
-    const uint64_t room = sc.partial_floats / (pairs * a.cols * (kv.d + 2));
-    splits = splits < room ? splits : room;
-    if (pairs * CTR_STRIDE > sc.ncounters || splits < 1) splits = 1;
-    a.splits = (uint32_t)splits;
-    if (pairs * splits > 0x7FFFFFFFu) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(pairs * splits));
+    // as many workgroups as the chip has CUs, unless there is not that much to share
+    uint64_t many = MOST_SPLITS;
+    const uint64_t tiles = b.row_start ? kv_places((uint64_t)b.rows * a.g, b.n_seqs, 16, 1) : (uint64_t)b.n_seqs * ((a.g + 15) / 16);
+    const uint64_t most = (uint64_t)b.max_pages << kv.shift;
+    a.quantum = kv_quantum(tiles * kv.n_kv, most);
+    if (!a.quantum) return hipErrorInvalidValue;
+    const uint64_t weight = tiles * kv.n_kv * ((most + a.quantum - 1) / a.quantum);
+    if (weight < many) many = weight;
+    if (many > MOST_SPLITS || many * CTR_STRIDE > sc.ncounters || many * 2 * a.cols * (kv.d + 2) > sc.partial_floats) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)many);
     const bool rules = call.cap > 0.0f || call.slopes || !(call.scale >= 0x1p-10f && call.scale <= 0x1p40f);
     if (call.bf16) return rules ? launch_split<false, true>(a, grid, s) : launch_split<false, false>(a, grid, s);
     return rules ? launch_split<true, true>(a, grid, s) : launch_split<true, false>(a, grid, s);

@@ -34,6 +34,7 @@ const char* check(const oxhip_kv_cache* kv, const oxhip_kv_batch* b, KvView* kvv
     if (!b->row_start && b->rows != b->n_seqs) return "without row_start, every sequence has one row";
     uint32_t shift = 0;
     while (((size_t)KV_BLOCK << shift) < page) shift++;
+    if (kv->n_pages > (((size_t)0x7FFFFFFFu / kv->n_kv) >> shift)) return "a cache has fewer than 2^31 blocks";
     *kvv = KvView{kv->k, kv->v, kv->k_scale, kv->v_scale, (uint32_t)kv->n_pages, (uint32_t)kv->n_kv, (uint32_t)kv->d, shift};
     *bv = KvBatchView{b->row_start, b->kv_len, b->pages, (uint32_t)b->n_seqs, (uint32_t)b->rows, (uint32_t)b->max_pages};
     return nullptr;

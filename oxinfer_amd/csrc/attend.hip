@@ -33,12 +33,12 @@ struct AttendArgs {
     float* partial;
     uint32_t* counters;
     float scale, cap;
-    uint32_t n_q, g, window, cols, vec, quantum;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
+    uint32_t n_q, g, window, cols, vec, quantum, many, least;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from it that 2^(NO_MAX - score) is 0
-constexpr uint32_t MOST_SPLITS = 256;  // workgroups of a launch, and so of a tile
+constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
 
 // Eight codes as f16 values, exactly.
@@ -106,12 +106,22 @@ __device__ __forceinline__ float tanh_of(float x) {
 // A value that all lanes hold alike, as a scalar.
 __device__ __forceinline__ uint32_t scalar(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-// Waves of a workgroup: as many as its registers leave room for on a CU, where a workgroup is alone.
-constexpr int split_waves(int kd) { return kd <= 4 ? 16 : 8; }
+// a / b of values below 2^31, mostly small ones: by the hardware's reciprocal where its error is less than one (a lone wave takes a microsecond for
+// four divisions of the general kind).
+__device__ __forceinline__ uint32_t divide(uint32_t a, uint32_t b) {
+    if (a >= 1u << 22) return a / b;
+    const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const int32_t r = (int32_t)(a - q * b);
+    return r < 0 ? q - 1 : r >= (int32_t)b ? q + 1 : q;
+}
+
+// Waves of a workgroup, and workgroups on a CU.
+constexpr int split_waves(int) { return 8; }
+constexpr int split_places(int kd) { return kd <= 4 ? 2 : 1; }
 
 // KD = d / 32; F32: f32 rows; RULES: capped or biased scores, or a factor outside the range that the plain path takes.
 template <int KD, bool F32, bool RULES>
-__global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void attend_split_kernel(AttendArgs a) {
     constexpr int NW = split_waves(KD), PLANES = F32 ? 2 : 1, CHUNK = KD >= 2 ? 64 : 32;  // channels whose sums the waves exchange at a time
     constexpr int RED = NW * 16 * (CHUNK + 1) > NW * 4 * (KD * 32 + 1) ? NW * 16 * (CHUNK + 1) : NW * 4 * (KD * 32 + 1), JOIN = 16 * MOST_SPLITS + NW * 128;
     __shared__ __align__(16) float lds[RED > JOIN ? RED : JOIN];
@@ -131,75 +141,70 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
         grp = lane >> 4;
     };
 
-    // This workgroup's share: all tiles' weights (kv_weight) lie one after the other, sequence by sequence, tile by tile, a tile's key heads
-    // together; every workgroup takes as much of them. A wave adds them up, a lane a sequence, 64 sequences at a time, for the others too: what
-    // decides how many barriers a wave passes is read once.
+    // Which tile, and which part of its blocks, is this workgroup's (kv_weight): a wave adds the sequences' weights up, a lane a sequence, 64 of them
+    // at a time, for the others too, so that what decides how many barriers a wave passes is read once.
     __shared__ int32_t seq_s[4][64];
-    __shared__ uint32_t upto_s[64];
-    KvSeq mine{};              // the lane's sequence of the 64 from s0 on
-    uint32_t mine_blocks, mine_upto, s0 = 0;  // its tiles' weight each; the weights of the lanes up to it
+    KvSeq mine{};                              // the lane's sequence of the 64 from s0 on
+    uint32_t mine_weight, mine_units, s0 = 0;  // its tiles' weight each; its tiles x key heads
     auto load = [&](uint32_t from) {
         s0 = from;
         __syncthreads();
         if (wave == 0) {
-            uint32_t all = 0;
-            mine_blocks = 1;
+            KvSeq q{};
+            uint32_t w = 1;
             if (s0 + lane < a.b.n_seqs) {
-                mine = kv_seq(a.b, (int32_t)(s0 + lane), a.kv.shift);
-                mine_blocks = kv_weight(mine, a.window, a.window && a.prefix ? a.prefix[s0 + lane] : 0, a.quantum);
-                all = kv_tiles(mine, g) * a.kv.n_kv * mine_blocks;
+                q = kv_seq(a.b, (int32_t)(s0 + lane), a.kv.shift);
+                w = kv_weight(q, a.window, a.window && a.prefix ? a.prefix[s0 + lane] : 0, a.quantum);
             }
-            seq_s[0][lane] = mine.row0;
-            seq_s[1][lane] = mine.n;
-            seq_s[2][lane] = mine.len;
-            seq_s[3][lane] = (int32_t)mine_blocks;
-            upto_s[lane] = lanes_upto(all);
+            seq_s[0][lane] = q.row0;
+            seq_s[1][lane] = q.n;
+            seq_s[2][lane] = q.len;
+            seq_s[3][lane] = (int32_t)w;
         }
         __syncthreads();
         mine.row0 = seq_s[0][lane];
         mine.n = seq_s[1][lane];
         mine.len = seq_s[2][lane];
-        mine_blocks = (uint32_t)seq_s[3][lane];
-        mine_upto = upto_s[lane];
-        return (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, 63);
+        mine_weight = (uint32_t)seq_s[3][lane];
+        mine_units = kv_tiles(mine, g) * a.kv.n_kv;
     };
+    auto last = [&](uint32_t upto) { return (uint32_t)__builtin_amdgcn_readlane((int)upto, 63); };
     uint32_t total = 0;
-    for (uint32_t from = 0; from < a.b.n_seqs; from += 64) total += load(from);
-    const uint32_t size = max((total + gridDim.x - 1) / gridDim.x, 1u), share0 = blockIdx.x * size, share1 = min(share0 + size, total);
-    if (share0 >= share1 || total <= share0) return;
-    uint32_t s_at = 0;  // where the weights of the 64 sequences in the lanes begin
-    if (a.b.n_seqs > 64) {
-        uint32_t here = load(0);
-        while (s_at + here <= share0) {
-            if (s0 + 64 >= a.b.n_seqs) return;
-            s_at += here;
-            here = load(s0 + 64);
+    for (uint32_t from = 0; from < a.b.n_seqs; from += 64) {
+        load(from);
+        total += last(lanes_upto(mine_units * mine_weight));
+    }
+    const uint32_t size = max(scalar(divide(total + a.many - 1, a.many)), a.least);
+    uint32_t at_wg = 0, at_part = 0;  // workgroups, and parts that workgroups leave for each other, of the sequences before these 64
+    uint32_t k, upto, parts_upto, from;
+    if (a.b.n_seqs > 64) load(0);
+    for (;;) {
+        k = divide(mine_weight + size - 1, size);
+        upto = lanes_upto(mine_units * k);
+        parts_upto = lanes_upto(k > 1 ? mine_units * k : 0);
+        const uint64_t behind = __ballot(at_wg + upto > blockIdx.x);  // sequences that end behind this workgroup
+        if (behind) {
+            from = (uint32_t)__builtin_ctzll(behind);
+            break;
         }
-    }
-  for (uint32_t place = share0; place < share1;) {
-    uint64_t behind = __ballot(s_at + mine_upto > place);  // sequences that end behind the place
-    while (!behind) {
         if (s0 + 64 >= a.b.n_seqs) return;
-        s_at += (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, 63);
+        at_wg += last(upto);
+        at_part += last(parts_upto);
         load(s0 + 64);
-        behind = __ballot(s_at + mine_upto > place);
     }
-    const uint32_t from = (uint32_t)__builtin_ctzll(behind), s = s0 + from;
+    const uint32_t s = s0 + from, active = (uint32_t)__builtin_amdgcn_readlane((int)k, from);  // workgroups that share a tile
     const KvSeq seq{(int32_t)s, __builtin_amdgcn_readlane(mine.row0, from), __builtin_amdgcn_readlane(mine.n, from), __builtin_amdgcn_readlane(mine.len, from)};
-    const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane((int)mine_blocks, from);
-    const uint32_t seq_at = s_at + (from ? (uint32_t)__builtin_amdgcn_readlane((int)mine_upto, from - 1) : 0u);
-    const uint32_t unit = (place - seq_at) / blocks, unit_at = seq_at + unit * blocks;
-    const uint32_t x0 = place - unit_at, x1 = min(blocks, share1 - unit_at);
-    const int32_t tile = (int32_t)(unit / a.kv.n_kv);
+    const uint32_t units = (uint32_t)__builtin_amdgcn_readlane((int)mine_units, from);
+    const uint32_t own = blockIdx.x - (at_wg + (uint32_t)__builtin_amdgcn_readlane((int)upto, from) - units * active);  // of the sequence's workgroups
+    const uint32_t unit = scalar(divide(own, active)), part = own - unit * active;
+    const int32_t tile = (int32_t)scalar(divide(unit, a.kv.n_kv));
     const uint32_t kvh = unit - (uint32_t)tile * a.kv.n_kv;
-    place = unit_at + x1;
-    const uint32_t first_wg = x0 ? unit_at / size : blockIdx.x, active = (unit_at + blocks - 1) / size - first_wg + 1;  // workgroups that share this tile
-    __syncthreads();  // (what the tile before left in LDS has been read)
-    anew();
+    // (where the tile's parts lie in the scratch)
+    const uint32_t first_part = active > 1 ? at_part + (uint32_t)__builtin_amdgcn_readlane((int)parts_upto, from) - (units - unit) * active : 0;
     const int64_t entries = (int64_t)seq.n * g;
     const uint32_t e = (uint32_t)tile * 16 + n, cols = (uint32_t)min((int64_t)16, entries - (int64_t)tile * 16);
     const bool live = n < cols;
-    const uint32_t i = live ? e / g : 0u, head = kvh * g + (live ? e % g : 0u);
+    const uint32_t i = live ? divide(e, g) : 0u, head = kvh * g + (live ? e - i * g : 0u);
     const size_t row = (size_t)seq.row0 + i;
     const int32_t pos = seq.len - seq.n + (int32_t)i;
 
@@ -215,7 +220,7 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
     const int32_t lo_min = tile_min(hi > lo ? lo : INT32_MAX), hi_max = tile_max(hi), lo_max = tile_max(live ? lo : 0), hi_min = tile_min(live ? hi : INT32_MAX);
     const int32_t pre_max = tile_max(pre);
     const KvSpan span = kv_span(pre_max, lo_min, hi_max);
-    const uint32_t b0 = x0 ? (uint32_t)((uint64_t)span.count * x0 / blocks) : 0u, b1 = x1 < blocks ? (uint32_t)((uint64_t)span.count * x1 / blocks) : span.count;
+    const uint32_t b0 = part ? (uint32_t)((uint64_t)span.count * part / active) : 0u, b1 = part + 1 < active ? (uint32_t)((uint64_t)span.count * (part + 1) / active) : span.count;
 
     // The entry's query as operands: in LDS, where all waves read it for each block (kept in registers, it would cost a wave in two its place on
     // the CU). Wave ks brings the channels 32 ks .. 32 ks + 31. What depends on memory goes in an order that keeps the chain short: queries and
@@ -315,7 +320,7 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
     for (int t = 0; t < 2 * KD; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = NO_MAX, l = 0.0f;
     // keys are on request from the block before, values from before the scores
-    if (steps) {
+    {
         lvs = __builtin_amdgcn_logf(vsc0);
         int32_t where_next;
         float ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), 0)), lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), 0)), ks_next, lv_next;
@@ -346,14 +351,14 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
             // scores: of keys k0 + 4 grp + r and k0 + 16 + 4 grp + r
             const float f = factor * ks_b;
             float x[8];  // scores times log2 e; without rules, what the products gave: their factor is above 0 and joins the exponent
-            const int32_t own = k0 + 4 * (int32_t)grp;
+            const int32_t key0 = k0 + 4 * (int32_t)grp;
 #pragma unroll
             for (int r = 0; r < 8; r++) {
                 x[r] = sc[r >> 2][r & 3];
                 if constexpr (RULES) {
                     x[r] *= f;
                     if (a.cap > 0.0f) x[r] = a.cap * tanh_of(x[r] / a.cap);
-                    x[r] -= slope * fabsf((float)(pos - (own + 16 * (r >> 2) + (r & 3))));
+                    x[r] -= slope * fabsf((float)(pos - (key0 + 16 * (r >> 2) + (r & 3))));
                     x[r] *= LOG2E;
                 }
             }
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
             if (!((k0 >= lo_max && end <= hi_min) || end <= pre_max)) {
 #pragma unroll
                 for (int r = 0; r < 8; r++) {
-                    const int32_t j = own + 16 * (r >> 2) + (r & 3);
+                    const int32_t j = key0 + 16 * (r >> 2) + (r & 3);
                     x[r] = (j >= lo && j < hi) || j < pre ? x[r] : -__builtin_inff();
                 }
             }
@@ -409,10 +414,18 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
     }
     __syncthreads();
     auto meet = [&](uint32_t entry, float& top, float& sum) {
-        top = m_s[0][entry];
-        for (int w = 1; w < NW; w++) top = fmaxf(top, m_s[w][entry]);
+        float mw[NW], lw[NW];
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            mw[w] = m_s[w][entry];
+            lw[w] = l_s[w][entry];
+        }
+        top = mw[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) top = fmaxf(top, mw[w]);
         sum = 0.0f;
-        for (int w = 0; w < NW; w++) sum += l_s[w][entry] * __builtin_amdgcn_exp2f(m_s[w][entry] - top);
+#pragma unroll
+        for (int w = 0; w < NW; w++) sum += lw[w] * __builtin_amdgcn_exp2f(mw[w] - top);
     };
     auto store = [&](uint32_t entry, uint32_t c, float x) {
         const uint32_t at = (uint32_t)tile * 16 + entry;
@@ -420,9 +433,8 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
         if constexpr (F32) static_cast<float*>(a.out)[to] = x;
         else static_cast<uint16_t*>(a.out)[to] = f32_to_bf16_bits(x);
     };
-    // [cols][d], then the maxima, then the sums: a workgroup's part of a tile that it begins (slot 1) or goes on with (slot 0)
     const size_t stride = (size_t)a.cols * (d + 2);
-    float* mine_part = a.partial + ((size_t)blockIdx.x * 2 + (x0 == 0)) * stride;
+    float* mine_part = a.partial + (size_t)(first_part + part) * stride;  // [cols][d], then the maxima, then the sums
     {
         float top, sum;
         meet(n, top, sum);
@@ -462,20 +474,20 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
     };
     if (cols <= 4) exchange(std::integral_constant<uint32_t, 4>{}, std::integral_constant<uint32_t, d>{});
     else exchange(std::integral_constant<uint32_t, 16>{}, std::integral_constant<uint32_t, CHUNK>{});
-    if (active == 1) continue;
+    if (active == 1) return;
     // The parts meet through memory: the last workgroup to arrive adds them, in their order; the counter returns to zero for the next
     // launch. (Device-scope accesses throughout and a wait for this thread's stores before the arrival: no cache is written back or emptied.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-        const uint32_t seen = __hip_atomic_fetch_add(&a.counters[(size_t)first_wg * CTR_STRIDE], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t seen = __hip_atomic_fetch_add(&a.counters[(size_t)first_part * CTR_STRIDE], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         last_s = seen == active - 1;
-        if (seen == active - 1) __hip_atomic_store(&a.counters[(size_t)first_wg * CTR_STRIDE], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (seen == active - 1) __hip_atomic_store(&a.counters[(size_t)first_part * CTR_STRIDE], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!last_s) continue;
+    if (!last_s) return;
     anew();
-    const float* all = a.partial + (size_t)first_wg * 2 * stride;  // part z: 2 z strides from here, the first one's one further
+    const float* all = a.partial + (size_t)first_part * stride;
     float* weight = lds;                        // [16][MOST_SPLITS]: what a split's part counts
     float* sums = lds + 16 * MOST_SPLITS;       // [512][2]
     for (uint32_t entry = wave; entry < cols; entry += NW) {  // an entry a wave, a split a lane
@@ -483,9 +495,8 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
 #pragma unroll
         for (uint32_t i = 0; i < MOST_SPLITS / 64; i++) {
             const uint32_t z = min(lane + 64 * i, active - 1);
-            const size_t part = (size_t)(z ? 2 * z : 1) * stride;
-            mz[i] = __hip_atomic_load(all + part + (size_t)a.cols * d + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            lz[i] = __hip_atomic_load(all + part + (size_t)a.cols * (d + 1) + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            mz[i] = __hip_atomic_load(all + z * stride + (size_t)a.cols * d + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            lz[i] = __hip_atomic_load(all + z * stride + (size_t)a.cols * (d + 1) + entry, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
 #pragma unroll
         for (uint32_t i = 0; i < MOST_SPLITS / 64; i++) top = fmaxf(top, mz[i]);
@@ -514,10 +525,7 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
             for (uint32_t z = z0; z < z1; z += 8) {
                 uint64_t v[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i++) {
-                    const uint32_t zi = min(z + i, z1 - 1);
-                    v[i] = __hip_atomic_load(p + (size_t)(zi ? 2 * zi : 1) * (stride / 2), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                for (uint32_t i = 0; i < 8; i++) v[i] = __hip_atomic_load(p + (size_t)min(z + i, z1 - 1) * (stride / 2), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++) {
                     const float w = z + i < z1 ? weight[entry * MOST_SPLITS + min(z + i, z1 - 1)] : 0.0f;
@@ -540,11 +548,10 @@ __global__ __launch_bounds__(64 * split_waves(KD)) void attend_split_kernel(Atte
             store(entry, idx * 2 % d + 1, y1);
         }
     }
-  }
 }
 
 template <bool F32, bool RULES>
-static hipError_t launch_split(const AttendArgs& a, dim3 grid, hipStream_t s) {
+static hipError_t launch_split(const AttendArgs& a, unsigned grid, hipStream_t s) {
     switch (a.kv.d / 32) {
         case 1: attend_split_kernel<1, F32, RULES><<<grid, 64 * split_waves(1), 0, s>>>(a); break;
         case 2: attend_split_kernel<2, F32, RULES><<<grid, 64 * split_waves(2), 0, s>>>(a); break;
@@ -579,19 +586,24 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     const size_t size = call.bf16 ? 2 : 4;
     a.vec = reinterpret_cast<uintptr_t>(call.q) % 16 == 0 && call.q_stride * size % 16 == 0 ? 1u : 0u;
     a.cols = b.row_start ? 16u : min(16u, a.g);
-    // as many workgroups as the chip has CUs, unless there is not that much to share
-    uint64_t many = MOST_SPLITS;
     const uint64_t tiles = b.row_start ? kv_places((uint64_t)b.rows * a.g, b.n_seqs, 16, 1) : (uint64_t)b.n_seqs * ((a.g + 15) / 16);
-    const uint64_t most = (uint64_t)b.max_pages << kv.shift;
-    a.quantum = kv_quantum(tiles * kv.n_kv, most);
+    const uint64_t units = tiles * kv.n_kv, most = (uint64_t)b.max_pages << kv.shift;  // (at most that many)
+    a.quantum = kv_quantum(units, most);
     if (!a.quantum) return hipErrorInvalidValue;
-    const uint64_t weight = tiles * kv.n_kv * ((most + a.quantum - 1) / a.quantum);
-    if (weight < many) many = weight;
-    if (many > MOST_SPLITS || many * CTR_STRIDE > sc.ncounters || many * 2 * a.cols * (kv.d + 2) > sc.partial_floats) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)many);
+    a.many = 256 * split_places((int)kv.d / 32);
+#ifdef OXHIP_TUNING
+    if (getenv("OX_MANY")) a.many = atoi(getenv("OX_MANY"));
+#endif
+    a.least = a.quantum < KV_LEAST ? KV_LEAST / a.quantum : 1;
+#ifdef OXHIP_TUNING
+    if (getenv("OX_LEAST")) a.least = atoi(getenv("OX_LEAST"));
+#endif
+    const uint64_t weight = (most + a.quantum - 1) / a.quantum, parts = (weight + a.least - 1) / a.least;  // of a tile, at most
+    uint64_t grid = units * parts < units + a.many ? units * parts : units + a.many;
+    if (a.many > MOST_SPLITS || 2 * a.many * CTR_STRIDE > sc.ncounters || 2 * (uint64_t)a.many * a.cols * (kv.d + 2) > sc.partial_floats || grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
     const bool rules = call.cap > 0.0f || call.slopes || !(call.scale >= 0x1p-10f && call.scale <= 0x1p40f);
-    if (call.bf16) return rules ? launch_split<false, true>(a, grid, s) : launch_split<false, false>(a, grid, s);
-    return rules ? launch_split<true, true>(a, grid, s) : launch_split<true, false>(a, grid, s);
+    if (call.bf16) return rules ? launch_split<false, true>(a, (unsigned)grid, s) : launch_split<false, false>(a, (unsigned)grid, s);
+    return rules ? launch_split<true, true>(a, (unsigned)grid, s) : launch_split<true, false>(a, (unsigned)grid, s);
 }
 
 }  // namespace oxhip

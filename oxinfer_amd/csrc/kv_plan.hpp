@@ -67,10 +67,11 @@ OXHIP_HD KvSpan kv_span(int64_t prefix, int64_t lo, int64_t hi) {
 }
 OXHIP_HD uint32_t kv_span_block(const KvSpan& s, uint32_t i) { return i < s.pre ? i : s.lo + (i - s.pre); }
 
-// What a tile of a sequence weighs where tiles are shared out among workgroups: the blocks that its last row can see, in quanta of
-// KV_QUANTUM blocks (more where 32 bits would not hold the weights' sum), so that a small call's shares begin and end where tiles do. (Rules that go
-// by the row are left out: a share is a part of a tile's weight, and gets that part of the blocks that the tile really has.)
-constexpr uint32_t KV_QUANTUM = 16;
+// A launch's workgroups over tiles of very different lengths: a tile of `blocks` blocks gets ceil(blocks / size) of them, size being all tiles'
+// blocks over the workgroups that the chip holds, and KV_LEAST blocks at least (a tile's parts have to meet again, which takes longer than to
+// read that many). A tile's blocks are here those that its sequence's last row can see; rules that go by the row are left out, and the parts
+// are parts of what the tile really has. Counted in quanta of blocks, 1 unless 32 bits would not hold the sum.
+constexpr uint32_t KV_LEAST = 32;
 OXHIP_HD uint32_t kv_weight(const KvSeq& q, uint32_t window, int32_t prefix, uint32_t quantum) {
     const uint32_t all = ((uint32_t)q.len + KV_BLOCK - 1) / KV_BLOCK;
     uint32_t blocks = all;
@@ -78,13 +79,13 @@ OXHIP_HD uint32_t kv_weight(const KvSeq& q, uint32_t window, int32_t prefix, uin
         const uint32_t pre = prefix > 0 ? ((uint32_t)prefix + KV_BLOCK - 1) / KV_BLOCK : 0, out = ((uint32_t)(q.len - q.n) - window + 1) / KV_BLOCK;
         blocks = pre < out ? all - out + pre : all;
     }
-    return blocks ? (blocks + quantum - 1) / quantum : 1;
+    return blocks ? (quantum == 1 ? blocks : (blocks + quantum - 1) / quantum) : 1;
 }
 OXHIP_HD uint32_t kv_tiles(const KvSeq& q, uint32_t g) { return (uint32_t)(((uint64_t)(uint32_t)q.n * g + 15) / 16); }
-// The quantum with which `tiles` tiles x heads of at most `blocks` blocks each weigh less than 2^31 in all (0: none does).
+// The quantum with which `tiles` tiles x heads of at most `blocks` blocks each come to less than 2^31 in all (0: none does).
 inline uint32_t kv_quantum(uint64_t tiles, uint64_t blocks) {
-    for (uint64_t q = KV_QUANTUM; q < ((uint64_t)1 << 31); q *= 2)
-        if (tiles * ((blocks + q - 1) / q) < ((uint64_t)1 << 31)) return (uint32_t)q;
+    for (uint64_t q = 1; q < ((uint64_t)1 << 31); q *= 2)
+        if (tiles < ((uint64_t)1 << 30) && tiles * ((blocks + q - 1) / q) < ((uint64_t)1 << 31)) return (uint32_t)q;
     return 0;
 }
 

@@ -14,106 +14,9 @@
 // bf16 rows: as one (11 bits, where the rows and results have 8); the rows are scaled by a power of two each, so that nothing overflows.
 #include <type_traits>
 
-#include "kv.hpp"
+#include "attend.hpp"
 
 namespace oxhip {
-
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-struct AttendArgs {
-    KvView kv;
-    KvBatchView b;
-    const void* q;
-    void* out;
-    size_t q_stride, out_stride;
-    const float* slopes;
-    const int32_t *prefix, *first;
-    float* partial;
-    uint32_t* counters;
-    float scale, cap;
-    uint32_t n_q, g, window, cols, vec, quantum, many, least;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
-};
-
-constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from it that 2^(NO_MAX - score) is 0
-constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
-constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
-
-// Eight codes as f16 values, exactly.
-__device__ __forceinline__ half8 code_values(uint32_t a, uint32_t b) {
-    const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    union { half2v h[4]; half8 v; } o;
-    o.h[0] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(a, 0x64646464u, 0x00050004u)) + off;
-    o.h[1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(a, 0x64646464u, 0x00070006u)) + off;
-    o.h[2] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(b, 0x64646464u, 0x00050004u)) + off;
-    o.h[3] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(b, 0x64646464u, 0x00070006u)) + off;
-    return o.v;
-}
-__device__ __forceinline__ f32x4 mma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-// Over the four lanes that hold an entry's scores, 16 apart: the largest, and the sum.
-template <class F>
-__device__ __forceinline__ float entry_fold(float v, F f) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float entry_max(float v) {
-    return entry_fold(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float entry_sum(float v) {
-    return entry_fold(v, [](float a, float b) { return a + b; });
-}
-template <int CTRL, int ROWS = 0xF>
-__device__ __forceinline__ int32_t lanes_of(int32_t v) {
-    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
-}
-// Over the 16 entries (the lanes of a row of 16), as a scalar.
-template <class F>
-__device__ __forceinline__ int32_t tile_fold(int32_t v, F f) {
-    v = f(v, lanes_of<0x128>(v));  // row_ror:8, 4, 2, 1
-    v = f(v, lanes_of<0x124>(v));
-    v = f(v, lanes_of<0x122>(v));
-    v = f(v, lanes_of<0x121>(v));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int32_t tile_min(int32_t v) {
-    return tile_fold(v, [](int32_t a, int32_t b) { return min(a, b); });
-}
-__device__ __forceinline__ int32_t tile_max(int32_t v) {
-    return tile_fold(v, [](int32_t a, int32_t b) { return max(a, b); });
-}
-// The sum of a wave's lanes up to one's own.
-__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
-    v += (uint32_t)lanes_of<0x111>((int32_t)v);  // row_shr:1, 2, 4, 8
-    v += (uint32_t)lanes_of<0x112>((int32_t)v);
-    v += (uint32_t)lanes_of<0x114>((int32_t)v);
-    v += (uint32_t)lanes_of<0x118>((int32_t)v);
-    v += (uint32_t)lanes_of<0x142, 0xA>((int32_t)v);  // row_bcast:15, then :31
-    v += (uint32_t)lanes_of<0x143, 0xC>((int32_t)v);
-    return v;
-}
-// tanh: by its series below 1/4 (the next term is 2^-27 of the value), where 1 - 2 / (e^2x + 1) cancels, and by that above.
-__device__ __forceinline__ float tanh_of(float x) {
-    const float a = fabsf(x), z = x * x;
-    const float series = x + x * z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f))));
-    const float e = __builtin_amdgcn_exp2f(2.0f * LOG2E * a);
-    return a < 0.25f ? series : copysignf(1.0f - 2.0f / (e + 1.0f), x);
-}
-
-// A value that all lanes hold alike, as a scalar.
-__device__ __forceinline__ uint32_t scalar(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-
-// a / b of values below 2^31, mostly small ones: by the hardware's reciprocal where its error is less than one (a lone wave takes a microsecond for
-// four divisions of the general kind).
-__device__ __forceinline__ uint32_t divide(uint32_t a, uint32_t b) {
-    if (a >= 1u << 22) return a / b;
-    const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
-    const int32_t r = (int32_t)(a - q * b);
-    return r < 0 ? q - 1 : r >= (int32_t)b ? q + 1 : q;
-}
 
 // Waves of a workgroup, and workgroups on a CU.
 constexpr int split_waves(int) { return 8; }
@@ -154,6 +57,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             uint32_t w = 1;
             if (s0 + lane < a.b.n_seqs) {
                 q = kv_seq(a.b, (int32_t)(s0 + lane), a.kv.shift);
+                if ((uint32_t)q.n * (uint64_t)g >= a.prompt) q.n = 0;  // (attend_prompt_kernel's)
                 w = kv_weight(q, a.window, a.window && a.prefix ? a.prefix[s0 + lane] : 0, a.quantum);
             }
             seq_s[0][lane] = q.row0;
@@ -231,27 +135,8 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
         if (!live) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = 0.0f;
-        } else if constexpr (F32) {
-            const float* p = static_cast<const float*>(a.q) + at;
-            if (a.vec & 1) {
-                const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = p[j];
-            }
         } else {
-            const uint16_t* p = static_cast<const uint16_t*>(a.q) + at;
-            if (a.vec & 1) {
-                const uint4 u = *reinterpret_cast<const uint4*>(p);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = bf16_bits_to_f32(p[j]);
-            }
+            load_query<F32>(a.q, at, a.vec & 1, v);
         }
     }
     const float slope = RULES && a.slopes && live ? a.slopes[head] : 0.0f;
@@ -584,24 +469,31 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.g = call.n_q / kv.n_kv;
     a.window = call.window;
     const size_t size = call.bf16 ? 2 : 4;
-    a.vec = reinterpret_cast<uintptr_t>(call.q) % 16 == 0 && call.q_stride * size % 16 == 0 ? 1u : 0u;
+    auto vec = [&](const void* p, size_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; };
+    a.vec = (vec(call.q, call.q_stride) ? 1u : 0u) | (vec(call.out, call.out_stride) ? 2u : 0u);
+    const bool rules = call.cap > 0.0f || call.slopes || !(call.scale >= 0x1p-10f && call.scale <= 0x1p40f);
+    // Sequences of many query entries go to the kernel that is bound by the matrix cores, those of few to this file's; which of them a batch
+    // has is known on the device alone, but where all rows together are few, or all one sequence's.
+    // It has tiles of 128 entries and takes a tile's keys one after the other, so it pays where its tiles fill the chip: 1024 rows alone or behind 8192
+    // tokens (32 heads of 128 over 8, bf16: 256 tiles) 33 and 238 us, here 45 and 306; 512 rows 21 and 208, here 22 and 155; of heads of 64 channels
+    // (8 over 4) 4096 rows 76 and 226, here 62 and 222.
+    const uint64_t all = (uint64_t)b.rows * a.g, fill = all * kv.n_kv / 128;
+    const bool prompts = b.row_start && all >= PROMPT_ENTRIES && fill >= 256 && fill * kv.d >= 256 * 128;
+    a.prompt = !prompts ? 0xFFFFFFFFu : b.n_seqs > 1 ? PROMPT_ENTRIES : 1;
+    if (prompts) {
+        const hipError_t e = launch_attend_prompt(a, call.bf16, rules, s);
+        if (e != hipSuccess || b.n_seqs == 1) return e;
+    }
     a.cols = b.row_start ? 16u : min(16u, a.g);
     const uint64_t tiles = b.row_start ? kv_places((uint64_t)b.rows * a.g, b.n_seqs, 16, 1) : (uint64_t)b.n_seqs * ((a.g + 15) / 16);
     const uint64_t units = tiles * kv.n_kv, most = (uint64_t)b.max_pages << kv.shift;  // (at most that many)
     a.quantum = kv_quantum(units, most);
     if (!a.quantum) return hipErrorInvalidValue;
     a.many = 256 * split_places((int)kv.d / 32);
-#ifdef OXHIP_TUNING
-    if (getenv("OX_MANY")) a.many = atoi(getenv("OX_MANY"));
-#endif
     a.least = a.quantum < KV_LEAST ? KV_LEAST / a.quantum : 1;
-#ifdef OXHIP_TUNING
-    if (getenv("OX_LEAST")) a.least = atoi(getenv("OX_LEAST"));
-#endif
     const uint64_t weight = (most + a.quantum - 1) / a.quantum, parts = (weight + a.least - 1) / a.least;  // of a tile, at most
     uint64_t grid = units * parts < units + a.many ? units * parts : units + a.many;
     if (a.many > MOST_SPLITS || 2 * a.many * CTR_STRIDE > sc.ncounters || 2 * (uint64_t)a.many * a.cols * (kv.d + 2) > sc.partial_floats || grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
-    const bool rules = call.cap > 0.0f || call.slopes || !(call.scale >= 0x1p-10f && call.scale <= 0x1p40f);
     if (call.bf16) return rules ? launch_split<false, true>(a, (unsigned)grid, s) : launch_split<false, false>(a, (unsigned)grid, s);
     return rules ? launch_split<true, true>(a, (unsigned)grid, s) : launch_split<true, false>(a, (unsigned)grid, s);
 }

@@ -71,8 +71,9 @@ class World:
         return out
 
 
-def attend(w, q, g, scale, cap=0.0, slopes=None, window=0, prefix=None, first=None, half=False):
-    """(out, bound) f64 [rows, n_kv * g, d]: the attention of q [rows, n_kv * g, d] over World w, and how far a result may be from it.
+def attend(w, q, g, scale, cap=0.0, slopes=None, window=0, prefix=None, first=None, half=False, heads=None):
+    """(out, bound) f64 [rows, n_kv * g, d]: the attention of q [rows, n_kv * g, d] over World w, and how far a result may be from it (of `heads`
+    alone, if given).
 
     The bound counts roundings, u = 2^-24 being half a step of f32, of the quantities that the kernel forms:
       a score's error: the product's d terms and the two halves' sum, (d + 8) u of sum |q k| scale, and 2^-22 of the row's largest |q| in each
@@ -96,7 +97,7 @@ def attend(w, q, g, scale, cap=0.0, slopes=None, window=0, prefix=None, first=No
             sees &= j[None] >= np.asarray(first)[r0 : r0 + n, None]
         if prefix is not None:
             sees |= j[None] < prefix[s]
-        for h in range(n_q):
+        for h in range(n_q) if heads is None else heads:
             x, kh, vh = q[r0 : r0 + n, h], k[:, h // g], v[:, h // g]
             score = scale * (x @ kh.T)
             mass = abs(scale) * (np.abs(x) @ np.abs(kh).T)

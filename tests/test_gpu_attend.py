@@ -18,7 +18,7 @@ def be():
     b.close()
 
 
-def check(be, w, g, dtype="f32", scale=None, seed=5, strided=False, odd=False, ragged=None, loud=2.0, **rules):
+def check(be, w, g, dtype="f32", scale=None, seed=5, strided=False, odd=False, ragged=None, loud=2.0, heads=None, **rules):
     """One call over World w against the reference; rows behind the last sequence and what lies between rows stay as they were."""
     from oxinfer_amd import hip
     rng = np.random.default_rng(seed)
@@ -37,9 +37,11 @@ def check(be, w, g, dtype="f32", scale=None, seed=5, strided=False, odd=False, r
     be.attend(cache, batch, q[:, :width], scale=scale, out=out[:, :width], **up)
     torch.cuda.synchronize()
     got = out.double().cpu().numpy()
-    want, tol = kv_ref.attend(w, q[: w.rows, :width].double().cpu().numpy().reshape(w.rows, n_q, w.d), g, scale, half=dtype == "bf16", **rules)
+    want, tol = kv_ref.attend(w, q[: w.rows, :width].double().cpu().numpy().reshape(w.rows, n_q, w.d), g, scale, half=dtype == "bf16", heads=heads, **rules)
     assert (got[w.rows :] == 7.5).all() and (got[:, width:] == 7.5).all(), "what is not the call's was written"
     off = np.abs(got[: w.rows, :width].reshape(want.shape) - want)
+    if heads is not None:
+        off, tol = off[:, heads], tol[:, heads]
     assert (off <= tol).all(), f"{np.max(off / np.maximum(tol, 1e-300)):.2f} times the bound"
     return got
 
@@ -233,6 +235,122 @@ def test_a_cache_of_more_than_4_gib(be):
     assert torch.equal(be.attend(cache, batch, q), be.attend(small_cache, small_batch, q))
     for a, b in zip(be.kv_read(cache, batch, 260), be.kv_read(small_cache, small_batch, 260)):
         assert torch.equal(a, b)
+
+
+# ---- batches of many rows, which the matrix-core-bound kernel takes: rows x heads of 256 tiles of 128 entries and more (a few heads are checked) ----
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", range(32, 257, 32))
+def test_prompts_of_every_head_size(be, d, dtype):
+    """Both widths of workgroup, the second from 1024 tiles on; last rows that fill a tile in part, keys that end inside a block."""
+    for rows, n_kv, g in ((max(130, 32768 * 128 // d // 64 + 3) if d < 128 else 513, 8, 8), (1029, 16, 8)):
+        if d < 128 and rows == 1029:
+            rows = 2053
+        w = kv_ref.World([rows + 77], n_kv, d, page=64, seed=d, n=[rows])
+        assert rows * g * n_kv // 128 >= 256 and rows * g * n_kv // 128 * d >= 256 * 128
+        check(be, w, g, dtype, heads=[0, n_kv * g - 1], ragged=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rules", RULES, ids=str)
+def test_prompts_with_masks_caps_and_biases(be, rules, dtype):
+    rules = dict(rules)
+    rng = np.random.default_rng(8)
+    n = [3, 211, 0, 130, 16, 1]
+    w = kv_ref.World([90, 350, 40, 130, 200, 333], 16, 128, page=32, seed=9, n=n)
+    g = 8
+    if rules.get("slopes"):
+        rules["slopes"] = np.exp2(-8 * np.arange(1, 129) / 128).astype(np.float32)
+    if "prefix" in rules:
+        rules["prefix"] = np.array((rules["prefix"] * 2)[:6], np.int32)
+    pos = np.concatenate([w.lens[s] - w.n[s] + np.arange(w.n[s]) for s in range(6)])
+    if rules.get("first") == "docs":
+        rules["first"] = (pos * rng.integers(0, 5, w.rows) // 4).astype(np.int32)
+    elif rules.get("first") == "none":
+        rules["first"] = np.where(np.arange(w.rows) % 2, 0, np.where(np.arange(w.rows) % 4, pos + 1, 2**31 - 1)).astype(np.int32)
+    check(be, w, g, dtype, loud=4.0, heads=[0, 60, 127], **rules)
+
+
+@pytest.mark.parametrize("n,lens", [([128, 1, 128], [128, 4000, 300]), ([15, 17, 400], [15, 17, 400]), ([300, 90], [70, 33]), ([1] * 70 + [290], [33] * 70 + [290])])
+@pytest.mark.parametrize("g", [3, 8, 16, 40])
+def test_prompts_beside_single_tokens(be, n, lens, g):
+    """Sequences on either side of the border between the kernels in one call, groups that tiles do not divide into, rows before the first token."""
+    n_kv = -(-256 * 128 // (sum(n) * g)) + 1
+    w = kv_ref.World(lens, n_kv, 128, page=64, seed=g, n=n)
+    for dtype in ("f32", "bf16"):
+        check(be, w, g, dtype, heads=[0, n_kv * g // 2, n_kv * g - 1], ragged=True)
+
+
+def test_a_prompt_in_a_buffer_for_more(be):
+    """The batch has room for many rows, the one sequence hardly any: the other rows stay as they are."""
+    from oxinfer_amd import hip
+    w = kv_ref.World([50], 8, 128, seed=2, n=[3])
+    cache, batch = w.tensors(hip, ragged=True)
+    big = hip.KvBatch(batch.kv_len, batch.pages, rows=1000, row_start=batch.row_start)
+    q = torch.randn(1000, 64 * 128, device="cuda")
+    out = torch.full_like(q, 3.0)
+    be.attend(cache, big, q, out=out)
+    want, tol = kv_ref.attend(w, q[:3].double().cpu().numpy().reshape(3, 64, 128), 8, 128**-0.5)
+    assert (np.abs(out[:3].double().cpu().numpy().reshape(want.shape) - want) <= tol).all() and (out[3:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_prompts_of_other_scales_strides_and_addresses(be, scale, dtype):
+    w = kv_ref.World([300, 64], 16, 128, page=64, seed=3, n=[260, 5])
+    check(be, w, 8, dtype, scale=scale, heads=[1, 77], strided=True)
+    check(be, w, 8, dtype, scale=0.1, heads=[1, 77], strided=True, odd=True)
+
+
+def test_prompts_pages_outside_the_cache_and_queries_that_are_not_numbers(be):
+    from oxinfer_amd import hip
+    w = kv_ref.World([400, 64], 16, 128, page=32, seed=3, n=[300, 5])
+    q = torch.randn(w.rows, 128 * 128, device="cuda")
+    cache, batch = w.tensors(hip)
+    want = be.attend(cache, batch, q, window=100)
+    pages = batch.pages.clone()
+    pages[0, 5] = w.n_pages  # tokens 160 .. 191 of the first sequence
+    got = be.attend(cache, hip.KvBatch(batch.kv_len, pages, rows=w.rows, row_start=batch.row_start), q, window=100)
+    pos = np.concatenate([w.lens[s] - w.n[s] + np.arange(w.n[s]) for s in range(2)])
+    sees = torch.from_numpy((np.repeat(np.arange(2), w.n) == 0) & (pos >= 160) & (pos - 99 <= 191)).cuda()
+    assert got[sees].isnan().all() and sees.any() and torch.equal(got[~sees], want[~sees])
+    bad = q.clone()
+    bad[7, 130] = float("nan")
+    bad[200, 5] = float("inf")
+    got = be.attend(cache, batch, bad, window=100).view(w.rows, 128, 128)
+    same = torch.ones(w.rows, 128, dtype=torch.bool)
+    same[7, 1] = same[200, 0] = False
+    assert torch.equal(got[same], want.view(w.rows, 128, 128)[same]) and got[7, 1].isnan().all() and got[200, 0].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompts_by_a_recorded_plan_and_the_same_bits_every_time(be, dtype):
+    from oxinfer_amd import hip
+    w = kv_ref.World([1000, 500, 700], 16, 128, page=64, seed=3, n=[300, 2, 150])
+    cache, batch = w.tensors(hip)
+    q = torch.randn(w.rows, 128 * 128, device="cuda").to(dtype)
+    out = torch.empty_like(q)
+    want = {}
+    lengths = [[1000, 500, 700], [300, 2, 150], [777, 499, 151], [1000, 500, 700]]
+    for lens in lengths:
+        batch.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        want[tuple(lens)] = be.attend(cache, batch, q)
+        for _ in range(5):
+            assert torch.equal(want[tuple(lens)], be.attend(cache, batch, q))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        be.attend(cache, batch, q, out=out)
+        stream.synchronize()
+        plan = be.plan_record(lambda: be.attend(cache, batch, q, out=out))
+        for lens in lengths:
+            batch.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+            out.fill_(9)
+            plan.replay()
+            stream.synchronize()
+            assert torch.equal(out, want[tuple(lens)]), lens
+    del plan
 
 
 def test_nothing_to_do(be):

@@ -9,47 +9,62 @@ __device__ __forceinline__ float load_value(const void* p, size_t i) {
     if constexpr (BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
     else return static_cast<const float*>(p)[i];
 }
-// Eight consecutive values; `vec`: they begin at a 16-byte boundary.
-template <bool BF16>
-__device__ __forceinline__ void load_eight(const void* p, size_t i, bool vec, float* v) {
+// N (4 or 8) consecutive values; `vec`: they begin at a 16-byte boundary (four bf16 ones: at an 8-byte one).
+template <bool BF16, int N>
+__device__ __forceinline__ void load_run(const void* p, size_t i, bool vec, float* v) {
     if (vec) {
-        if constexpr (BF16) {
-            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[2 * j] = __uint_as_float(w[j] << 16);
-                v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-            }
+        uint32_t w[BF16 ? N / 2 : N];
+        if constexpr (BF16 && N == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+            w[0] = u.x; w[1] = u.y;
         } else {
-            const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i), b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+            for (int k = 0; k < (BF16 ? N / 2 : N); k += 4) {
+                const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (BF16 ? 2 : 4) + 4 * k);
+                w[k] = u.x; w[k + 1] = u.y; w[k + 2] = u.z; w[k + 3] = u.w;
+            }
         }
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = __uint_as_float(!BF16 ? w[BF16 ? 0 : j] : j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = load_value<BF16>(p, i + j);
+        for (int j = 0; j < N; j++) v[j] = load_value<BF16>(p, i + j);
     }
 }
 
-// Channels c .. c + 7 of a head rotated by the angles of position `pos`, in f64 (exact products, one rounding): (a, b) -> (a cos - b sin,
+// N (4 or 8) channels c .. of a head rotated by the angles of position `pos`, in f64 (exact products, one rounding): (a, b) -> (a cos - b sin,
 // b cos + a sin) for the pairs (i, i + half), or (2 i, 2 i + 1) where they are interleaved; channels past the pairs stay as they are.
-// A position that the table does not hold gives NaN.
-template <bool BF16>
-__device__ __forceinline__ void rotate_eight(const RopeView& r, const void* p, size_t head, uint32_t c, int32_t pos, bool vec, double* x) {
-    float v[8];
-    load_eight<BF16>(p, head + c, vec, v);
+// A position that the table does not hold gives NaN. `even`: half is a multiple of 8, so that a run of channels is all of one kind and its
+// partners and angles are runs too.
+template <bool BF16, int N>
+__device__ __forceinline__ void rotate(const RopeView& r, const void* p, size_t head, uint32_t c, int32_t pos, bool vec, bool even, double* x) {
+    float v[N];
+    load_run<BF16, N>(p, head + c, vec, v);
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = v[j];
+    for (int j = 0; j < N; j++) x[j] = v[j];
     if (c >= 2 * r.half) return;
     if ((uint32_t)pos >= r.n_pos) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = c + j < 2 * r.half ? (double)__builtin_nanf("") : x[j];
+        for (int j = 0; j < N; j++) x[j] = c + j < 2 * r.half ? (double)__builtin_nanf("") : x[j];
         return;
     }
     const float2* t = reinterpret_cast<const float2*>(r.table) + (size_t)(uint32_t)pos * r.half;
+    if (even && !r.interleaved) {
+        const bool second = c >= r.half;
+        const uint32_t other = second ? c - r.half : c + r.half;
+        float o[N];
+        load_run<BF16, N>(p, head + other, vec, o);
+        const float2* angle = t + (second ? other : c);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < N; j++) {
+            const float2 a = angle[j];
+            const double turned = (double)o[j] * (double)a.y;
+            x[j] = (double)v[j] * (double)a.x + (second ? turned : -turned);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
         const uint32_t cj = c + j;
         if (cj >= 2 * r.half) continue;
         const bool second = r.interleaved ? (cj & 1) : cj >= r.half;
@@ -61,13 +76,53 @@ __device__ __forceinline__ void rotate_eight(const RopeView& r, const void* p, s
     }
 }
 
-template <bool BF16>
-__device__ __forceinline__ void store_value(void* p, size_t i, double x) {
-    if constexpr (BF16) {
-        static_cast<uint16_t*>(p)[i] = f32_to_bf16_bits((float)x);  // (by way of f32: half a step of bf16 and 2^-24 of the value at most)
+template <bool BF16, int N>
+__device__ __forceinline__ void store_run(void* p, size_t i, bool vec, const double* x) {
+    uint32_t w[N];  // (f64 to bf16 by way of f32: half a step of bf16 and 2^-24 of the value at most)
+#pragma unroll
+    for (int j = 0; j < N; j++) w[j] = BF16 ? f32_to_bf16_bits((float)x[j]) : __float_as_uint((float)x[j]);
+    if (vec && BF16) {
+        uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + i);
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+        else *reinterpret_cast<uint4*>(o) = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4 % N] | w[5 % N] << 16, w[6 % N] | w[7 % N] << 16);
+    } else if (vec) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + i + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
     } else {
-        static_cast<float*>(p)[i] = (float)x;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            if constexpr (BF16) static_cast<uint16_t*>(p)[i + j] = (uint16_t)w[j];
+            else static_cast<uint32_t*>(p)[i + j] = w[j];
+        }
     }
+}
+
+// What 8 bits hold: no NaN, and nothing past the largest scale.
+__device__ __forceinline__ double storable(double x) {
+    return x == x ? fmin(fmax(x, -127.0 * KV_SCALE_MAX), 127.0 * KV_SCALE_MAX) : 0.0;
+}
+// The scale of a block whose new tokens' largest magnitude is `top`; `was`: what it has been for the tokens that are there, KV_SCALE_MIN if there are none.
+__device__ __forceinline__ float grown_scale(float was, double top) {
+    const float need = fmaxf((float)(top / 127.0), KV_SCALE_MIN);
+    if (!(was > KV_SCALE_MIN)) return need;
+    const int more = __builtin_amdgcn_frexp_expf(need) - __builtin_amdgcn_frexp_expf(was) + (__builtin_amdgcn_frexp_mantf(need) > __builtin_amdgcn_frexp_mantf(was) ? 1 : 0);
+    return ldexpf(was, max(more, 0));
+}
+__device__ __forceinline__ float sound_scale(float held) { return held > KV_SCALE_MIN && held < 2.0f * KV_SCALE_MAX ? held : KV_SCALE_MIN; }
+// The code of x: the integer next to x / scale, halves to the even one (x - r scale is exact, so a product with the reciprocal that came to lie on the
+// other side of a border shows).
+__device__ __forceinline__ uint32_t code_of(double x, double scale, double inv) {
+    double r = rint(x * inv);
+    const double off = fma(-r, scale, x), far = fabs(off), half = 0.5 * scale;
+    if (far > half || (far == half && ((int)r & 1))) r += off > 0.0 ? 1.0 : -1.0;
+    return (uint32_t)((int)fmin(fmax(r, -127.0), 127.0) + 128);
+}
+// Four codes held by `was` / `scale` of their steps.
+__device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) r |= (uint32_t)((int)rintf(((float)((w >> (8 * j)) & 0xFF) - 128.0f) * ratio) + 128) << (8 * j);
+    return r;
 }
 
 struct AppendArgs {
@@ -77,7 +132,8 @@ struct AppendArgs {
     const void *k, *v, *q;
     void* q_out;
     size_t k_stride, v_stride, q_stride, q_out_stride;
-    uint32_t vec;  // k, v and q by 16 bytes
+    uint32_t vec, even;  // k, v, q and q_out by 16 bytes; whole runs of 8 channels rotate alike
+    uint32_t tasks;      // heads of a sequence: keys, values, queries
 };
 
 // One block of 32 positions (those of them that the call's rows take) of one head per workgroup: blockIdx.y below n_kv its keys, below
@@ -114,15 +170,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 #pragma unroll
         for (int i = 0; i < MOST; i++) {
             const uint32_t u = tid + i * 256, t = u / per, c = u % per * 8;
-            if (u < units) rotate_eight<BF16>(a.rope, a.q, (first + t) * a.q_stride + head, c, lo + (int32_t)t, a.vec & 4, x[i]);
+            if (u < units) rotate<BF16, 8>(a.rope, a.q, (first + t) * a.q_stride + head, c, lo + (int32_t)t, a.vec & 4, a.even, x[i]);
         }
         __syncthreads();  // q_out may be q: a pair's other half is read by another thread, before anything is stored
 #pragma unroll
         for (int i = 0; i < MOST; i++) {
             const uint32_t u = tid + i * 256, t = u / per, c = u % per * 8;
-            if (u >= units) continue;
-#pragma unroll
-            for (int j = 0; j < 8; j++) store_value<BF16>(a.q_out, (first + t) * a.q_out_stride + head + c + j, x[i][j]);
+            if (u < units) store_run<BF16, 8>(a.q_out, (first + t) * a.q_out_stride + head + c, a.vec & 8, x[i]);
         }
         return;
     }
@@ -144,11 +198,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         const uint32_t u = tid + i * 256;
         if (u < units) {
             const uint32_t t = u / per, c = u % per * 8;
-            if (values) rotate_eight<BF16>(none, a.v, (first + t) * a.v_stride + (size_t)head * d, c, 0, a.vec & 2, x[i]);
-            else rotate_eight<BF16>(a.rope, a.k, (first + t) * a.k_stride + (size_t)head * d, c, lo + (int32_t)t, a.vec & 1, x[i]);
+            if (values) rotate<BF16, 8>(none, a.v, (first + t) * a.v_stride + (size_t)head * d, c, 0, a.vec & 2, true, x[i]);
+            else rotate<BF16, 8>(a.rope, a.k, (first + t) * a.k_stride + (size_t)head * d, c, lo + (int32_t)t, a.vec & 1, a.even, x[i]);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[i][j] = x[i][j] == x[i][j] ? fmin(fmax(x[i][j], -127.0 * KV_SCALE_MAX), 127.0 * KV_SCALE_MAX) : 0.0;  // (8 bits hold no NaN)
+                x[i][j] = storable(x[i][j]);
                 top = fmax(top, fabs(x[i][j]));
             }
         }
@@ -158,13 +212,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     if ((tid & 63) == 0) top_s[tid >> 6] = top;
     __syncthreads();
     top = fmax(fmax(top_s[0], top_s[1]), fmax(top_s[2], top_s[3]));
-    const float need = fmaxf((float)(top / 127.0), KV_SCALE_MIN);
-    const float was = held > KV_SCALE_MIN && held < 2.0f * KV_SCALE_MAX ? held : KV_SCALE_MIN;
-    float scale = need;
-    if (was > KV_SCALE_MIN) {
-        const int more = __builtin_amdgcn_frexp_expf(need) - __builtin_amdgcn_frexp_expf(was) + (__builtin_amdgcn_frexp_mantf(need) > __builtin_amdgcn_frexp_mantf(was) ? 1 : 0);
-        scale = ldexpf(was, max(more, 0));
-    }
+    const float was = sound_scale(held), scale = grown_scale(was, top);
     const bool rescale = old && scale != was;
     const bool whole = rescale || hi - lo > 8;  // the block goes out through its image
     if (whole && old) {
@@ -174,21 +222,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
             uint32_t w[4] = {u.x, u.y, u.z, u.w};
             if (rescale) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint32_t r = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float c = rintf(((float)((w[k] >> (8 * j)) & 0xFF) - 128.0f) * ratio);
-                        r |= (uint32_t)((int)c + 128) << (8 * j);
-                    }
-                    w[k] = r;
-                }
+                for (int k = 0; k < 4; k++) w[k] = rescaled(w[k], ratio);
             }
             *reinterpret_cast<uint4*>(image + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncthreads();
     }
-    const double inv = 1.0 / (double)scale, half = 0.5 * (double)scale;
+    const double inv = 1.0 / (double)scale;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
         const uint32_t u = tid + i * 256;
@@ -196,14 +236,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         const uint32_t t = (uint32_t)(lo - p0) + u / per, c = u % per * 8;
         uint32_t code[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            // the integer next to x / scale, halves to the even one: x - r scale is exact, so a product with the reciprocal that came to
-            // lie on the other side of a border shows
-            double r = rint(x[i][j] * inv);
-            const double off = fma(-r, (double)scale, x[i][j]), far = fabs(off);
-            if (far > half || (far == half && ((int)r & 1))) r += off > 0.0 ? 1.0 : -1.0;
-            code[j] = (uint32_t)((int)fmin(fmax(r, -127.0), 127.0) + 128);
-        }
+        for (int j = 0; j < 8; j++) code[j] = code_of(x[i][j], scale, inv);
         if (values) {
             uint8_t* to = (whole ? image : codes) + kv_value_offset(t, c);  // (eight consecutive channels lie 16 bytes apart)
 #pragma unroll
@@ -237,20 +270,92 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     }
 }
 
+// The same for one new token a sequence (row_start NULL): a wave takes one head's keys, values or query, four channels a lane, and needs no other
+// wave. A step of 64 sequences, 32 query heads over 8 of 128 channels: 11.9 us with the kernel above, a workgroup to a head, XSTEP here.
+template <bool BF16>
+__global__ __launch_bounds__(256) void kv_append_step_kernel(AppendArgs a) {
+    const uint32_t d = a.kv.d, lane = threadIdx.x & 63, c = 4 * lane;
+    const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), s = task / a.tasks, what = task % a.tasks;  // (a sequence's heads: keys, values, queries)
+    if (s >= a.b.n_seqs) return;
+    const bool live = c < d;
+    const bool key = what < a.kv.n_kv, query = what >= 2 * a.kv.n_kv;
+    const uint32_t head = query ? what - 2 * a.kv.n_kv : key ? what : what - a.kv.n_kv;
+    // what the arrays of the batch say is on its way while the values come
+    const int32_t len = a.b.kv_len[s];
+    const KvSeq q = kv_part((int32_t)s, (int32_t)s, (int32_t)s + 1, len, a.b.rows, a.b.max_pages, a.kv.shift);
+    const int32_t pos = q.len - 1;
+    double x[4] = {0.0, 0.0, 0.0, 0.0};
+    if (live) {
+        RopeView none{};
+        if (query) rotate<BF16, 4>(a.rope, a.q, (size_t)s * a.q_stride + (size_t)head * d, c, pos, a.vec & 4, a.even, x);
+        else if (key) rotate<BF16, 4>(a.rope, a.k, (size_t)s * a.k_stride + (size_t)head * d, c, pos, a.vec & 1, a.even, x);
+        else rotate<BF16, 4>(none, a.v, (size_t)s * a.v_stride + (size_t)head * d, c, 0, a.vec & 2, true, x);
+    }
+    if (pos < 0) return;
+    if (query) {
+        // (q_out may be q: a pair's other half was read by another lane of this wave, before)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (live) store_run<BF16, 4>(a.q_out, (size_t)s * a.q_out_stride + (size_t)head * d + c, a.vec & 8, x);
+        return;
+    }
+    const uint32_t block = (uint32_t)pos / KV_BLOCK, t = (uint32_t)pos % KV_BLOCK;
+    const int32_t page = kv_page(a.b, a.kv, (int32_t)s, block);
+    if (page < 0) return;
+    const size_t index = kv_block_index(a.kv, page, head, block);
+    uint8_t* codes = (key ? a.kv.k : a.kv.v) + index * KV_BLOCK * d;
+    float* scale_at = (key ? a.kv.k_scale : a.kv.v_scale) + index;
+    const float was = t ? sound_scale(*scale_at) : KV_SCALE_MIN;
+    double top = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        x[j] = storable(x[j]);
+        top = fmax(top, fabs(x[j]));
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) top = fmax(top, __shfl_xor(top, m));
+    const float scale = grown_scale(was, top);
+    if (t && scale != was) {  // the codes that are there, first
+        for (uint32_t i = lane; i < KV_BLOCK * d / 16; i += 64) {
+            uint4 u = *reinterpret_cast<const uint4*>(codes + 16 * i);
+            const float ratio = was / scale;
+            u.x = rescaled(u.x, ratio);
+            u.y = rescaled(u.y, ratio);
+            u.z = rescaled(u.z, ratio);
+            u.w = rescaled(u.w, ratio);
+            *reinterpret_cast<uint4*>(codes + 16 * i) = u;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the token's own bytes go there behind them)
+    }
+    if (lane == 0 && (!t || scale != was)) *scale_at = scale;
+    if (!live) return;
+    const double inv = 1.0 / (double)scale;
+    uint32_t code[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) code[j] = code_of(x[j], scale, inv);
+    if (key) {
+        *reinterpret_cast<uint32_t*>(codes + kv_key_offset(t, c)) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+    } else {
+        uint8_t* to = codes + kv_value_offset(t, c);
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[16 * j] = (uint8_t)code[j];
+    }
+}
+
 struct ReadArgs {
     KvView kv;
     KvBatchView b;
     void *k_out, *v_out;
     int32_t count;
     uint32_t blocks;  // of a sequence's places, whole or in part
+    uint32_t vec;     // k_out by 16 bytes
 };
 
 // The values that the last `count` tokens of every sequence stand for, [sequence][token][head][d]: a block's part of them per workgroup
-// (blockIdx.y: the head's keys, then the head's values), through an image of the block in LDS. Places before a sequence's first token are
-// zeros, those of a page that the table does not name NaN. The bound is memory: a byte read, an f32 (or bf16) written.
+// (blockIdx.y: the head's keys, then the head's values), 16 codes a thread as they lie: of keys eight channels of two tokens, of values eight
+// tokens of two channels. Places before a sequence's first token are zeros, those of a page that the table does not name NaN. The bound is
+// memory: a byte read, an f32 (or bf16) written.
 template <bool BF16>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
-    __shared__ __align__(16) uint8_t image[KV_BLOCK * KV_MAX_D];
     const uint32_t d = a.kv.d, tid = threadIdx.x;
     const bool values = blockIdx.y >= a.kv.n_kv;
     void* out = values ? a.v_out : a.k_out;
@@ -262,43 +367,72 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
     const int32_t p0 = block * (int32_t)KV_BLOCK, lo = max(p0, start), hi = min(p0 + (int32_t)KV_BLOCK, q.len);
     if (hi <= lo) return;
     const uint32_t head = blockIdx.y - (values ? a.kv.n_kv : 0u);
-    float scale = 0.0f;
+    const uint8_t* codes = nullptr;
+    float scale = 0.0f, nothing = 0.0f;
     if (block >= 0) {
         const int32_t page = kv_page(a.b, a.kv, s, (uint32_t)block);
-        scale = __builtin_nanf("");
+        nothing = __builtin_nanf("");
         if (page >= 0) {
             const size_t index = kv_block_index(a.kv, page, head, (uint32_t)block);
-            const uint8_t* codes = (values ? a.kv.v : a.kv.k) + index * KV_BLOCK * d;
+            codes = (values ? a.kv.v : a.kv.k) + index * KV_BLOCK * d;
             scale = (values ? a.kv.v_scale : a.kv.k_scale)[index];
-            for (uint32_t i = tid; i < KV_BLOCK * d / 16; i += 256) *reinterpret_cast<uint4*>(image + 16 * i) = *reinterpret_cast<const uint4*>(codes + 16 * i);
         }
-        __syncthreads();
     }
-    const bool none = block < 0 || scale != scale;  // (the image holds nothing)
-    for (uint32_t u = tid; u < (uint32_t)(hi - lo) * d; u += 256) {
-        const uint32_t t = (uint32_t)(lo - p0) + u / d, c = u % d;
-        const float code = none ? 0.0f : (float)image[values ? kv_value_offset(t, c) : kv_key_offset(t, c)] - 128.0f;
-        const size_t to = (((size_t)s * a.count + (size_t)(p0 + (int32_t)t - start)) * a.kv.n_kv + head) * d + c;
-        const float x = none ? scale : code * scale;
-        if constexpr (BF16) static_cast<uint16_t*>(out)[to] = f32_to_bf16_bits(x);
-        else static_cast<float*>(out)[to] = x;
+    const size_t row = (size_t)a.kv.n_kv * d, base = (size_t)s * a.count * row + (size_t)head * d;
+    for (uint32_t i = tid; i < 2 * d; i += 256) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (codes) u = *reinterpret_cast<const uint4*>(codes + 16 * i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w}, g = i % 64 / 16, n = i % 16;
+        float x[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) x[k] = codes ? ((float)((w[k / 4] >> (8 * (k % 4))) & 0xFF) - 128.0f) * scale : nothing;
+        if (values) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int32_t p = p0 + (int32_t)(k % 8 / 4 * 16 + 4 * g + k % 4);
+                const size_t to = base + (size_t)(p - start) * row + i / 64 * 32 + k / 8 * 16 + n;
+                if (p < lo || p >= hi) continue;
+                if constexpr (BF16) static_cast<uint16_t*>(out)[to] = f32_to_bf16_bits(x[k]);
+                else static_cast<float*>(out)[to] = x[k];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int32_t p = p0 + (int32_t)(k * 16 + n);
+                const size_t to = base + (size_t)(p - start) * row + i / 64 * 32 + g * 8;
+                if (p < lo || p >= hi) continue;
+                double y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = x[8 * k + j];
+                store_run<BF16, 8>(out, to, a.vec, y);
+            }
+        }
     }
 }
 
 hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
                             size_t q_stride, void* q_out, size_t q_out_stride, uint32_t n_q, bool bf16, hipStream_t s) {
-    AppendArgs a{kv, b, rope, k, v, q, q_out, k_stride, v_stride, q_stride, q_out_stride, 0};
+    AppendArgs a{kv, b, rope, k, v, q, q_out, k_stride, v_stride, q_stride, q_out_stride, 0, 0, 2 * kv.n_kv + n_q};
     const size_t size = bf16 ? 2 : 4;
     auto vec = [&](const void* p, size_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; };
-    a.vec = (vec(k, k_stride) ? 1u : 0u) | (vec(v, v_stride) ? 2u : 0u) | (vec(q, q_stride) ? 4u : 0u);
-    const dim3 grid((unsigned)(b.row_start ? kv_places(b.rows, b.n_seqs, KV_BLOCK, 2) : b.n_seqs), 2 * kv.n_kv + n_q);
+    a.vec = (vec(k, k_stride) ? 1u : 0u) | (vec(v, v_stride) ? 2u : 0u) | (vec(q, q_stride) ? 4u : 0u) | (vec(q_out, q_out_stride) ? 8u : 0u);
+    a.even = rope.half % 8 == 0;
+    if (!b.row_start) {
+        const uint64_t tasks = (uint64_t)b.n_seqs * a.tasks;
+        if (tasks > 0x7FFFFFFFu) return hipErrorInvalidValue;
+        const unsigned grid = (unsigned)((tasks + 3) / 4);
+        if (bf16) kv_append_step_kernel<true><<<grid, 256, 0, s>>>(a);
+        else kv_append_step_kernel<false><<<grid, 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    const dim3 grid((unsigned)kv_places(b.rows, b.n_seqs, KV_BLOCK, 2), a.tasks);
     if (bf16) kv_append_kernel<true><<<grid, 256, 0, s>>>(a);
     else kv_append_kernel<false><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvView& kv, const KvBatchView& b, size_t count, void* k_out, void* v_out, bool bf16, hipStream_t s) {
-    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)((count + 2 * KV_BLOCK - 2) / KV_BLOCK)};
+    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)((count + 2 * KV_BLOCK - 2) / KV_BLOCK), reinterpret_cast<uintptr_t>(k_out) % 16 == 0};
     const dim3 grid(a.blocks * b.n_seqs, 2 * kv.n_kv);
     if (bf16) kv_read_kernel<true><<<grid, 256, 0, s>>>(a);
     else kv_read_kernel<false><<<grid, 256, 0, s>>>(a);

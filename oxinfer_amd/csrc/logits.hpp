@@ -24,8 +24,8 @@ struct LogitArgs {
     uint32_t slices, vec;
 };
 
-// Workgroups that share a row's vocabulary.
-constexpr uint32_t LOGIT_SLICE = 4096;
-inline size_t logit_slices(size_t vocab) { return (vocab + LOGIT_SLICE - 1) / LOGIT_SLICE; }
+// Logits of a row that a workgroup takes.
+inline uint32_t logit_slice(size_t rows, size_t vocab) { return rows * ((vocab + 4095) / 4096) >= 256 ? 4096 : 2048; }
+inline size_t logit_slices(size_t rows, size_t vocab) { return (vocab + logit_slice(rows, vocab) - 1) / logit_slice(rows, vocab); }
 
 }  // namespace oxhip

@@ -252,38 +252,37 @@ class QAct:
                        self.hsums.data_ptr(), self.sums16.data_ptr(), t, n_in)
 
 
-def _array(name, t, dtypes, device=None, shape=None):
-    """Checks a dense device tensor that the library gets by its pointer; returns the pointer (None for None)."""
+# Checks of the tensors that the library gets by their pointers. They are most of what a call costs the host, so each asks a tensor for little: the
+# wrong ones are told apart where they are found wrong.
+def _array(name, t, dtype, device=None, count=None):
+    """A dense device tensor of `dtype` (with `count` values, if given): its pointer, or None for None."""
     if t is None:
         return None
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name}: {t.dtype}, wanted {' or '.join(map(str, dtypes))}")
-    if not t.is_cuda or (device is not None and t.device.index != device):
-        raise ValueError(f"{name}: on {t.device}, wanted cuda:{device if device is not None else '*'}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: not contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted {tuple(shape)}")
+    if t.dtype is not dtype or not t.is_contiguous() or t.get_device() < 0 or (device is not None and t.get_device() != device) or (count is not None and t.numel() != count):
+        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}; wanted {dtype}"
+                         f"{'' if count is None else f' of {count} values'} on cuda:{'*' if device is None else device}")
     return t.data_ptr()
 
 
-def _rows(name, t, width, rows, dtypes, device):
-    """Checks rows [rows, ...] of `width` dense values each, which may lie further apart; returns (pointer, stride in values)."""
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name}: {t.dtype}, wanted {' or '.join(map(str, dtypes))}")
-    if not t.is_cuda or t.device.index != device:
+def _rows(name, t, width, rows, device):
+    """Rows [rows, ...] of `width` dense values each, f32 or bf16, which may lie further apart: (pointer, stride in values, bf16)."""
+    bf16 = t.dtype is _torch.bfloat16
+    if not bf16 and t.dtype is not _torch.float32:
+        raise ValueError(f"{name}: {t.dtype}, wanted torch.float32 or torch.bfloat16")
+    if t.get_device() != device:
         raise ValueError(f"{name}: on {t.device}, wanted cuda:{device}")
-    if t.dim() < 2 or t.shape[0] < rows or math.prod(t.shape[1:]) != width:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted at least {rows} rows of {width} values")
+    shape, strides = t.shape, t.stride()
+    if len(shape) < 2 or shape[0] < rows or math.prod(shape[1:]) != width:
+        raise ValueError(f"{name}: shape {tuple(shape)}, wanted at least {rows} rows of {width} values")
     dense = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size != 1 and stride != dense:
+    for i in range(len(shape) - 1, 0, -1):
+        if strides[i] != dense and shape[i] != 1:
             raise ValueError(f"{name}: a row's values are not dense")
-        dense *= size
-    stride = t.stride(0) if t.shape[0] > 1 else width
+        dense *= shape[i]
+    stride = strides[0] if shape[0] > 1 else width
     if stride < width:
         raise ValueError(f"{name}: rows overlap")
-    return t.data_ptr(), stride
+    return t.data_ptr(), stride, int(bf16)
 
 
 class KvCache:
@@ -292,14 +291,16 @@ class KvCache:
 
     def __init__(self, k, v, k_scale, v_scale, page_tokens, d):
         import torch
+        if k.dim() != 4 or page_tokens < 32 or k.shape[2] != page_tokens // 32 or k.shape[3] != 32 * d:
+            raise ValueError(f"k: shape {tuple(k.shape)}, wanted [n_pages, n_kv, {page_tokens // 32}, {32 * d}]")
         n_pages, n_kv = k.shape[:2]
-        per = page_tokens // 32
-        dev = k.device.index if k.is_cuda else None
-        p = [_array(n, t, (torch.uint8,), dev, (n_pages, n_kv, per, 32 * d)) for n, t in (("k", k), ("v", v))]
-        p += [_array(n, t, (torch.float32,), dev, (n_pages, n_kv, per)) for n, t in (("k_scale", k_scale), ("v_scale", v_scale))]
+        dev, blocks = k.get_device() if k.is_cuda else None, n_pages * n_kv * (page_tokens // 32)
+        p = [_array(n, t, torch.uint8, dev, blocks * 32 * d) for n, t in (("k", k), ("v", v))]
+        p += [_array(n, t, torch.float32, dev, blocks) for n, t in (("k_scale", k_scale), ("v_scale", v_scale))]
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.page_tokens, self.n_kv, self.d, self.device = page_tokens, n_kv, d, dev
         self.c = KvCacheC(*p, n_pages, page_tokens, n_kv, d)
+        self.ref = C.byref(self.c)
 
 
 class KvBatch:
@@ -308,14 +309,17 @@ class KvBatch:
 
     def __init__(self, kv_len, pages, rows=None, row_start=None):
         import torch
-        n, dev = kv_len.numel(), kv_len.device.index if kv_len.is_cuda else None
-        p = _array("kv_len", kv_len, (torch.int32,), dev, (n,)), _array("pages", pages, (torch.int32,), dev, (n, pages.shape[-1]))
-        start = _array("row_start", row_start, (torch.int32,), dev, (n + 1,))
+        n, dev = kv_len.numel(), kv_len.get_device() if kv_len.is_cuda else None
+        if pages.dim() != 2:
+            raise ValueError(f"pages: shape {tuple(pages.shape)}, wanted [{n}, max_pages]")
+        p = _array("kv_len", kv_len, torch.int32, dev), _array("pages", pages, torch.int32, dev, n * pages.shape[1])
+        start = _array("row_start", row_start, torch.int32, dev, n + 1)
         if rows is None and row_start is not None:
             raise ValueError("rows: how many the batch has in all is the host's to know")
         self.kv_len, self.pages, self.row_start = kv_len, pages, row_start
         self.rows, self.n_seqs, self.device = n if rows is None else rows, n, dev
         self.c = KvBatchC(n, self.rows, start, *p, pages.shape[1])
+        self.ref = C.byref(self.c)
 
 
 class Rope:
@@ -323,9 +327,11 @@ class Rope:
 
     def __init__(self, table, interleaved=False):
         import torch
-        p = _array("table", table, (torch.float32,), table.device.index, (table.shape[0], table.shape[1], 2))
+        if table.dim() != 3 or table.shape[2] != 2:
+            raise ValueError(f"table: shape {tuple(table.shape)}, wanted [n_pos, n_rot / 2, 2]")
         self.table = table
-        self.c = RopeC(p, table.shape[0], 2 * table.shape[1], int(interleaved))
+        self.c = RopeC(_array("table", table, torch.float32), table.shape[0], 2 * table.shape[1], int(interleaved))
+        self.ref, self.device = C.byref(self.c), table.get_device()
 
 
 class HipBackend:
@@ -625,15 +631,9 @@ class HipBackend:
     # ---- attention over an 8-bit cache, the logits' rules ---------------------------------------------------------
     def _stream_here(self):
         """The current torch stream of this backend's device, which need not be the current device."""
-        import torch
-        if torch._C._cuda_getDevice() == self.device:
+        if _torch._C._cuda_getDevice() == self.device:
             return self._stream()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _float_rows(self, name, t, width, rows):
-        import torch
-        p, stride = _rows(name, t, width, rows, (torch.float32, torch.bfloat16), self.device)
-        return p, stride, 1 if t.dtype == torch.bfloat16 else 0
+        return _torch.cuda.current_stream(self.device).cuda_stream
 
     def _held(self, cache, batch):
         if cache.device != self.device or batch.device != self.device:
@@ -650,66 +650,69 @@ class HipBackend:
     def kv_append(self, cache, batch, k, v, q=None, rope=None, q_out=None):
         """The rows' keys and values [rows, n_kv * d] (f32 or bf16; any row stride) into the cache; the keys, and the queries [rows, n_q * d],
         rotated by `rope`. Returns the rotated queries (`q_out`, which may be q) or None."""
-        import torch
         self._held(cache, batch)
-        width = cache.n_kv * cache.d
-        kp, ks, kd = self._float_rows("k", k, width, batch.rows)
-        vp, vs, vd = self._float_rows("v", v, width, batch.rows)
+        dev, rows, width = self.device, batch.rows, cache.n_kv * cache.d
+        kp, ks, kd = _rows("k", k, width, rows, dev)
+        vp, vs, vd = _rows("v", v, width, rows, dev)
         qp = op = None
         qs = os_ = n_q = 0
+        qd = od = kd
         if q is not None:
-            n_q = math.prod(q.shape[1:]) // cache.d
-            qp, qs, qd = self._float_rows("q", q, n_q * cache.d, batch.rows)
+            q_width = math.prod(q.shape[1:])
+            n_q = q_width // cache.d
+            qp, qs, qd = _rows("q", q, n_q * cache.d, rows, dev)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            op, os_, od = self._float_rows("q_out", q_out, n_q * cache.d, batch.rows)
-            if qd != kd or od != kd:
-                raise ValueError("q, q_out, k and v have one type")
+                q_out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                op, os_ = q_out.data_ptr(), q_width
+            else:
+                op, os_, od = _rows("q_out", q_out, n_q * cache.d, rows, dev)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if kd != vd:
+        if not kd == vd == qd == od:
             raise ValueError("q, q_out, k and v have one type")
-        if batch.rows and not self.lib.oxhip_dev_kv_append(self.ctx, C.byref(cache.c), C.byref(batch.c), kp, ks, vp, vs, qp, qs, op, os_, n_q, kd,
-                                            C.byref(rope.c) if rope is not None else None, self._stream_here()):
+        if rope is not None and rope.device != dev:
+            raise ValueError(f"rope: wanted on cuda:{dev}")
+        if rows and not self.lib.oxhip_dev_kv_append(self.ctx, cache.ref, batch.ref, kp, ks, vp, vs, qp, qs, op, os_, n_q, kd, rope.ref if rope is not None else None,
+                                                     self._stream_here()):
             raise RuntimeError(self.last_error())
         return q_out
 
     def kv_read(self, cache, batch, count, dtype=None):
         """The values that the last `count` tokens of every sequence stand for: (k, v), each [n_seqs, count, n_kv, d] f32 (or bf16)."""
-        import torch
         self._held(cache, batch)
-        dtype = dtype or torch.float32
-        if dtype not in (torch.float32, torch.bfloat16):
+        dtype = dtype or _torch.float32
+        if dtype not in (_torch.float32, _torch.bfloat16):
             raise ValueError(f"dtype: {dtype}")
-        k, v = (torch.empty((batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype, device=cache.k.device) for _ in range(2))
-        if count and not self.lib.oxhip_dev_kv_read(self.ctx, C.byref(cache.c), C.byref(batch.c), count, k.data_ptr(), v.data_ptr(),
-                                                    int(dtype == torch.bfloat16), self._stream_here()):
+        both = _torch.empty((2, batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype, device=cache.k.device)
+        k, v = both.unbind(0)
+        if count and not self.lib.oxhip_dev_kv_read(self.ctx, cache.ref, batch.ref, count, k.data_ptr(), v.data_ptr(), int(dtype == _torch.bfloat16), self._stream_here()):
             raise RuntimeError(self.last_error())
         return k, v
 
     def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
         """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of
         `oxhip_attend_rules`. Returns out, of q's shape and type."""
-        import torch
         self._held(cache, batch)
-        n_q = math.prod(q.shape[1:]) // cache.d
-        qp, qs, qd = self._float_rows("q", q, n_q * cache.d, batch.rows)
+        dev, width = self.device, math.prod(q.shape[1:])
+        n_q = width // cache.d
+        qp, qs, qd = _rows("q", q, n_q * cache.d, batch.rows, dev)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        op, os_, od = self._float_rows("out", out, n_q * cache.d, batch.rows)
-        if qd != od:
-            raise ValueError("q and out have one type")
+            out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            op, os_ = out.data_ptr(), width
+        else:
+            op, os_, od = _rows("out", out, n_q * cache.d, batch.rows, dev)
+            if qd != od:
+                raise ValueError("q and out have one type")
         rules = None
         if cap or window or slopes is not None or prefix is not None or first is not None:
             if window < 0:
                 raise ValueError("window: at least 0")
             if first is not None and first.numel() < batch.rows:
                 raise ValueError("first: one for each row")
-            rules = C.byref(AttendRulesC(cap, _array("slopes", slopes, (torch.float32,), self.device, (n_q,)), window,
-                                         _array("prefix", prefix, (torch.int32,), self.device, (batch.n_seqs,)),
-                                         _array("first", first, (torch.int32,), self.device)))
-        if batch.rows and not self.lib.oxhip_dev_attend(self.ctx, C.byref(cache.c), C.byref(batch.c), qp, qs, n_q, qd, cache.d**-0.5 if scale is None else scale, rules,
-                                         op, os_, self._stream_here()):
+            rules = C.byref(AttendRulesC(cap, _array("slopes", slopes, _torch.float32, dev, n_q), window, _array("prefix", prefix, _torch.int32, dev, batch.n_seqs),
+                                         _array("first", first, _torch.int32, dev)))
+        if batch.rows and not self.lib.oxhip_dev_attend(self.ctx, cache.ref, batch.ref, qp, qs, n_q, qd, cache.d**-0.5 if scale is None else scale, rules, op, os_,
+                                                        self._stream_here()):
             raise RuntimeError(self.last_error())
         return out
 
@@ -717,38 +720,43 @@ class HipBackend:
                       presence=None, frequency=None, bias_start=None, bias_id=None, bias=None, allowed=None, allowed_row=None):
         """The rules of `oxhip_logit_rules` on rows of logits [rows, vocab] (f32 or bf16; any row stride): (out, next), the adjusted logits (`out`
         may be `logits`) and the best token of each row, int32. history int32 [rows, most], allowed int32 words [masks, (vocab + 31) / 32]."""
-        import torch
         t, vocab = logits.shape
-        lp, ls, ld = self._float_rows("logits", logits, vocab, t)
-        op, os_ = None, 0
-        if out is not None or want_out:
-            if out is None:
-                out = torch.empty((t, vocab), dtype=logits.dtype, device=logits.device)
-            op, os_, od = self._float_rows("out", out, vocab, t)
+        dev, i32, f32 = self.device, _torch.int32, _torch.float32
+        lp, ls, ld = _rows("logits", logits, vocab, t, dev)
+        op, os_, best = None, 0, None
+        if out is not None:
+            op, os_, od = _rows("out", out, vocab, t, dev)
             if od != ld:
                 raise ValueError("logits and out have one type")
-        best = torch.empty(t, dtype=torch.int32, device=logits.device) if want_next else None
-        ints, floats = (torch.int32,), (torch.float32,)
-
-        def array(name, v, dtypes, *shape):
-            return _array(name, v, dtypes, self.device, shape)
-
-        for name, v, n in (("history", history, t), ("allowed", allowed, 1)):
-            if v is not None and (v.dim() != 2 or v.shape[0] < n):
-                raise ValueError(f"{name}: shape {tuple(v.shape)}")
+        elif want_out:
+            out = _torch.empty((t, vocab), dtype=logits.dtype, device=logits.device)
+            op, os_ = out.data_ptr(), vocab
+        if want_next:
+            best = _torch.empty(t, dtype=i32, device=logits.device)
+        elif op is None:
+            raise ValueError("neither the adjusted logits nor the best tokens are wanted")
         rules = None
         if history is not None or bias_start is not None or allowed is not None:
-            rules = C.byref(LogitRulesC(
-                array("history", history, ints, t, history.shape[1]) if history is not None else None, history.shape[1] if history is not None else 0,
-                array("history_len", history_len, ints, t), array("prompt_len", prompt_len, ints, t), array("repetition", repetition, floats, t),
-                array("presence", presence, floats, t), array("frequency", frequency, floats, t), array("bias_start", bias_start, ints, t + 1),
-                _array("bias_id", bias_id, ints, self.device), _array("bias", bias, floats, self.device, bias_id.shape if bias_id is not None else None),
-                bias_id.numel() if bias_id is not None else 0, _array("allowed", allowed, ints, self.device), allowed.shape[0] if allowed is not None else 0,
-                allowed.shape[1] if allowed is not None else 0, array("allowed_row", allowed_row, ints, t)))
+            r = LogitRulesC()
+            if history is not None:
+                if history.dim() != 2 or history.shape[0] != t:
+                    raise ValueError(f"history: shape {tuple(history.shape)}, wanted [{t}, most]")
+                r.history, r.history_stride, r.history_len = _array("history", history, i32, dev), history.shape[1], _array("history_len", history_len, i32, dev, t)
+            r.prompt_len = _array("prompt_len", prompt_len, i32, dev, t)
+            r.repetition, r.presence, r.frequency = _array("repetition", repetition, f32, dev, t), _array("presence", presence, f32, dev, t), _array("frequency", frequency, f32, dev, t)
+            if bias_start is not None or bias_id is not None or bias is not None:
+                n = bias_id.numel() if bias_id is not None else 0
+                r.bias_start, r.bias_id, r.bias, r.n_bias = _array("bias_start", bias_start, i32, dev, t + 1), _array("bias_id", bias_id, i32, dev), _array("bias", bias, f32, dev, n), n
+                if bias_id is not None and bias_start is not None and bias is not None and not n:  # (no biases at all: their tensors have no address)
+                    r.bias_start = r.bias_id = r.bias = None
+            if allowed is not None:
+                if allowed.dim() != 2:
+                    raise ValueError(f"allowed: shape {tuple(allowed.shape)}, wanted [masks, words]")
+                r.allowed, r.n_allowed, r.allowed_stride = _array("allowed", allowed, i32, dev), allowed.shape[0], allowed.shape[1]
+            r.allowed_row = _array("allowed_row", allowed_row, i32, dev, t)
+            rules = C.byref(r)
         elif any(v is not None for v in (history_len, prompt_len, repetition, presence, frequency, bias_id, bias, allowed_row)):
             raise ValueError("penalties need a history, biases bias_start, allowed_row masks")
-        if op is None and best is None:
-            raise ValueError("neither the adjusted logits nor the best tokens are wanted")
         if t and not self.lib.oxhip_dev_logits(self.ctx, lp, ls, op, os_, t, vocab, ld, rules, best.data_ptr() if want_next else None, self._stream_here()):
             raise RuntimeError(self.last_error())
         return out, best

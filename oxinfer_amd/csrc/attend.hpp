@@ -92,15 +92,6 @@ __device__ __forceinline__ float tanh_of(float x) {
 // A value that all lanes hold alike, as a scalar.
 __device__ __forceinline__ uint32_t scalar(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-// a / b of values below 2^31, mostly small ones: by the hardware's reciprocal where its error is less than one (a lone wave takes a microsecond for
-// four divisions of the general kind).
-__device__ __forceinline__ uint32_t divide(uint32_t a, uint32_t b) {
-    if (a >= 1u << 22) return a / b;
-    const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
-    const int32_t r = (int32_t)(a - q * b);
-    return r < 0 ? q - 1 : r >= (int32_t)b ? q + 1 : q;
-}
-
 // Eight consecutive values of a row of queries; `vec`: by 16 bytes.
 template <bool F32>
 __device__ __forceinline__ void load_query(const void* q, size_t at, bool vec, float* v) {

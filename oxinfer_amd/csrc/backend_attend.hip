@@ -202,7 +202,7 @@ int oxhip_dev_logits(oxhip_ctx* c, const void* logits, size_t stride, void* out,
     if (next) {
         DecodeScratch* sc = parts(c, s, who);
         if (!sc) return 0;
-        if (rows * CTR_STRIDE > sc->ncounters || rows * logit_slices(rows, vocab) * 2 > sc->partial_floats) return refuse(who, "too many rows for `next` in one call (16384 at most)");
+        if (rows * CTR_STRIDE > sc->ncounters || rows * logit_slices(vocab) * 2 > sc->partial_floats) return refuse(who, "too many rows for `next` in one call (16384 at most)");
         a.best = reinterpret_cast<uint64_t*>(sc->partial);
         a.counters = sc->counters;
     }

@@ -46,4 +46,13 @@ __device__ __forceinline__ size_t kv_block_index(const KvView& kv, int32_t page,
     return (((size_t)(uint32_t)page * kv.n_kv + head) << kv.shift) + (block & ((1u << kv.shift) - 1));
 }
 
+// a / b of values below 2^31, mostly small ones: by the hardware's reciprocal where its error is less than one (a lone wave takes a microsecond for
+// four divisions of the general kind).
+__device__ __forceinline__ uint32_t divide(uint32_t a, uint32_t b) {
+    if (a >= 1u << 22) return a / b;
+    const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const int32_t r = (int32_t)(a - q * b);
+    return r < 0 ? q - 1 : r >= (int32_t)b ? q + 1 : q;
+}
+
 }  // namespace oxhip

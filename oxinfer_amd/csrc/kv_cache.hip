@@ -144,10 +144,11 @@ struct AppendArgs {
 // nothing and grows to what is needed.)
 // The bound is memory: rows read once, a byte a value written. A block that is new, or most of it, goes out as whole 16-byte lines through an
 // image in LDS (a value operand's tokens lie 1 byte apart, its channels 16); single tokens are stored as they lie.
-template <bool BF16>
+// MOST: runs of eight channels a thread holds, d / 64.
+template <bool BF16, int MOST>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     __shared__ double top_s[4];
-    __shared__ __align__(16) uint8_t image[KV_BLOCK * KV_MAX_D];
+    __shared__ __align__(16) uint8_t image[KV_BLOCK * 64 * MOST];
     const uint32_t d = a.kv.d, tid = threadIdx.x;
     int32_t s = (int32_t)blockIdx.x, place = 0;
     if (a.b.row_start) {
@@ -163,7 +164,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     const uint32_t per = d / 8, units = (uint32_t)(hi - lo) * per;  // eight channels of a token each
     const size_t first = (size_t)(q.row0 + (lo - before));
 
-    constexpr int MOST = KV_BLOCK * KV_MAX_D / 8 / 256;
     double x[MOST][8];
     if (blockIdx.y >= 2 * a.kv.n_kv) {
         const size_t head = (size_t)(blockIdx.y - 2 * a.kv.n_kv) * d;
@@ -347,15 +347,17 @@ struct ReadArgs {
     void *k_out, *v_out;
     int32_t count;
     uint32_t blocks;  // of a sequence's places, whole or in part
-    uint32_t vec;     // k_out by 16 bytes
+    uint32_t vec;     // k_out and v_out by 16 bytes
 };
 
 // The values that the last `count` tokens of every sequence stand for, [sequence][token][head][d]: a block's part of them per workgroup
-// (blockIdx.y: the head's keys, then the head's values), 16 codes a thread as they lie: of keys eight channels of two tokens, of values eight
-// tokens of two channels. Places before a sequence's first token are zeros, those of a page that the table does not name NaN. The bound is
-// memory: a byte read, an f32 (or bf16) written.
+// (blockIdx.y: the head's keys, then the head's values). The block goes through LDS, so that whole rows are written: keys lie there by octets of
+// channels (264 bytes each, an odd number of 8-byte banks), values by KiB as in the cache (1056 bytes), which lets the lanes of a token's
+// channels read from banks of their own. Places before a sequence's first token are zeros, those of a page that the table does not name
+// NaN. The bound is memory: a byte read, an f32 (or bf16) written.
 template <bool BF16>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
+    __shared__ __align__(16) uint8_t image[KV_MAX_D / 8 * 264];
     const uint32_t d = a.kv.d, tid = threadIdx.x;
     const bool values = blockIdx.y >= a.kv.n_kv;
     void* out = values ? a.v_out : a.k_out;
@@ -367,45 +369,53 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
     const int32_t p0 = block * (int32_t)KV_BLOCK, lo = max(p0, start), hi = min(p0 + (int32_t)KV_BLOCK, q.len);
     if (hi <= lo) return;
     const uint32_t head = blockIdx.y - (values ? a.kv.n_kv : 0u);
-    const uint8_t* codes = nullptr;
-    float scale = 0.0f, nothing = 0.0f;
-    if (block >= 0) {
-        const int32_t page = kv_page(a.b, a.kv, s, (uint32_t)block);
-        nothing = __builtin_nanf("");
-        if (page >= 0) {
-            const size_t index = kv_block_index(a.kv, page, head, (uint32_t)block);
-            codes = (values ? a.kv.v : a.kv.k) + index * KV_BLOCK * d;
-            scale = (values ? a.kv.v_scale : a.kv.k_scale)[index];
+    const int32_t page = block >= 0 ? kv_page(a.b, a.kv, s, (uint32_t)block) : -1;
+    float scale = block >= 0 ? __builtin_nanf("") : 0.0f;
+    if (page >= 0) {
+        const size_t index = kv_block_index(a.kv, page, head, (uint32_t)block);
+        const uint8_t* codes = (values ? a.kv.v : a.kv.k) + index * KV_BLOCK * d;
+        scale = (values ? a.kv.v_scale : a.kv.k_scale)[index];
+        for (uint32_t i = tid; i < 2 * d; i += 256) {
+            const uint4 u = *reinterpret_cast<const uint4*>(codes + 16 * i);
+            if (values) {
+                *reinterpret_cast<uint4*>(image + i / 64 * 1056 + i % 64 * 16) = u;
+            } else {
+                uint8_t* to = image + i / 16 * 264 + i % 16 * 8;
+                *reinterpret_cast<uint2*>(to) = make_uint2(u.x, u.y);
+                *reinterpret_cast<uint2*>(to + 128) = make_uint2(u.z, u.w);
+            }
         }
     }
-    const size_t row = (size_t)a.kv.n_kv * d, base = (size_t)s * a.count * row + (size_t)head * d;
-    for (uint32_t i = tid; i < 2 * d; i += 256) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (codes) u = *reinterpret_cast<const uint4*>(codes + 16 * i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w}, g = i % 64 / 16, n = i % 16;
-        float x[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) x[k] = codes ? ((float)((w[k / 4] >> (8 * (k % 4))) & 0xFF) - 128.0f) * scale : nothing;
+    __syncthreads();
+    const uint32_t per = d / 4, many = (uint32_t)(hi - lo) * per;  // four channels a thread
+    const size_t row = (size_t)a.kv.n_kv * d, base = ((size_t)s * a.count + (size_t)(lo - start)) * row + (size_t)head * d;
+    for (uint32_t u = tid; u < many; u += 256) {
+        const uint32_t r = divide(u, per), c = (u - r * per) * 4, t = (uint32_t)(lo - p0) + r;
+        uint32_t code[4];
         if (values) {
+            const uint8_t* from = image + c / 32 * 1056 + t % 16 / 4 * 256 + c % 16 * 16 + c % 32 / 16 * 8 + t / 16 * 4 + t % 4;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const int32_t p = p0 + (int32_t)(k % 8 / 4 * 16 + 4 * g + k % 4);
-                const size_t to = base + (size_t)(p - start) * row + i / 64 * 32 + k / 8 * 16 + n;
-                if (p < lo || p >= hi) continue;
-                if constexpr (BF16) static_cast<uint16_t*>(out)[to] = f32_to_bf16_bits(x[k]);
-                else static_cast<float*>(out)[to] = x[k];
-            }
+            for (int j = 0; j < 4; j++) code[j] = from[16 * j];
         } else {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(image + c / 8 * 264 + t * 8 + c % 8);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int32_t p = p0 + (int32_t)(k * 16 + n);
-                const size_t to = base + (size_t)(p - start) * row + i / 64 * 32 + g * 8;
-                if (p < lo || p >= hi) continue;
-                double y[8];
+            for (int j = 0; j < 4; j++) code[j] = (w >> (8 * j)) & 0xFF;
+        }
+        uint32_t w[4];
 #pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = x[8 * k + j];
-                store_run<BF16, 8>(out, to, a.vec, y);
-            }
+        for (int j = 0; j < 4; j++) {
+            const float x = page >= 0 ? ((float)code[j] - 128.0f) * scale : scale;
+            w[j] = BF16 ? f32_to_bf16_bits(x) : __float_as_uint(x);
+        }
+        const size_t to = base + r * row + c;
+        if constexpr (BF16) {
+            uint16_t* o = static_cast<uint16_t*>(out) + to;
+            if (a.vec) *reinterpret_cast<uint2*>(o) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            else o[0] = (uint16_t)w[0], o[1] = (uint16_t)w[1], o[2] = (uint16_t)w[2], o[3] = (uint16_t)w[3];
+        } else {
+            uint32_t* o = static_cast<uint32_t*>(out) + to;
+            if (a.vec) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+            else o[0] = w[0], o[1] = w[1], o[2] = w[2], o[3] = w[3];
         }
     }
 }
@@ -426,13 +436,15 @@ hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeVi
         return hipGetLastError();
     }
     const dim3 grid((unsigned)kv_places(b.rows, b.n_seqs, KV_BLOCK, 2), a.tasks);
-    if (bf16) kv_append_kernel<true><<<grid, 256, 0, s>>>(a);
-    else kv_append_kernel<false><<<grid, 256, 0, s>>>(a);
+    auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
+    if (kv.d <= 64) bf16 ? go(kv_append_kernel<true, 1>) : go(kv_append_kernel<false, 1>);
+    else if (kv.d <= 128) bf16 ? go(kv_append_kernel<true, 2>) : go(kv_append_kernel<false, 2>);
+    else bf16 ? go(kv_append_kernel<true, 4>) : go(kv_append_kernel<false, 4>);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvView& kv, const KvBatchView& b, size_t count, void* k_out, void* v_out, bool bf16, hipStream_t s) {
-    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)((count + 2 * KV_BLOCK - 2) / KV_BLOCK), reinterpret_cast<uintptr_t>(k_out) % 16 == 0};
+    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)((count + 2 * KV_BLOCK - 2) / KV_BLOCK), (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0};
     const dim3 grid(a.blocks * b.n_seqs, 2 * kv.n_kv);
     if (bf16) kv_read_kernel<true><<<grid, 256, 0, s>>>(a);
     else kv_read_kernel<false><<<grid, 256, 0, s>>>(a);

@@ -272,6 +272,8 @@ def _rows(name, t, width, rows, device):
     if t.get_device() != device:
         raise ValueError(f"{name}: on {t.device}, wanted cuda:{device}")
     shape, strides = t.shape, t.stride()
+    if len(shape) == 2 and shape[1] == width and strides[1] == 1 and shape[0] >= rows and strides[0] >= width:
+        return t.data_ptr(), strides[0], int(bf16)
     if len(shape) < 2 or shape[0] < rows or math.prod(shape[1:]) != width:
         raise ValueError(f"{name}: shape {tuple(shape)}, wanted at least {rows} rows of {width} values")
     dense = 1
@@ -684,10 +686,10 @@ class HipBackend:
         if dtype not in (_torch.float32, _torch.bfloat16):
             raise ValueError(f"dtype: {dtype}")
         both = _torch.empty((2, batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype, device=cache.k.device)
-        k, v = both.unbind(0)
-        if count and not self.lib.oxhip_dev_kv_read(self.ctx, cache.ref, batch.ref, count, k.data_ptr(), v.data_ptr(), int(dtype == _torch.bfloat16), self._stream_here()):
+        at = both.data_ptr()
+        if count and not self.lib.oxhip_dev_kv_read(self.ctx, cache.ref, batch.ref, count, at, at + both.nbytes // 2, int(dtype is _torch.bfloat16), self._stream_here()):
             raise RuntimeError(self.last_error())
-        return k, v
+        return both.unbind(0)
 
     def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
         """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of

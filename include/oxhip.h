@@ -326,7 +326,8 @@ int oxhip_dev_moe_routed(oxhip_ctx* ctx, oxhip_moe* m, const float* x, size_t t,
  * runs as Op::QkRope and Op::Attend, src/gpu_decode.rs) ---------------------------------------------------------------
  * The cache: pages of `page_tokens` tokens (a power of two, 32 at least), cut into blocks of 32. A block holds, for one key head, 32 d
  * codes of keys (and of values) and one f32 scale for each; a code u stands for (u - 128) * scale. d is a multiple of 32, 256 at most.
- * All arrays are the caller's, on the device, and start out as they like; k and v begin at multiples of 16 bytes. Codes of block
+ * All arrays are the caller's, on the device, and start out as they like; k and v begin at multiples of 16 bytes; a cache has fewer than
+ * 2^31 blocks. Codes of block
  * [page][head][block of the page], a byte each: the key of token t, channel c at c / 32 * 1024 + c % 32 / 8 * 256 + t % 16 * 16 +
  * t / 16 * 8 + c % 8, its value at c / 32 * 1024 + t % 16 / 4 * 256 + c % 16 * 16 + c % 32 / 16 * 8 + t / 16 * 4 + t % 4: a matrix
  * instruction's operands in the order in which a wave reads them. */
@@ -341,7 +342,8 @@ typedef struct {
 /* The sequences of a call and their rows (query rows, or new tokens). Sequence s has the rows row_start[s] .. row_start[s + 1] - 1 and
  * holds kv_len[s] tokens, these rows among them: its last row is token kv_len[s] - 1. Token p lies in page pages[s][p / page_tokens]. All three
  * arrays are on the device, so that a recorded plan's replays find the lengths of their step there; the calls read no more of them
- * than the sizes here say. Rows behind the last sequence are left as they are; a sequence may have no rows. */
+ * than the sizes here say, and they stay as they are until a call's work on the device is done. Rows behind the last sequence are left
+ * as they are; a sequence may have no rows. */
 typedef struct {
     size_t n_seqs, rows;
     const int32_t* row_start; /* [n_seqs + 1], ascending; or NULL: one row per sequence (rows == n_seqs) */
@@ -364,8 +366,8 @@ typedef struct {
  * tokens come in one call. Tokens that come later and do not fit double it until they do, and the codes that are there are rounded to the new scale:
  * none is further than a scale from its value, however many calls fill a block (half a scale where it did not grow). Scales stay within 2^-60 and
  * 2^61, larger values are cut to 127 * 2^60; NaN is stored as 0. A row whose position the table does not hold: q NaN, the key's rotated
- * channels 0. A page number outside the cache: that token is not stored. A page that a call appends to belongs to one sequence of it; pages
- * that are only read may be shared. */
+ * channels 0. A page number outside the cache: that token is not stored. A page that a call appends to stands once in one sequence's table;
+ * pages that are only read may be shared. */
 int oxhip_dev_kv_append(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* k, size_t k_stride, const void* v, size_t v_stride,
                         const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream);
 /* The values that the last `count` tokens of every sequence stand for, k_out / v_out [n_seqs, count, n_kv, d] of `dtype` (either may be NULL);
@@ -373,7 +375,7 @@ int oxhip_dev_kv_append(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv
 int oxhip_dev_kv_read(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, size_t count, void* k_out, void* v_out, int dtype, void* stream);
 
 /* What a row at position p sees of its sequence: the keys j with j < prefix[s], and those with first[row] <= j <= p and j > p - window. Their
- * scores: cap * tanh(score / cap), then less slopes[head] * |p - j|. A NULL (or 0) field sets no such rule. */
+ * scores: cap * tanh(score / cap) (cap within 2^-60 and 2^60), then less slopes[head] * |p - j|. A NULL (or 0) field sets no such rule. */
 typedef struct {
     float cap;
     const float* slopes;   /* [n_q] */
@@ -382,7 +384,7 @@ typedef struct {
     const int32_t* first;  /* [rows]: the first key of the row's document */
 } oxhip_attend_rules;
 /* out [rows, n_q, d] = softmax(scale * q K^T, as the rules have it) V over the cache, query head h reading key head h * n_kv / n_q (n_q a
- * multiple of n_kv); q and out of `dtype`, rows *_stride values apart (0 = dense). Scores, weights' sums and results are formed in
+ * multiple of n_kv); q and out (apart from each other) of `dtype`, rows *_stride values apart (0 = dense); |scale| <= 2^120. Scores, weights' sums and results are formed in
  * f32; f32 rows enter as two f16 values each (22 bits), bf16 rows as one. A row that sees no key gives zeros; one that would see a token of a page
  * outside the cache NaN. The stream's scratch (as oxhip_dev_decode_batch's) is made with the first call on it. */
 int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* q, size_t q_stride, size_t n_q, int dtype, float scale,

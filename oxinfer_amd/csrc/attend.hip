@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             load_query<F32>(a.q, at, a.vec & 1, v);
         }
     }
-    const float slope = RULES && a.slopes && live ? a.slopes[head] : 0.0f;
+    const float slope = RULES && a.slopes && live ? a.slopes[head] * LOG2E : 0.0f, cap = a.cap * LOG2E, cap_inv = a.cap > 0.0f ? 1.0f / cap : 0.0f;
     const uint32_t steps = b1 > b0 + wave ? (b1 - b0 - wave + NW - 1) / NW : 0;  // of this wave: blocks b0 + wave, + NW, ...
     // Where the wave's blocks lie, and their scales: for 64 of them at a time, a lane a block. A block's number and scales as scalars, one
     // block ahead of its use; a block of no page reads the cache's first (nothing is made of it).
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
 #pragma unroll
     for (int ks = 1; ks < KD; ks++) top = fmaxf(top, top_s[ks][n]);
     const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);  // (scaled to 2^14 at most)
-    const float factor = ldexpf(RULES ? a.scale : a.scale * LOG2E, ex - 14);     // of a score, with the key scale: natural units where RULES, else times log2 e
+    const float factor = ldexpf(a.scale * LOG2E, ex - 14);  // of a score, with the key scale, times log2 e
     if (wave < KD) {
         const float up = ldexpf(1.0f, 14 - ex);
         half8 hi8, lo8;
@@ -240,11 +240,17 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
 #pragma unroll
             for (int r = 0; r < 8; r++) {
                 x[r] = sc[r >> 2][r & 3];
-                if constexpr (RULES) {
-                    x[r] *= f;
-                    if (a.cap > 0.0f) x[r] = a.cap * tanh_of(x[r] / a.cap);
-                    x[r] -= slope * fabsf((float)(pos - (key0 + 16 * (r >> 2) + (r & 3))));
-                    x[r] *= LOG2E;
+                if constexpr (RULES) x[r] *= f;
+            }
+            if constexpr (RULES) {
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int r = 0; r < 8; r++) x[r] = cap * tanh_of(x[r] * cap_inv);
+                }
+                if (a.slopes) {
+                    const float far = (float)(pos - key0);
+#pragma unroll
+                    for (int r = 0; r < 8; r++) x[r] = fmaf(-slope, fabsf(far - (float)(16 * (r >> 2) + (r & 3))), x[r]);
                 }
             }
             const int32_t end = k0 + (int32_t)KV_BLOCK;
@@ -258,7 +264,8 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if constexpr (!RULES) top *= f;
             if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM))) {
-                const float to = fmaxf(m, entry_max(top) + lv), down = __builtin_amdgcn_exp2f(m - to);
+                // (an entry whose own scores need it: another row's do not change a row's bits)
+                const float own = entry_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
@@ -465,7 +472,6 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.counters = sc.counters;
     a.scale = call.scale;
     a.cap = call.cap;
-    a.n_q = call.n_q;
     a.g = call.n_q / kv.n_kv;
     a.window = call.window;
     const size_t size = call.bf16 ? 2 : 4;
@@ -490,7 +496,9 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.quantum = kv_quantum(units, most);
     if (!a.quantum) return hipErrorInvalidValue;
     a.many = 256 * split_places((int)kv.d / 32);
-    a.least = a.quantum < KV_LEAST ? KV_LEAST / a.quantum : 1;
+    // (blocks of wide heads hold more: 16 x 5 drafted rows of d = 256 24.9 us in parts of 16 blocks and more, 26.2 of 32)
+    const uint32_t least = kv.d > 128 ? KV_LEAST / 2 : KV_LEAST;
+    a.least = a.quantum < least ? least / a.quantum : 1;
     const uint64_t weight = (most + a.quantum - 1) / a.quantum, parts = (weight + a.least - 1) / a.least;  // of a tile, at most
     uint64_t grid = units * parts < units + a.many ? units * parts : units + a.many;
     if (a.many > MOST_SPLITS || 2 * a.many * CTR_STRIDE > sc.ncounters || 2 * (uint64_t)a.many * a.cols * (kv.d + 2) > sc.partial_floats || grid > 0x7FFFFFFFu) return hipErrorInvalidValue;

@@ -19,7 +19,7 @@ struct AttendArgs {
     float* partial;
     uint32_t* counters;
     float scale, cap;
-    uint32_t n_q, g, window, cols, vec, quantum, many, least, prompt;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
+    uint32_t g, window, cols, vec, quantum, many, least, prompt;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -86,7 +86,7 @@ __device__ __forceinline__ float tanh_of(float x) {
     const float a = fabsf(x), z = x * x;
     const float series = x + x * z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * (0.0218694885f - z * 0.00886323553f))));
     const float e = __builtin_amdgcn_exp2f(2.0f * LOG2E * a);
-    return a < 0.25f ? series : copysignf(1.0f - 2.0f / (e + 1.0f), x);
+    return a < 0.25f ? series : copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
 }
 
 // A value that all lanes hold alike, as a scalar.

@@ -28,7 +28,7 @@ __device__ __forceinline__ float half_sum(float v) {
 }
 
 // Two waves on a SIMD, where half of its registers hold what a wave keeps, cover each other's barriers and exponentials (a prompt of 4096 rows, 32
-// heads of 128 channels over 8: one wave of 64 entries a SIMD 225 us, two of 32 in workgroups of four waves 177, of eight 158; 0.87 PFLOP/s).
+// heads of 128 channels over 8: one wave of 64 entries a SIMD 225 us, two of 32 in workgroups of four waves 177, of eight 157; 0.88 PFLOP/s).
 // KD = d / 32; PLACES: waves on a SIMD.
 template <int KD, int WAVES, int PLACES, bool F32, bool RULES>
 __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(AttendArgs a) {
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
 
     // queries as operands, scaled to 2^14 at most
     half8 qh[KD * 2], ql[F32 ? KD * 2 : 1];
-    float factor;  // of a score, with the key scale: natural units where RULES, else times log2 e
+    float factor;  // of a score, with the key scale, times log2 e
     {
         float v[KD * 2][8], top = 0.0f;
 #pragma unroll
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
         top = half_max(top);
         const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);
         const float up = ldexpf(1.0f, 14 - ex);
-        factor = ldexpf(RULES ? a.scale : a.scale * LOG2E, ex - 14);
+        factor = ldexpf(a.scale * LOG2E, ex - 14);
 #pragma unroll
         for (int x = 0; x < KD * 2; x++)
 #pragma unroll
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
                 if constexpr (F32) ql[x][j] = (_Float16)(q - (float)qh[x][j]);
             }
     }
-    const float slope = RULES && a.slopes && live ? a.slopes[head] : 0.0f;
+    const float slope = RULES && a.slopes && live ? a.slopes[head] * LOG2E : 0.0f, cap = a.cap * LOG2E, cap_inv = a.cap > 0.0f ? 1.0f / cap : 0.0f;
 
     // Where blocks lie, and their scales: 64 blocks at a time, a lane a block; past the last block, the last one again.
     int32_t where_l = -1;
@@ -232,22 +232,26 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             constexpr int odd = decltype(parity)::value;
             const int32_t k0 = (int32_t)(kv_span_block(span, i) * KV_BLOCK);
             const float lv = lv_next[0], ks = ks_next[0];
-            // the step's codes (keys of block i + 2, values of block i), then the next ones on their way
+            // values of block i - 1; the step's codes (keys of block i + 2, values of block i), and the next ones on their way
+            values(v_s[odd ^ 1]);
             put(raw[odd], k_s[odd], v_s[odd]);
             ask(raw[odd], w_next[4], w_next[2]);
-            // values of block i - 1; the largest scores of block i
-            values(v_s[odd ^ 1]);
+            // the largest scores of block i
             const int32_t end = k0 + (int32_t)KV_BLOCK;
             const bool whole = (k0 >= lo_max && end <= hi_min) || end <= pre_max;
             const float f = factor * ks;
             if (w_next[0] < 0 && ((k0 < hi && end > lo) || k0 < pre)) l = __builtin_nanf("");  // no page of the cache
             if constexpr (RULES) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    float x = sc[r] * f;
-                    if (a.cap > 0.0f) x = a.cap * tanh_of(x / a.cap);
-                    x -= slope * fabsf((float)(pos - (k0 + (r >> 2) * 8 + 4 * (int32_t)h + (r & 3))));
-                    sc[r] = x * LOG2E;
+                for (int r = 0; r < 16; r++) sc[r] *= f;
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) sc[r] = cap * tanh_of(sc[r] * cap_inv);
+                }
+                if (a.slopes) {
+                    const float far = (float)(pos - (k0 + 4 * (int32_t)h));
+#pragma unroll
+                    for (int r = 0; r < 16; r++) sc[r] = fmaf(-slope, fabsf(far - (float)((r >> 2) * 8 + (r & 3))), sc[r]);
                 }
             }
             if (!whole) {
@@ -262,7 +266,8 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
             if constexpr (!RULES) top *= f;
             if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM))) {
-                const float to = fmaxf(m, half_max(top) + lv), down = __builtin_amdgcn_exp2f(m - to);
+                // (an entry whose own scores need it: another row's do not change a row's bits)
+                const float own = half_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
@@ -270,7 +275,10 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             }
             // keys of block i + 1; the weights of block i
             f32x16 ahead;
+            // (the wave that has matrix instructions to issue goes before the one that has exponentials)
+            __builtin_amdgcn_s_setprio(1);
             keys(k_s[odd ^ 1], ahead);
+            __builtin_amdgcn_s_setprio(0);
             const float unscale = __builtin_amdgcn_exp2f(-lv);
             const float shift = lv + HEAD_ROOM - m;
             float sum = 0.0f;
@@ -336,7 +344,7 @@ static hipError_t launch_waves(const AttendArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 // Eight waves turn the codes into operands half as often as four, where their tiles still fill the chip and are filled themselves: prompts of 2048
-// and 4096 rows (32 heads over 8, bf16) 64 and 177 us with four, 73 and 158 with eight; 4096 rows behind 8192 tokens 725 and 683.
+// and 4096 rows (32 heads over 8, bf16) 64 and 177 us with four, 73 and 157 with eight; 4096 rows behind 8192 tokens 725 and 683.
 template <int KD, bool F32, bool RULES>
 static hipError_t launch_prompt(const AttendArgs& a, hipStream_t s) {
     const uint64_t entries = (uint64_t)a.b.rows * a.g;

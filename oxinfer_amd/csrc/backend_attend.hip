@@ -115,13 +115,14 @@ int oxhip_dev_attend(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batc
     if (const char* why = check(kv, b, &kvv, &bv)) return refuse(who, why);
     if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "rows are f32 or bf16");
     if (!n_q || n_q % kv->n_kv || n_q > 65536) return refuse(who, "the query heads are a multiple of the key heads, 65536 at most");
-    if (!std::isfinite(scale)) return refuse(who, "the scale is a finite number");
+    if (!(std::fabs(scale) <= 0x1p120f)) return refuse(who, "the scale lies within -2^120 and 2^120");
     const size_t size = dtype == OXHIP_BF16 ? 2 : 4, width = n_q * kv->d;
     if (!aligned(q, size) || !aligned(out, size)) return refuse(who, "rows begin at multiples of their values' size");
     if ((q_stride && q_stride < width) || (out_stride && out_stride < width)) return refuse(who, "rows lie at least a row apart");
+    if (q == out) return refuse(who, "out lies apart from q");
     AttendCall call{};
     if (rules) {
-        if (!(rules->cap >= 0.0f) || !std::isfinite(rules->cap)) return refuse(who, "a cap is a finite number above 0, or 0 for none");
+        if (!(rules->cap == 0.0f || (rules->cap >= 0x1p-60f && rules->cap <= 0x1p60f))) return refuse(who, "a cap lies within 2^-60 and 2^60, or is 0 for none");
         if (!aligned(rules->slopes, 4) || !aligned(rules->prefix, 4) || !aligned(rules->first, 4)) return refuse(who, "an array of 4-byte values at an odd address");
         call.cap = rules->cap;
         call.slopes = rules->slopes;

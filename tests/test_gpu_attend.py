@@ -325,6 +325,23 @@ def test_prompts_pages_outside_the_cache_and_queries_that_are_not_numbers(be):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [[5, 3], [300, 5]])
+def test_a_rows_bits_do_not_depend_on_the_rows_beside_it(be, n, dtype):
+    from oxinfer_amd import hip
+    w = kv_ref.World([900, 64], 2, 128, page=32, seed=3, n=n)
+    cache, batch = w.tensors(hip)
+    q = torch.randn(w.rows, 8 * 128, device="cuda").to(dtype)
+    want = be.attend(cache, batch, q)
+    for part in (slice(0, None, 3), slice(1, None, 2)):
+        other = q.clone()
+        other[part] *= 64
+        kept = torch.ones(w.rows, dtype=torch.bool)
+        kept[part] = False
+        got = be.attend(cache, batch, other)
+        assert torch.equal(got[kept], want[kept]) and not torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_prompts_by_a_recorded_plan_and_the_same_bits_every_time(be, dtype):
     from oxinfer_amd import hip
     w = kv_ref.World([1000, 500, 700], 16, 128, page=64, seed=3, n=[300, 2, 150])

@@ -41,6 +41,16 @@ int main() {
             if (std::scanf("%d %d %d %d %u %u %u", &s, &r0, &r1, &len, &rows, &pages, &shift) != 7) return 1;
             const KvSeq q = kv_part(s, r0, r1, len, rows, pages, shift);
             std::printf("%d %d %d %d\n", q.s, q.row0, q.n, q.len);
+        } else if (!std::strcmp(what, "weight")) {
+            int n, len, prefix;
+            unsigned window, quantum, g;
+            if (std::scanf("%d %d %u %d %u %u", &n, &len, &window, &prefix, &quantum, &g) != 6) return 1;
+            const KvSeq q{0, 0, n, len};
+            std::printf("%u %u\n", kv_weight(q, window, prefix, quantum), kv_tiles(q, g));
+        } else if (!std::strcmp(what, "quantum")) {
+            unsigned long long tiles, blocks;
+            if (std::scanf("%llu %llu", &tiles, &blocks) != 2) return 1;
+            std::printf("%u\n", kv_quantum(tiles, blocks));
         } else {
             int id;
             unsigned most, n_pages, block, shift;
@@ -99,6 +109,33 @@ def test_spans_of_blocks(ask):
         assert got == sorted(want), (pre, lo, hi)
 
 
+def test_weights_of_tiles(ask):
+    """A sequence's weight is no less than the blocks that any of its rows sees (window and prefix as the launch has them), and no
+    more than all of its blocks; its tiles hold its entries. Lengths below the rows (rows at negative positions) count all blocks."""
+    rng = np.random.default_rng(3)
+    cases = [(1, 0, 0, 0), (1, 1, 0, 0), (1, 33, 1, 0), (5, 3, 2, 0), (1, 2**31 - 64, 0, 0), (1, 2**31 - 64, 2**31 - 2, 2**31 - 1), (4, 1000, 100, 2**31 - 1), (4, 1000, 100, -7), (300, 64, 10, 5)]
+    cases += [(int(rng.integers(1, 400)), int(rng.integers(0, 5000)), int(rng.integers(0, 700)), int(rng.integers(-50, 5000))) for _ in range(400)]
+    gs = [int(rng.choice([1, 3, 8, 17])) for _ in cases]
+    quanta = [int(2 ** rng.integers(0, 4)) for _ in cases]
+    got = ask([f"weight {n} {ln} {w} {p} {q} {g}" for (n, ln, w, p), q, g in zip(cases, quanta, gs)])
+    for (n, ln, w, p), q, g, (weight, tiles) in zip(cases, quanta, gs, got):
+        everything = -(-ln // 32)
+        lo = max(ln - n - w + 1, 0) // 32 if w else 0
+        seen = everything - lo + min(-(-max(min(p, ln), 0) // 32), lo)  # of all its rows together
+        assert max(1, -(-seen // q)) <= weight <= max(1, -(-everything // q)), (n, ln, w, p, q)
+        assert tiles == -(-n * g // 16)
+
+
+def test_quanta_of_launches(ask):
+    """32 bits hold the sum of all tiles' weights, in the smallest power of two of blocks that does it; none for a launch that is too large."""
+    cases = [(1, 1), (1, 2**26), (31, 2**26), (32, 2**26), (2**20, 2**26), (2**30 - 1, 2**26), (2**30, 1), (2**40, 2**26)]
+    for (tiles, blocks), (q,) in zip(cases, ask([f"quantum {t} {b}" for t, b in cases])):
+        if tiles >= 2**30:
+            assert q == 0
+        else:
+            assert q & (q - 1) == 0 and q and tiles * -(-blocks // q) < 2**31 and (q == 1 or tiles * -(-blocks // (q // 2)) >= 2**31)
+
+
 def test_unsound_sequences_and_pages(ask):
     """Rows outside the batch, lengths outside the table and pages outside the cache are cut off before anything is read with them."""
     parts = [("0 0 4 7 4 2 0", [0, 0, 4, 7]), ("1 -5 3 7 4 2 0", [1, 0, 3, 7]), ("1 2 9 7 4 2 0", [1, 2, 2, 7]), ("1 9 2 7 4 2 0", [1, 9, 0, 7]), ("2 5 9 7 4 2 0", [2, 5, 0, 7]),
@@ -135,7 +172,7 @@ def said(lib, ok):
 
 
 BAD_KV = [dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(k=P + 8), dict(v=P + 1), dict(k_scale=P + 2), dict(d=0), dict(d=48), dict(d=288), dict(page_tokens=16), dict(page_tokens=0),
-          dict(page_tokens=96), dict(page_tokens=2**31), dict(n_kv=0), dict(n_kv=20000), dict(n_pages=0), dict(n_pages=2**31)]
+          dict(page_tokens=96), dict(page_tokens=2**31), dict(n_kv=0), dict(n_kv=20000), dict(n_pages=0), dict(n_pages=2**31), dict(n_pages=2**29, n_kv=2), dict(n_pages=2**31 // 256 + 1, n_kv=4, page_tokens=2048)]
 BAD_B = [dict(kv_len=None), dict(pages=None), dict(kv_len=P + 1), dict(row_start=P + 2), dict(n_seqs=0), dict(n_seqs=2**25, rows=2**25), dict(max_pages=0), dict(max_pages=2**31), dict(max_pages=2**26), dict(rows=4),
          dict(rows=2**29, row_start=P)]
 OF_KV = [(a, ()) for a in BAD_KV] + [((), a) for a in BAD_B]
@@ -146,7 +183,7 @@ def test_caches_and_batches_that_are_refused(lib, kv, b):
     from oxinfer_amd import hip
     good, bad = structs(hip), structs(hip, kv, b)
     for cache, batch, null in ((*good, True), (*bad, False)):
-        for ok in (lambda: lib.oxhip_dev_attend(None, C.byref(cache), C.byref(batch), P, 0, 4, 0, 1.0, None, P, 0, None),
+        for ok in (lambda: lib.oxhip_dev_attend(None, C.byref(cache), C.byref(batch), P, 0, 4, 0, 1.0, None, 2 * P, 0, None),
                    lambda: lib.oxhip_dev_kv_append(None, C.byref(cache), C.byref(batch), P, 0, P, 0, None, 0, None, 0, 0, 0, None, None),
                    lambda: lib.oxhip_dev_kv_read(None, C.byref(cache), C.byref(batch), 5, P, P, 0, None)):
             assert ("null context" in said(lib, ok())) == null
@@ -156,13 +193,13 @@ def test_rows_and_rules_that_are_refused(lib):
     from oxinfer_amd import hip
     cache, batch = (C.byref(s) for s in structs(hip))
 
-    def attend(q=P, qs=0, n_q=4, dtype=0, scale=0.5, rules=None, out=P, os=0):
+    def attend(q=P, qs=0, n_q=4, dtype=0, scale=0.5, rules=None, out=2 * P, os=0):
         return said(lib, lib.oxhip_dev_attend(None, cache, batch, q, qs, n_q, dtype, scale, C.byref(hip.AttendRulesC(**rules)) if rules is not None else None, out, os, None))
 
-    for good in (dict(), dict(dtype=1, q=P + 2, out=P + 2), dict(qs=256, os=300), dict(scale=-2.0), dict(scale=0.0), dict(rules=dict(cap=30.0, slopes=P, window=2**40, prefix=P, first=P))):
+    for good in (dict(), dict(dtype=1, q=P + 2, out=2 * P + 2), dict(qs=256, os=300), dict(scale=-2.0), dict(scale=0.0), dict(rules=dict(cap=30.0, slopes=P, window=2**40, prefix=P, first=P))):
         assert "null context" in attend(**good), good
     for bad in (dict(q=None), dict(out=None), dict(q=P + 2), dict(out=P + 1, dtype=1), dict(n_q=0), dict(n_q=3), dict(n_q=2**17), dict(dtype=2), dict(dtype=-1), dict(scale=float("inf")), dict(scale=float("nan")),
-                dict(qs=255), dict(os=1), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=float("nan"))), dict(rules=dict(cap=float("inf"))), dict(rules=dict(slopes=P + 1)), dict(rules=dict(first=P + 2))):
+                dict(qs=255), dict(os=1), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=float("nan"))), dict(rules=dict(cap=float("inf"))), dict(rules=dict(cap=1e30)), dict(rules=dict(cap=1e-30)), dict(scale=1.4e36), dict(scale=-1e38), dict(out=P, q=P),  dict(rules=dict(slopes=P + 1)), dict(rules=dict(first=P + 2))):
         assert "null context" not in attend(**bad), bad
 
     def append(k=P, ks=0, v=P, vs=0, q=P, qs=0, out=P, os=0, n_q=4, dtype=0, rope=None):

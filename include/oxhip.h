@@ -396,10 +396,10 @@ int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_ba
  *            repetition[row]; one that occurs n > 0 times behind the prompt: l - frequency[row] * n - presence[row]. Ids outside the vocabulary
  *            count for nothing.
  *   bias:    entries bias_start[row] .. bias_start[row + 1] - 1 of bias_id / bias are added; of an id that is named twice, the last.
- *   allowed: bit id % 32 of word id / 32 of mask allowed_row[row] (NULL: mask `row`; -1: no mask): where it is 0 the logit becomes -infinity. A mask
+ *   allowed: bit id % 32 of word id / 32 of mask allowed_row[row] (NULL: mask `row`; negative: no mask): where it is 0 the logit becomes -infinity. A mask
  *            number of n_allowed or more allows nothing. */
 typedef struct {
-    const int32_t* history;     /* [rows], history_stride ids apart */
+    const int32_t* history;     /* [rows, history_stride] */
     size_t history_stride;
     const int32_t* history_len; /* [rows] */
     const int32_t* prompt_len;  /* [rows]; NULL: no prompt */

@@ -258,7 +258,8 @@ def _array(name, t, dtype, device=None, count=None):
     """A dense device tensor of `dtype` (with `count` values, if given): its pointer, or None for None."""
     if t is None:
         return None
-    if t.dtype is not dtype or not t.is_contiguous() or t.get_device() < 0 or (device is not None and t.get_device() != device) or (count is not None and t.numel() != count):
+    on = t.get_device()
+    if t.dtype is not dtype or not t.is_contiguous() or on < 0 or (on != device and device is not None) or (count is not None and t.numel() != count):
         raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}; wanted {dtype}"
                          f"{'' if count is None else f' of {count} values'} on cuda:{'*' if device is None else device}")
     return t.data_ptr()
@@ -664,7 +665,7 @@ class HipBackend:
             n_q = q_width // cache.d
             qp, qs, qd = _rows("q", q, n_q * cache.d, rows, dev)
             if q_out is None:
-                q_out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = q.new_empty(q.shape)
                 op, os_ = q_out.data_ptr(), q_width
             else:
                 op, os_, od = _rows("q_out", q_out, n_q * cache.d, rows, dev)
@@ -685,7 +686,7 @@ class HipBackend:
         dtype = dtype or _torch.float32
         if dtype not in (_torch.float32, _torch.bfloat16):
             raise ValueError(f"dtype: {dtype}")
-        both = _torch.empty((2, batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype, device=cache.k.device)
+        both = cache.k_scale.new_empty((2, batch.n_seqs, count, cache.n_kv, cache.d), dtype=dtype)
         at = both.data_ptr()
         if count and not self.lib.oxhip_dev_kv_read(self.ctx, cache.ref, batch.ref, count, at, at + both.nbytes // 2, int(dtype is _torch.bfloat16), self._stream_here()):
             raise RuntimeError(self.last_error())
@@ -699,7 +700,7 @@ class HipBackend:
         n_q = width // cache.d
         qp, qs, qd = _rows("q", q, n_q * cache.d, batch.rows, dev)
         if out is None:
-            out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
             op, os_ = out.data_ptr(), width
         else:
             op, os_, od = _rows("out", out, n_q * cache.d, batch.rows, dev)
@@ -731,10 +732,10 @@ class HipBackend:
             if od != ld:
                 raise ValueError("logits and out have one type")
         elif want_out:
-            out = _torch.empty((t, vocab), dtype=logits.dtype, device=logits.device)
+            out = logits.new_empty((t, vocab))
             op, os_ = out.data_ptr(), vocab
         if want_next:
-            best = _torch.empty(t, dtype=i32, device=logits.device)
+            best = logits.new_empty(t, dtype=i32)
         elif op is None:
             raise ValueError("neither the adjusted logits nor the best tokens are wanted")
         rules = None
@@ -744,8 +745,9 @@ class HipBackend:
                 if history.dim() != 2 or history.shape[0] != t:
                     raise ValueError(f"history: shape {tuple(history.shape)}, wanted [{t}, most]")
                 r.history, r.history_stride, r.history_len = _array("history", history, i32, dev), history.shape[1], _array("history_len", history_len, i32, dev, t)
-            r.prompt_len = _array("prompt_len", prompt_len, i32, dev, t)
-            r.repetition, r.presence, r.frequency = _array("repetition", repetition, f32, dev, t), _array("presence", presence, f32, dev, t), _array("frequency", frequency, f32, dev, t)
+            for name, value, kind in (("prompt_len", prompt_len, i32), ("repetition", repetition, f32), ("presence", presence, f32), ("frequency", frequency, f32)):
+                if value is not None:
+                    setattr(r, name, _array(name, value, kind, dev, t))
             if bias_start is not None or bias_id is not None or bias is not None:
                 n = bias_id.numel() if bias_id is not None else 0
                 r.bias_start, r.bias_id, r.bias, r.n_bias = _array("bias_start", bias_start, i32, dev, t + 1), _array("bias_id", bias_id, i32, dev), _array("bias", bias, f32, dev, n), n

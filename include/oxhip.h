@@ -346,7 +346,7 @@ typedef struct {
  * as they are; a sequence may have no rows. */
 typedef struct {
     size_t n_seqs, rows;
-    const int32_t* row_start; /* [n_seqs + 1], ascending; or NULL: one row per sequence (rows == n_seqs) */
+    const int32_t* row_start; /* [n_seqs + 1], ascending (attend leaves rows out otherwise); or NULL: one row per sequence (rows == n_seqs) */
     const int32_t* kv_len;    /* [n_seqs] */
     const int32_t* pages;     /* [n_seqs, max_pages]; entries that no token needs may hold anything */
     size_t max_pages;

@@ -56,7 +56,9 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
         if (wave == 0) {
             KvSeq q{};
             uint32_t w = 1;
+            bool falls = false;
             if (s0 + lane < a.b.n_seqs) {
+                falls = a.b.row_start && a.b.row_start[s0 + lane + 1] < a.b.row_start[s0 + lane];
                 q = kv_seq(a.b, (int32_t)(s0 + lane), a.kv.shift);
                 if ((uint32_t)q.n * (uint64_t)g >= a.prompt) q.n = 0;  // (attend_prompt_kernel's)
                 w = kv_weight(q, a.window, a.window && a.prefix ? a.prefix[s0 + lane] : 0, a.quantum);
@@ -64,7 +66,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             seq_s[0][lane] = q.row0;
             seq_s[1][lane] = q.n;
             seq_s[2][lane] = q.len;
-            seq_s[3][lane] = (int32_t)w;
+            seq_s[3][lane] = __ballot(falls) ? 0 : (int32_t)w;  // (a weight is 1 at least)
         }
         __syncthreads();
         mine.row0 = seq_s[0][lane];
@@ -77,6 +79,9 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     uint32_t total = 0;
     for (uint32_t from = 0; from < a.b.n_seqs; from += 64) {
         load(from);
+        // Row numbers that do not ascend may come to more tiles than the launch has workgroups for, and parts that never arrive would leave their
+        // counters behind for later calls: nothing is done then.
+        if (!last(mine_weight)) return;
         total += last(lanes_upto(mine_units * mine_weight));
     }
     const uint32_t size = max(scalar(divide(total + a.many - 1, a.many)), a.least);

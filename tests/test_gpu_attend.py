@@ -324,6 +324,24 @@ def test_prompts_pages_outside_the_cache_and_queries_that_are_not_numbers(be):
     assert torch.equal(got[same], want.view(w.rows, 128, 128)[same]) and got[7, 1].isnan().all() and got[200, 0].isnan().all()
 
 
+@pytest.mark.parametrize("seqs", [3, 70])
+def test_row_numbers_that_do_not_ascend_leave_nothing_behind(be, seqs):
+    """Sequences that claim each other's rows: nothing is written, and the next call of the same stream is right (parts that wait for others
+    meet by counters)."""
+    from oxinfer_amd import hip
+    w = kv_ref.World([3000] * seqs, 2, 64, page=64, seed=4, n=[2] * seqs)
+    cache, batch = w.tensors(hip, ragged=True)
+    q = torch.randn(w.rows, 8 * 64, device="cuda")
+    want = be.attend(cache, batch, q)
+    for at, value in ((seqs - 1, 0), (1, 2 * seqs), (0, 2**31 - 1), (seqs, -(2**31))):
+        start = batch.row_start.clone()
+        start[at] = value
+        out = torch.full_like(q, 7.5)
+        be.attend(cache, hip.KvBatch(batch.kv_len, batch.pages, rows=w.rows, row_start=start), q, out=out)
+        assert (out == 7.5).all()
+        assert torch.equal(be.attend(cache, batch, q), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n", [[5, 3], [300, 5]])
 def test_a_rows_bits_do_not_depend_on_the_rows_beside_it(be, n, dtype):

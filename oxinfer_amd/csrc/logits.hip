@@ -46,6 +46,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void logits_kernel(LogitArgs a) {
     __shared__ uint32_t count[SLICE];
     __shared__ uint64_t best_s[LOGIT_THREADS / 64];
     __shared__ uint32_t last_s;
+    __shared__ uint32_t met_s[LOGIT_THREADS / 64];
     const uint32_t tid = threadIdx.x, slice = blockIdx.x / a.rows, row = blockIdx.x % a.rows, v0 = slice * SLICE;
     const uint32_t here = min(SLICE, a.vocab - v0);
     auto at = [&](int k) { return (uint32_t)(W * (tid + (k / W) * LOGIT_THREADS) + k % W); };  // of the slice: a thread's k-th logit
@@ -120,12 +121,26 @@ __global__ __launch_bounds__(LOGIT_THREADS) void logits_kernel(LogitArgs a) {
             if (t < here) f(i, t, a.bias[i]);
         }
     };
-    if (counted) {
-        const uint32_t n = (uint32_t)min((size_t)max(len, 0), a.history_stride), said = min((uint32_t)max(prompt, 0), n);
+    const uint32_t n = counted ? (uint32_t)min((size_t)max(len, 0), a.history_stride) : 0u, said = min((uint32_t)max(prompt, 0), n);
+    // What the slice has: bit 0 tokens of the history, bit 1 biases. Most slices have none of a few biases, and then none of their three barriers
+    // (64 rows of 151936 bf16, 2000 tokens of history and up to 20 biases each: 28.3 -> 25.7 us).
+    uint32_t met = 0;
+    if (counted || biased) {
+        bool any = n > HELD * LOGIT_THREADS;  // (those that no register holds are not looked at for this)
 #pragma unroll
-        for (uint32_t k = 0; k < HELD; k++) place[k] = tid + k * LOGIT_THREADS < n ? place[k] : NOWHERE;
+        for (uint32_t k = 0; k < HELD; k++) {
+            place[k] = tid + k * LOGIT_THREADS < n ? place[k] : NOWHERE;
+            any = any || place[k] < here;
+        }
+        const uint32_t flags = (__ballot(any) ? 1u : 0u) | (__ballot(bias_place < here || b1 > b0 + LOGIT_THREADS) ? 2u : 0u);
+        if ((tid & 63) == 0) met_s[tid >> 6] = flags;
         tokens(0, n, [&](uint32_t t) { count[t] = 1; });
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < LOGIT_THREADS / 64; w++) met |= met_s[w];
+        met = (uint32_t)__builtin_amdgcn_readfirstlane((int)met);
+    }
+    if (met & 1) {
         tokens(said, n, [&](uint32_t t) { atomicAdd(&count[t], 1u); });
         __syncthreads();
         tokens(0, n, [&](uint32_t t) {
@@ -138,7 +153,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void logits_kernel(LogitArgs a) {
         });
         __syncthreads();
     }
-    if (biased) {
+    if (met & 2) {
         biases([&](uint32_t, uint32_t t, float) { count[t] = 0; });
         __syncthreads();
         biases([&](uint32_t i, uint32_t t, float) { atomicMax(&count[t], i + 1); });
@@ -153,7 +168,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void logits_kernel(LogitArgs a) {
     for (int k = 0; k < PER; k += W) {
         const uint32_t i = at(k);
         if (i >= here) continue;
-        if (counted || biased) {
+        if (met) {
 #pragma unroll
             for (int j = 0; j < W; j += 4) {
                 const float4 f = *reinterpret_cast<const float4*>(&x_s[i + j]);

@@ -121,6 +121,21 @@ def test_long_histories(be, most):
     check(be, torch.randn(3, 5000, device="cuda"), make(3, 5000, most=most, biases=300, seed=most))
 
 
+@pytest.mark.parametrize("split", [(0, 0), (4096, 512), (4200, 600), (5000, 700)])
+def test_slices_that_only_some_rules_reach(be, split):
+    """Histories and biases that lie in one slice of the vocabulary at first, and in others behind their first entries."""
+    r = np.random.default_rng(7)
+    hist, bias = np.empty((2, 5000), np.int32), np.empty(1400, np.int32)
+    hist[:, : split[0]], hist[:, split[0] :] = r.integers(0, 4096, (2, split[0])), r.integers(4096, 8192, (2, 5000 - split[0]))
+    ids = r.integers(12288, 16384, (2, 700))
+    ids[:, : split[1]] = r.integers(0, 4096, (2, split[1]))
+    bias[:] = ids.reshape(-1)
+    a = dict(history=hist, history_len=np.array([5000, 4500], np.int32), prompt_len=np.array([10, 4400], np.int32), repetition=np.array([1.3, 0.9], np.float32),
+             presence=np.array([0.5, -0.25], np.float32), frequency=np.array([0.01, 0.25], np.float32), bias_start=np.array([0, 700, 1400], np.int32), bias_id=bias,
+             bias=r.normal(size=1400).astype(np.float32))
+    check(be, torch.from_numpy(r.normal(size=(2, 17000)).astype(np.float32)).cuda(), a)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("strided", [1, 8])
 def test_strides(be, strided, dtype):

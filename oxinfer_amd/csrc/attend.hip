@@ -150,11 +150,12 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     // Where the wave's blocks lie, and their scales: for 64 of them at a time, a lane a block. A block's number and scales as scalars, one
     // block ahead of its use; a block of no page reads the cache's first (nothing is made of it).
     int32_t at = -1;
-    float ksc = 0.0f, lvs = 0.0f;
+    float ksc = 1.0f, lvs = 0.0f;
     auto page_of = [&](uint32_t t) { return t + lane < steps ? kv_page(a.b, a.kv, (int32_t)s, kv_span_block(span, b0 + wave + (t + lane) * NW)) : -1; };
     auto scales_of = [&](uint32_t t, int32_t page) {
         float vsc = 1.0f;
         at = -1;
+        ksc = 1.0f;  // (of a block of no page, too: what rows do not see of it is -infinity times this)
         if (page >= 0) {
             at = (int32_t)kv_block_index(a.kv, page, kvh, kv_span_block(span, b0 + wave + (t + lane) * NW));
             ksc = a.kv.k_scale[at];

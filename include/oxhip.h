@@ -325,7 +325,8 @@ int oxhip_dev_moe_routed(oxhip_ctx* ctx, oxhip_moe* m, const float* x, size_t t,
 /* ---- attention over an 8-bit cache (between the q / k / v linears and the output projection: what the reference's graph
  * runs as Op::QkRope and Op::Attend, src/gpu_decode.rs) ---------------------------------------------------------------
  * The cache: pages of `page_tokens` tokens (a power of two, 32 at least), cut into blocks of 32. A block holds, for one key head, 32 d
- * codes of keys (and of values) and one f32 scale for each; a code u stands for (u - 128) * scale. d is a multiple of 32, 256 at most.
+ * codes of keys (and of values) and one f32 scale for each; a code u stands for (u - 128) * scale. A scale is 0 or more and below 2^61; to oxhip_dev_attend
+ * one under 2^-60 is 0. d is a multiple of 32, 256 at most.
  * All arrays are the caller's, on the device, and start out as they like; k and v begin at multiples of 16 bytes; a cache has fewer than
  * 2^31 blocks. Codes of block
  * [page][head][block of the page], a byte each: the key of token t, channel c at c / 32 * 1024 + c % 32 / 8 * 256 + t % 16 * 16 +

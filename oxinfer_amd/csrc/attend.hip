@@ -158,13 +158,13 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
         ksc = 1.0f;  // (of a block of no page, too: what rows do not see of it is -infinity times this)
         if (page >= 0) {
             at = (int32_t)kv_block_index(a.kv, page, kvh, kv_span_block(span, b0 + wave + (t + lane) * NW));
-            ksc = a.kv.k_scale[at];
+            ksc = key_scale(a.kv.k_scale[at]);
             vsc = a.kv.v_scale[at];
         }
         return vsc;
     };
     auto locate = [&](uint32_t t, int32_t& where, float& ks_b, float& lv) {
-        if ((t & 63) == 0) lvs = __builtin_amdgcn_logf(scales_of(t, page_of(t)));  // (log2)
+        if ((t & 63) == 0) lvs = value_log(scales_of(t, page_of(t)));  // (log2)
         const uint32_t from = t & 63;
         where = __builtin_amdgcn_readlane(at, from);
         ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), from));
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     float m = NO_MAX, l = 0.0f;
     // keys are on request from the block before, values from before the scores
     {
-        lvs = __builtin_amdgcn_logf(vsc0);
+        lvs = value_log(vsc0);
         int32_t where_next;
         float ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), 0)), lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), 0)), ks_next, lv_next;
         for (uint32_t t = 0; t < steps; t++) {
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             // no page of the cache: rows that would see it come out as NaN
             l = none && ((k0 < hi && k0 + (int32_t)KV_BLOCK > lo) || k0 < pre) ? __builtin_nanf("") : l;
             // scores: of keys k0 + 4 grp + r and k0 + 16 + 4 grp + r
-            const float f = factor * ks_b;
+            const float f = RULES ? factor * ks_b : fmaxf(factor * ks_b, LEAST_FACTOR);
             float x[8];  // scores times log2 e; without rules, what the products gave: their factor is above 0 and joins the exponent
             const int32_t key0 = k0 + 4 * (int32_t)grp;
 #pragma unroll
@@ -270,13 +270,22 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if constexpr (!RULES) top *= f;
-            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM))) {
+            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM)) || no_values(lv)) {
                 // (an entry whose own scores need it: another row's do not change a row's bits)
                 const float own = entry_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
                 for (int c = 0; c < 2 * KD; c++) acc[c] *= down;
+                if (no_values(lv)) {  // (weights for the sum alone)
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        sum += __builtin_amdgcn_exp2f(RULES ? x[r] + (lv + HEAD_ROOM - m) : fmaf(x[r], f, lv + HEAD_ROOM - m));
+                        x[r] = -__builtin_inff();
+                    }
+                    l += sum * __builtin_amdgcn_exp2f(-lv);
+                }
             }
             const float shift = lv + HEAD_ROOM - m;
             half8 ph, pl;

@@ -27,6 +27,14 @@ constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from 
 constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
 
+// Scales under KV_SCALE_MIN count as 0. A block of such keys scores 0; a masked score times its factor is to stay -infinity, so a factor is LEAST_FACTOR at
+// least (the products of a row and a key are below 2^29: what that makes of them no weight shows). A block of such values has a logarithm that no
+// other has, its weights are taken for the sum alone.
+__device__ __forceinline__ float key_scale(float held) { return held < KV_SCALE_MIN ? 0.0f : held; }
+constexpr float LEAST_FACTOR = 0x1p-100f, NO_VALUES = -61.0f;
+__device__ __forceinline__ float value_log(float held) { return held < KV_SCALE_MIN ? NO_VALUES : __builtin_amdgcn_logf(held); }
+__device__ __forceinline__ bool no_values(float log) { return __float_as_uint(log) == __builtin_bit_cast(uint32_t, NO_VALUES); }
+
 // Eight codes as f16 values, exactly.
 __device__ __forceinline__ half8 code_values(uint32_t a, uint32_t b) {
     const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};

@@ -142,11 +142,11 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             const int32_t page = kv_page(a.b, a.kv, s, blk);
             if (page >= 0) {
                 where_l = (int32_t)kv_block_index(a.kv, page, kvh, blk);
-                ksc_l = a.kv.k_scale[where_l];
+                ksc_l = key_scale(a.kv.k_scale[where_l]);
                 vsc = a.kv.v_scale[where_l];
             }
         }
-        lvs_l = __builtin_amdgcn_logf(vsc);  // (log2)
+        lvs_l = value_log(vsc);  // (log2)
     };
     // A block's codes, by 16 bytes a thread: unit u of its keys, then of its values.
     uint4 raw[2][REGS];
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             // the largest scores of block i
             const int32_t end = k0 + (int32_t)KV_BLOCK;
             const bool whole = (k0 >= lo_max && end <= hi_min) || end <= pre_max;
-            const float f = factor * ks;
+            const float f = RULES ? factor * ks : fmaxf(factor * ks, LEAST_FACTOR);
             if (w_next[0] < 0 && ((k0 < hi && end > lo) || k0 < pre)) l = __builtin_nanf("");  // no page of the cache
             if constexpr (RULES) {
 #pragma unroll
@@ -265,13 +265,22 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
 #pragma unroll
             for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
             if constexpr (!RULES) top *= f;
-            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM))) {
+            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM)) || no_values(lv)) {
                 // (an entry whose own scores need it: another row's do not change a row's bits)
                 const float own = half_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
                 for (int c = 0; c < KD; c++) acc[c] *= down;
+                if (no_values(lv)) {  // (weights for the sum alone)
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        sum += __builtin_amdgcn_exp2f(RULES ? sc[r] + (lv + HEAD_ROOM - m) : fmaf(sc[r], f, lv + HEAD_ROOM - m));
+                        sc[r] = -__builtin_inff();
+                    }
+                    l += sum * __builtin_amdgcn_exp2f(-lv);
+                }
             }
             // keys of block i + 1; the weights of block i
             f32x16 ahead;

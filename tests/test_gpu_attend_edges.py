@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests import kv_ref
+from tests.test_gpu_attend import check
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,32 @@ def test_a_missing_page_that_part_of_a_prompts_tile_sees(be, dtype, rules):
     """Rows from position 101 on, four to a wave's tile: one of these holds 157 .. 160."""
     w = kv_ref.World([400, 64], 16, 128, page=32, seed=3, n=[299, 5])
     missing_pages(be, w, 8, dtype, [(0, 5)], window=100, **rules)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [0.0, 1e-42, 1e-25])
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("n,n_kv,d,g", [([1, 1], 2, 64, 3), ([5, 40], 2, 64, 3), ([299, 5], 16, 128, 8)], ids=["one", "few", "prompt"])
+def test_scales_of_zero(be, n, n_kv, d, g, which, value, dtype):
+    """Blocks whose scale is 0, or under the least one, which counts as 0: their keys score 0, their values are 0. Blocks of the first tokens, and the last, of
+    which rows see a part."""
+    w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
+    for s in range(2):
+        for b in (0, (w.lens[s] - 1) // 32):
+            if which != "v":
+                w.ks[w.table[s, b], :, 0] = value
+            if which != "k":
+                w.vs[w.table[s, b], :, 0] = value
+    heads = None if d == 64 else [0, 60, 127]
+    sequence = w.sequence
+    w.sequence = lambda s: [x * (np.repeat(scales[w.table[s, : -(-w.lens[s] // 32)], :, 0], 32, 0)[: w.lens[s]] >= 2.0**-60)[..., None] for x, scales in zip(sequence(s), (w.ks, w.vs))]
+    check(be, w, g, dtype, ragged=True, heads=heads)
+    check(be, w, g, dtype, ragged=True, heads=heads, cap=20.0, window=70)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_new_cache_holds_zeros(be, dtype):
+    from oxinfer_amd import hip
+    cache = be.kv_cache(4, 2, 64)
+    batch = hip.KvBatch(torch.tensor([130, 7], dtype=torch.int32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda").repeat(2, 1))
+    assert (be.attend(cache, batch, torch.randn(2, 4 * 64, device="cuda").to(dtype)) == 0).all()

@@ -191,14 +191,13 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     float top = top_s[0][n];
 #pragma unroll
     for (int ks = 1; ks < KD; ks++) top = fmaxf(top, top_s[ks][n]);
-    const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);  // (scaled to 2^14 at most)
-    const float factor = ldexpf(a.scale * LOG2E, ex - 14);  // of a score, with the key scale, times log2 e
+    const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;  // (scaled to 2^14 at most)
+    const ScoreFactor factor(a.scale, ex - 14);
     if (wave < KD) {
-        const float up = ldexpf(1.0f, 14 - ex);
         half8 hi8, lo8;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float x = v[j] * up;
+            const float x = ldexpf(v[j], 14 - ex);
             hi8[j] = (_Float16)x;
             if constexpr (F32) lo8[j] = (_Float16)(x - (float)hi8[j]);
         }
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             // no page of the cache: rows that would see it come out as NaN
             l = none && ((k0 < hi && k0 + (int32_t)KV_BLOCK > lo) || k0 < pre) ? __builtin_nanf("") : l;
             // scores: of keys k0 + 4 grp + r and k0 + 16 + 4 grp + r
-            const float f = RULES ? factor * ks_b : fmaxf(factor * ks_b, LEAST_FACTOR);
+            const float f = factor.template of<RULES>(ks_b);
             float x[8];  // scores times log2 e; without rules, what the products gave: their factor is above 0 and joins the exponent
             const int32_t key0 = k0 + 4 * (int32_t)grp;
 #pragma unroll

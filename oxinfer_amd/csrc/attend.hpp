@@ -27,13 +27,25 @@ constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from 
 constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
 
-// Scales under KV_SCALE_MIN count as 0. A block of such keys scores 0; a masked score times its factor is to stay -infinity, so a factor is LEAST_FACTOR at
-// least (the products of a row and a key are below 2^29: what that makes of them no weight shows). A block of such values has a logarithm that no
-// other has, its weights are taken for the sum alone.
+// Scales under KV_SCALE_MIN count as 0. A block of such keys scores 0. A block of such values has a logarithm that no other has, its weights are taken for
+// the sum alone.
 __device__ __forceinline__ float key_scale(float held) { return held < KV_SCALE_MIN ? 0.0f : held; }
-constexpr float LEAST_FACTOR = 0x1p-100f, NO_VALUES = -61.0f;
+constexpr float NO_VALUES = -61.0f;
 __device__ __forceinline__ float value_log(float held) { return held < KV_SCALE_MIN ? NO_VALUES : __builtin_amdgcn_logf(held); }
 __device__ __forceinline__ bool no_values(float log) { return __float_as_uint(log) == __builtin_bit_cast(uint32_t, NO_VALUES); }
+
+// What makes a score, times log2 e, of the product of a row's operands and a block's codes: the call's scale, the key scale, and the power of two that the
+// row's operands were divided by. One at a time they may leave f32, so the powers are added first. A masked score times its factor is to stay -infinity: without rules
+// it is above 0 (products are below 2^29, so that no weight shows a factor of 2^-100), and it is finite, so that a product of 0 stays 0.
+struct ScoreFactor {
+    float scale;  // 0.5 to 1 times log2 e, with the call's sign
+    int power;
+    __device__ __forceinline__ ScoreFactor(float call, int row) : scale(__builtin_amdgcn_frexp_mantf(call) * LOG2E), power(__builtin_amdgcn_frexp_expf(call) + row) {}
+    template <bool RULES>
+    __device__ __forceinline__ float of(float key) const {
+        return __builtin_amdgcn_fmed3f(ldexpf(scale * key, power), RULES ? -0x1p127f : 0x1p-100f, 0x1p127f);
+    }
+};
 
 // Eight codes as f16 values, exactly.
 __device__ __forceinline__ half8 code_values(uint32_t a, uint32_t b) {

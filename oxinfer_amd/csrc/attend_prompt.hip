@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
 
     // queries as operands, scaled to 2^14 at most
     half8 qh[KD * 2], ql[F32 ? KD * 2 : 1];
-    float factor;  // of a score, with the key scale, times log2 e
+    int row_power;  // what they are divided by
     {
         float v[KD * 2][8], top = 0.0f;
 #pragma unroll
@@ -116,14 +116,13 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[x][j]));
         }
         top = half_max(top);
-        const int ex = max(top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0, -40);
-        const float up = ldexpf(1.0f, 14 - ex);
-        factor = ldexpf(a.scale * LOG2E, ex - 14);
+        const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
+        row_power = ex - 14;
 #pragma unroll
         for (int x = 0; x < KD * 2; x++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float q = v[x][j] * up;
+                const float q = ldexpf(v[x][j], 14 - ex);
                 qh[x][j] = (_Float16)q;
                 if constexpr (F32) ql[x][j] = (_Float16)(q - (float)qh[x][j]);
             }
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             // the largest scores of block i
             const int32_t end = k0 + (int32_t)KV_BLOCK;
             const bool whole = (k0 >= lo_max && end <= hi_min) || end <= pre_max;
-            const float f = RULES ? factor * ks : fmaxf(factor * ks, LEAST_FACTOR);
+            const float f = ScoreFactor(a.scale, row_power).template of<RULES>(ks);
             if (w_next[0] < 0 && ((k0 < hi && end > lo) || k0 < pre)) l = __builtin_nanf("");  // no page of the cache
             if constexpr (RULES) {
 #pragma unroll

@@ -95,3 +95,13 @@ def test_a_new_cache_holds_zeros(be, dtype):
     cache = be.kv_cache(4, 2, 64)
     batch = hip.KvBatch(torch.tensor([130, 7], dtype=torch.int32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda").repeat(2, 1))
     assert (be.attend(cache, batch, torch.randn(2, 4 * 64, device="cuda").to(dtype)) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q,scale,k", [(-90, 90, 0), (-90, 37, 53), (-140, 117, 23), (-70, 10, 60), (-64, 4, 60), (-100, 40, 60), (100, -50, -50), (50, 2, -52), (110, -110, 0), (120, -120, 0)])
+@pytest.mark.parametrize("n,n_kv,d,g", [([5, 40], 2, 64, 3), ([299, 5], 16, 128, 8)], ids=["few", "prompt"])
+def test_rows_scales_and_keys_of_any_size(be, n, n_kv, d, g, q, scale, k, dtype):
+    """Powers of two on the rows, the scale and the keys whose product is 1."""
+    w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
+    w.ks *= np.float32(2.0**k)
+    check(be, w, g, dtype, ragged=True, heads=None if d == 64 else [0, 60, 127], loud=2.0 ** (q + 1), scale=2.0 ** (scale - 3))

@@ -12,6 +12,7 @@
 // hardly ever behind a wave's first blocks): of weights rounded to f16, small ones keep as many bits as there are.
 // f32 rows: q and p' go in as two f16 values each (value and residual, 22 bits), twice the matrix instructions, which the reads hide.
 // bf16 rows: as one (11 bits, where the rows and results have 8); the rows are scaled by a power of two each, so that nothing overflows.
+#include <cmath>
 #include <type_traits>
 
 #include "attend.hpp"
@@ -151,6 +152,8 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     // block ahead of its use; a block of no page reads the cache's first (nothing is made of it).
     int32_t at = -1;
     float ksc = 1.0f, lvs = 0.0f;
+    float m = NO_MAX, l = 0.0f, bar;
+    bool watch = false;  // a block without values is among the wave's
     auto page_of = [&](uint32_t t) { return t + lane < steps ? kv_page(a.b, a.kv, (int32_t)s, kv_span_block(span, b0 + wave + (t + lane) * NW)) : -1; };
     auto scales_of = [&](uint32_t t, int32_t page) {
         float vsc = 1.0f;
@@ -158,13 +161,20 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
         ksc = 1.0f;  // (of a block of no page, too: what rows do not see of it is -infinity times this)
         if (page >= 0) {
             at = (int32_t)kv_block_index(a.kv, page, kvh, kv_span_block(span, b0 + wave + (t + lane) * NW));
-            ksc = key_scale(a.kv.k_scale[at]);
+            ksc = key_scale(a.kv.k_scale[at]) * a.scale;
             vsc = a.kv.v_scale[at];
         }
         return vsc;
     };
+    auto look_out = [&]() {
+        watch = watch || __builtin_amdgcn_ballot_w64(no_values(lvs));
+        bar = bar_of(m, watch);
+    };
     auto locate = [&](uint32_t t, int32_t& where, float& ks_b, float& lv) {
-        if ((t & 63) == 0) lvs = value_log(scales_of(t, page_of(t)));  // (log2)
+        if ((t & 63) == 0) {
+            lvs = value_log(scales_of(t, page_of(t)));  // (log2)
+            look_out();
+        }
         const uint32_t from = t & 63;
         where = __builtin_amdgcn_readlane(at, from);
         ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), from));
@@ -191,13 +201,12 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     float top = top_s[0][n];
 #pragma unroll
     for (int ks = 1; ks < KD; ks++) top = fmaxf(top, top_s[ks][n]);
-    const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;  // (scaled to 2^14 at most)
-    const ScoreFactor factor(a.scale, ex - 14);
+    const int down = row_power(top), power = a.power + down;
     if (wave < KD) {
         half8 hi8, lo8;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float x = ldexpf(v[j], 14 - ex);
+            const float x = ldexpf(v[j], -down);
             hi8[j] = (_Float16)x;
             if constexpr (F32) lo8[j] = (_Float16)(x - (float)hi8[j]);
         }
@@ -209,10 +218,10 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
     f32x4 acc[2 * KD];
 #pragma unroll
     for (int t = 0; t < 2 * KD; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = NO_MAX, l = 0.0f;
     // keys are on request from the block before, values from before the scores
     {
         lvs = value_log(vsc0);
+        look_out();
         int32_t where_next;
         float ks_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), 0)), lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lvs), 0)), ks_next, lv_next;
         for (uint32_t t = 0; t < steps; t++) {
@@ -240,7 +249,7 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             // no page of the cache: rows that would see it come out as NaN
             l = none && ((k0 < hi && k0 + (int32_t)KV_BLOCK > lo) || k0 < pre) ? __builtin_nanf("") : l;
             // scores: of keys k0 + 4 grp + r and k0 + 16 + 4 grp + r
-            const float f = factor.template of<RULES>(ks_b);
+            float f = score_factor<RULES>(ks_b, power);
             float x[8];  // scores times log2 e; without rules, what the products gave: their factor is above 0 and joins the exponent
             const int32_t key0 = k0 + 4 * (int32_t)grp;
 #pragma unroll
@@ -269,24 +278,35 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if constexpr (!RULES) top *= f;
-            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM)) || no_values(lv)) {
+            float shift = lv + HEAD_ROOM - m;
+            if (__builtin_amdgcn_ballot_w64(top + lv > bar)) {
                 // (an entry whose own scores need it: another row's do not change a row's bits)
                 const float own = entry_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
                 for (int c = 0; c < 2 * KD; c++) acc[c] *= down;
+                shift = lv + HEAD_ROOM - m;
+                bar = bar_of(m, watch);
+                if (__builtin_amdgcn_ballot_w64(is_far(m))) {  // (the scores become exponents)
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        const float apart = ((RULES ? x[r] : x[r] * f) - m) + (lv + HEAD_ROOM), near = RULES ? x[r] + shift : fmaf(x[r], f, shift);
+                        x[r] = !is_far(m) ? near : apart > F16_ROOM ? F16_ROOM : apart;
+                    }
+                    f = 1.0f;
+                    shift = 0.0f;
+                }
                 if (no_values(lv)) {  // (weights for the sum alone)
                     float sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 8; r++) {
-                        sum += __builtin_amdgcn_exp2f(RULES ? x[r] + (lv + HEAD_ROOM - m) : fmaf(x[r], f, lv + HEAD_ROOM - m));
+                        sum += __builtin_amdgcn_exp2f(RULES ? x[r] + shift : fmaf(x[r], f, shift));
                         x[r] = -__builtin_inff();
                     }
                     l += sum * __builtin_amdgcn_exp2f(-lv);
                 }
             }
-            const float shift = lv + HEAD_ROOM - m;
             half8 ph, pl;
             float sum = 0.0f;
 #pragma unroll
@@ -485,7 +505,9 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.first = call.first;
     a.partial = sc.partial;
     a.counters = sc.counters;
-    a.scale = call.scale;
+    int power;
+    a.scale = std::frexp(call.scale, &power) * LOG2E;
+    a.power = power;
     a.cap = call.cap;
     a.g = call.n_q / kv.n_kv;
     a.window = call.window;

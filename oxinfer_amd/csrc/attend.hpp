@@ -18,7 +18,8 @@ struct AttendArgs {
     const int32_t *prefix, *first;
     float* partial;
     uint32_t* counters;
-    float scale, cap;
+    float scale, cap;  // scale: the mantissa of the call's, times log2 e
+    int32_t power;     // the call's scale's
     uint32_t g, window, cols, vec, quantum, many, least, prompt;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
 };
 
@@ -26,6 +27,13 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from it that 2^(NO_MAX - score) is 0
 constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
+// Maxima past this are far: a step of f32 there is 1/8 and more, and an exponent made in one rounding of a score, or of the maximum and the value scale's
+// logarithm, may be off by one, past what f16 holds. Far rows take score less maximum first, which is exact for those that count; what the
+// maximum's own rounding leaves (the logarithm at most) is cut off below 2^16.
+constexpr float FAR = 0x1p20f, F16_ROOM = 15.9f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > FAR && m > NO_MAX; }
+// What a block's largest score may be before a step leaves the common path: the maximum is to be set anew, or `each` step has what that path does not do.
+__device__ __forceinline__ float bar_of(float m, bool each) { return each || is_far(m) ? -__builtin_inff() : m + (MOST_ROOM - HEAD_ROOM); }
 
 // Scales under KV_SCALE_MIN count as 0. A block of such keys scores 0. A block of such values has a logarithm that no other has, its weights are taken for
 // the sum alone.
@@ -34,18 +42,16 @@ constexpr float NO_VALUES = -61.0f;
 __device__ __forceinline__ float value_log(float held) { return held < KV_SCALE_MIN ? NO_VALUES : __builtin_amdgcn_logf(held); }
 __device__ __forceinline__ bool no_values(float log) { return __float_as_uint(log) == __builtin_bit_cast(uint32_t, NO_VALUES); }
 
-// What makes a score, times log2 e, of the product of a row's operands and a block's codes: the call's scale, the key scale, and the power of two that the
-// row's operands were divided by. One at a time they may leave f32, so the powers are added first. A masked score times its factor is to stay -infinity: without rules
-// it is above 0 (products are below 2^29, so that no weight shows a factor of 2^-100), and it is finite, so that a product of 0 stays 0.
-struct ScoreFactor {
-    float scale;  // 0.5 to 1 times log2 e, with the call's sign
-    int power;
-    __device__ __forceinline__ ScoreFactor(float call, int row) : scale(__builtin_amdgcn_frexp_mantf(call) * LOG2E), power(__builtin_amdgcn_frexp_expf(call) + row) {}
-    template <bool RULES>
-    __device__ __forceinline__ float of(float key) const {
-        return __builtin_amdgcn_fmed3f(ldexpf(scale * key, power), RULES ? -0x1p127f : 0x1p-100f, 0x1p127f);
-    }
-};
+// What makes a score, times log2 e, of the product of a row's operands and a block's codes: the call's scale (its mantissa times log2 e, which the key scales
+// are multiplied with) and two powers of two, the call's and the one that the row's operands were divided by. Either may lie outside f32, so they are added first. A masked
+// score times its factor is to stay -infinity: without rules it is above 0 (products are below 2^29, so that no weight shows a factor of 2^-100).
+template <bool RULES>
+__device__ __forceinline__ float score_factor(float scaled_key, int power) {
+    const float f = ldexpf(scaled_key, power);
+    return RULES ? f : fmaxf(f, 0x1p-100f);
+}
+// The power of two by which a row whose largest value is `top` is divided, so that it lies below 2^14; a row of zeros has a factor that is not infinite.
+__device__ __forceinline__ int row_power(float top) { return top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 14 : -1000; }
 
 // Eight codes as f16 values, exactly.
 __device__ __forceinline__ half8 code_values(uint32_t a, uint32_t b) {

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
 
     // queries as operands, scaled to 2^14 at most
     half8 qh[KD * 2], ql[F32 ? KD * 2 : 1];
-    int row_power;  // what they are divided by
+    int power;  // of their scores' factor
     {
         float v[KD * 2][8], top = 0.0f;
 #pragma unroll
@@ -116,13 +116,13 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[x][j]));
         }
         top = half_max(top);
-        const int ex = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
-        row_power = ex - 14;
+        const int down = row_power(top);
+        power = a.power + down;
 #pragma unroll
         for (int x = 0; x < KD * 2; x++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float q = ldexpf(v[x][j], 14 - ex);
+                const float q = ldexpf(v[x][j], -down);
                 qh[x][j] = (_Float16)q;
                 if constexpr (F32) ql[x][j] = (_Float16)(q - (float)qh[x][j]);
             }
@@ -132,6 +132,8 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
     // Where blocks lie, and their scales: 64 blocks at a time, a lane a block; past the last block, the last one again.
     int32_t where_l = -1;
     float ksc_l = 1.0f, lvs_l = 0.0f;
+    float m = NO_MAX, bar;
+    bool watch = false;  // a block without values is among the wave's
     auto look = [&](uint32_t from) {
         float vsc = 1.0f;
         where_l = -1;
@@ -141,11 +143,13 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             const int32_t page = kv_page(a.b, a.kv, s, blk);
             if (page >= 0) {
                 where_l = (int32_t)kv_block_index(a.kv, page, kvh, blk);
-                ksc_l = key_scale(a.kv.k_scale[where_l]);
+                ksc_l = key_scale(a.kv.k_scale[where_l]) * a.scale;
                 vsc = a.kv.v_scale[where_l];
             }
         }
         lvs_l = value_log(vsc);  // (log2)
+        watch = watch || __builtin_amdgcn_ballot_w64(no_values(lvs_l));
+        bar = bar_of(m, watch);
     };
     // A block's codes, by 16 bytes a thread: unit u of its keys, then of its values.
     uint4 raw[2][REGS];
@@ -172,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
     };
     f32x16 acc[KD], sc;
     half8 ph[2], pl[2];
-    float m = NO_MAX, l = 0.0f;
+    float l = 0.0f;
     ph[0] = ph[1] = half8{0, 0, 0, 0, 0, 0, 0, 0};
     if constexpr (F32) pl[0] = pl[1] = half8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             // the largest scores of block i
             const int32_t end = k0 + (int32_t)KV_BLOCK;
             const bool whole = (k0 >= lo_max && end <= hi_min) || end <= pre_max;
-            const float f = ScoreFactor(a.scale, row_power).template of<RULES>(ks);
+            float f = score_factor<RULES>(ks, power);
             if (w_next[0] < 0 && ((k0 < hi && end > lo) || k0 < pre)) l = __builtin_nanf("");  // no page of the cache
             if constexpr (RULES) {
 #pragma unroll
@@ -264,18 +268,30 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
 #pragma unroll
             for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
             if constexpr (!RULES) top *= f;
-            if (__builtin_amdgcn_ballot_w64(top + lv > m + (MOST_ROOM - HEAD_ROOM)) || no_values(lv)) {
+            float shift = lv + HEAD_ROOM - m;
+            if (__builtin_amdgcn_ballot_w64(top + lv > bar)) {
                 // (an entry whose own scores need it: another row's do not change a row's bits)
                 const float own = half_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= down;
 #pragma unroll
                 for (int c = 0; c < KD; c++) acc[c] *= down;
+                shift = lv + HEAD_ROOM - m;
+                bar = bar_of(m, watch);
+                if (__builtin_amdgcn_ballot_w64(is_far(m))) {  // (the scores become exponents)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const float apart = ((RULES ? sc[r] : sc[r] * f) - m) + (lv + HEAD_ROOM), near = RULES ? sc[r] + shift : fmaf(sc[r], f, shift);
+                        sc[r] = !is_far(m) ? near : apart > F16_ROOM ? F16_ROOM : apart;
+                    }
+                    f = 1.0f;
+                    shift = 0.0f;
+                }
                 if (no_values(lv)) {  // (weights for the sum alone)
                     float sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        sum += __builtin_amdgcn_exp2f(RULES ? sc[r] + (lv + HEAD_ROOM - m) : fmaf(sc[r], f, lv + HEAD_ROOM - m));
+                        sum += __builtin_amdgcn_exp2f(RULES ? sc[r] + shift : fmaf(sc[r], f, shift));
                         sc[r] = -__builtin_inff();
                     }
                     l += sum * __builtin_amdgcn_exp2f(-lv);
@@ -288,7 +304,6 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             keys(k_s[odd ^ 1], ahead);
             __builtin_amdgcn_s_setprio(0);
             const float unscale = __builtin_amdgcn_exp2f(-lv);
-            const float shift = lv + HEAD_ROOM - m;
             float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; u++)

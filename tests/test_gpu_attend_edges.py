@@ -105,3 +105,53 @@ def test_rows_scales_and_keys_of_any_size(be, n, n_kv, d, g, q, scale, k, dtype)
     w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
     w.ks *= np.float32(2.0**k)
     check(be, w, g, dtype, ragged=True, heads=None if d == 64 else [0, 60, 127], loud=2.0 ** (q + 1), scale=2.0 ** (scale - 3))
+
+
+def one_key(be, w, g, dtype, scale, slopes=None, heads=None, loud=2.0, cached=None):
+    """Scores so far apart that a row's softmax is its best key's alone, by a margin past all errors of f32 scores: the results are that key's values.
+    A weight's error: the rounding to f16 (2^-11, or 2^-21 in two), and what the logarithm and exponentials of the value scale leave, 16 u of 84."""
+    from oxinfer_amd import hip
+    rng = np.random.default_rng(11)
+    n_q = w.n_kv * g
+    cache, batch = w.tensors(hip, ragged=True)
+    q = torch.from_numpy(loud * rng.normal(size=(w.rows, n_q * w.d))).to("cuda", dtype)
+    up = None if slopes is None else torch.from_numpy(np.asarray(slopes, np.float32)).cuda()
+    got = be.attend(cache, batch, q, scale=scale, slopes=up).double().cpu().numpy().reshape(w.rows, n_q, w.d)
+    hq, pos = q.double().cpu().numpy().reshape(w.rows, n_q, w.d), positions(w)
+    half = dtype == torch.bfloat16
+    rel = (2.0**-11 if half else 2.0**-21) + 2 * 8 * 84 * 2.0**-24 + (2.0**-8 if half else 2.0**-24)
+    checked = 0
+    for s in range(len(w.lens)):
+        k, v = w.sequence(s)
+        for r in range(w.start[s], w.start[s + 1]):
+            for h in range(n_q) if heads is None else heads:
+                j = np.arange(pos[r] + 1)
+                score = scale * (k[j, h // g] @ hq[r, h])
+                mass = abs(scale) * (np.abs(k[j, h // g]) @ np.abs(hq[r, h])).max()
+                if slopes is not None:
+                    bias = float(np.float32(slopes[h])) * (pos[r] - j)
+                    score, mass = score - bias, mass + bias.max()
+                best = np.argsort(score)[-2:]
+                if len(best) == 2 and score[best[1]] - score[best[0]] < 2.0**-16 * mass + 100:
+                    continue
+                checked += 1
+                want = v[best[-1], h // g]
+                assert (np.abs(got[r, h] - want) <= rel * np.abs(want)).all(), (r, h)
+    assert checked >= w.rows * (n_q if heads is None else len(heads)) // 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [2.0**14, 2.0**19, 2.0**22, -(2.0**22), 2.0**30, 2.0**39, 2.0**60, -(2.0**100)])
+@pytest.mark.parametrize("n,n_kv,d,g", [([1, 1], 2, 64, 3), ([5, 40], 2, 64, 3), ([299, 5], 16, 128, 8)], ids=["one", "few", "prompt"])
+def test_scores_far_from_zero(be, n, n_kv, d, g, scale, dtype):
+    w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
+    one_key(be, w, g, dtype, scale, heads=None if d == 64 else [0, 60, 127])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("slope", [1e3, 1e7, 1e9, 1e20, 1e35])
+@pytest.mark.parametrize("n,n_kv,d,g", [([1, 1], 2, 64, 3), ([5, 40], 2, 64, 3), ([299, 5], 16, 128, 8)], ids=["one", "few", "prompt"])
+def test_steep_slopes(be, n, n_kv, d, g, slope, dtype):
+    """A row's own key is what is left."""
+    w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
+    one_key(be, w, g, dtype, d**-0.5, slopes=np.full(n_kv * g, slope), heads=None if d == 64 else [0, 60, 127])

@@ -741,13 +741,19 @@ class HipBackend:
         rules = None
         if history is not None or bias_start is not None or allowed is not None:
             r = LogitRulesC()
+            empty = False
             if history is not None:
-                if history.dim() != 2 or history.shape[0] != t:
-                    raise ValueError(f"history: shape {tuple(history.shape)}, wanted [{t}, most]")
-                r.history, r.history_stride, r.history_len = _array("history", history, i32, dev), history.shape[1], _array("history_len", history_len, i32, dev, t)
+                if history.dim() != 2 or history.shape[0] != t or history_len is None:
+                    raise ValueError(f"history: shape {tuple(history.shape)}{', without history_len' if history_len is None else ''}, wanted [{t}, most] and a length for each row")
+                empty = not history.shape[1]  # (no token at all: the tensor has no address, and no logit a penalty)
+                at, lens = _array("history", history, i32, dev), _array("history_len", history_len, i32, dev, t)
+                if not empty:
+                    r.history, r.history_stride, r.history_len = at, history.shape[1], lens
             for name, value, kind in (("prompt_len", prompt_len, i32), ("repetition", repetition, f32), ("presence", presence, f32), ("frequency", frequency, f32)):
                 if value is not None:
-                    setattr(r, name, _array(name, value, kind, dev, t))
+                    at = _array(name, value, kind, dev, t)
+                    if not empty:
+                        setattr(r, name, at)
             if bias_start is not None or bias_id is not None or bias is not None:
                 n = bias_id.numel() if bias_id is not None else 0
                 r.bias_start, r.bias_id, r.bias, r.n_bias = _array("bias_start", bias_start, i32, dev, t + 1), _array("bias_id", bias_id, i32, dev), _array("bias", bias, f32, dev, n), n

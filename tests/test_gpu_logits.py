@@ -224,3 +224,20 @@ def test_the_bindings_refusals(be):
                 dict(allowed=i[:, None]), dict(allowed_row=i), dict(out=x.bfloat16()), dict(want_out=False, want_next=False), dict(logits=x.half()), dict(logits=x.cpu())):
         with pytest.raises((ValueError, RuntimeError)):
             be.adjust_logits(**(dict(logits=x) | bad))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("others", [False, True])
+def test_a_history_without_room(be, others, dtype):
+    """A sampler's first step without a prompt: no token has come, so no penalty touches a logit; the other rules hold."""
+    x = torch.randn(3, 5000, device="cuda").to(dtype)
+    a = {k: torch.from_numpy(v).cuda() for k, v in make(3, 5000).items()}
+    names = ("history", "history_len", "prompt_len", "repetition", "presence", "frequency")
+    rest = {k: v for k, v in a.items() if k not in names} if others else {}
+    none = dict(history=a["history"][:, :0], **{k: a[k] for k in names[1:]})
+    want, best = be.adjust_logits(x, **rest)
+    got, again = be.adjust_logits(x, **none, **rest)
+    assert torch.equal(got, want) and torch.equal(best, again)
+    for bad in (dict(history_len=None), dict(history_len=a["history_len"][:2]), dict(repetition=a["prompt_len"]), dict(history=a["history"][:2, :0]), dict(history=a["history"][:, :0].long())):
+        with pytest.raises(ValueError):
+            be.adjust_logits(x, **(none | bad))

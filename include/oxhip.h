@@ -414,8 +414,9 @@ typedef struct {
     const int32_t* allowed_row; /* [rows] */
 } oxhip_logit_rules;
 /* logits [rows, vocab] of `dtype`, rows `stride` values apart (0 = dense), to `out` (the same buffer, one apart from it, or NULL), and the id of
- * each row's largest resulting logit to `next` (or NULL): the lowest of equal ones, NaN passed over, -1 where all are -infinity. With `next`, the rows are
- * 16384 at most; scratch as oxhip_dev_attend's. */
+ * each row's largest resulting logit to `next` (or NULL): the lowest of equal ones, NaN passed over, -1 where all are -infinity. A vocabulary has 2^31 - 4096
+ * ids at most. With `next`, there are 16384 rows at most, and 2^21 slices of 4096 logits in all of them (rows * ceil(vocab / 4096)); scratch as
+ * oxhip_dev_attend's. */
 int oxhip_dev_logits(oxhip_ctx* ctx, const void* logits, size_t stride, void* out, size_t out_stride, size_t rows, size_t vocab, int dtype,
                      const oxhip_logit_rules* rules, int32_t* next, void* stream);
 

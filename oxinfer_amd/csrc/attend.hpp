@@ -25,7 +25,7 @@ struct AttendArgs {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float NO_MAX = -1.7e38f;      // below any score, and far enough from it that 2^(NO_MAX - score) is 0
-constexpr uint32_t MOST_SPLITS = 512;  // workgroups of a launch, and so of a tile
+constexpr uint32_t MOST_SPLITS = 512;  // parts of a tile: the workgroups that the chip holds, at most
 constexpr float HEAD_ROOM = 11.0f, MOST_ROOM = 15.0f;  // log2 of a weight when the maximum is set, and before it is set anew
 // Maxima past this are far: a step of f32 there is 1/8 and more, and an exponent made in one rounding of a score, or of the maximum and the value scale's
 // logarithm, may be off by one, past what f16 holds. Far rows take score less maximum first, which is exact for those that count; what the

@@ -154,7 +154,7 @@ int oxhip_dev_logits(oxhip_ctx* c, const void* logits, size_t stride, void* out,
     if (!logits || (!out && !next)) return refuse(who, "null argument");
     if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "logits are f32 or bf16");
     const size_t size = dtype == OXHIP_BF16 ? 2 : 4;
-    if (!vocab || vocab > 0x7FFFF000u || rows > ((size_t)1 << 24)) return refuse(who, "a vocabulary of 1 to 2^31 - 4097, 2^24 rows at most");
+    if (!vocab || vocab > 0x7FFFF000u || rows > ((size_t)1 << 24)) return refuse(who, "a vocabulary of 1 to 2^31 - 4096, 2^24 rows at most");
     if (!aligned(logits, size) || !aligned(out, size) || !aligned(next, 4)) return refuse(who, "rows begin at multiples of their values' size");
     if ((stride && stride < vocab) || (out_stride && out_stride < vocab)) return refuse(who, "rows lie at least a row apart");
     LogitArgs a{};
@@ -195,6 +195,8 @@ int oxhip_dev_logits(oxhip_ctx* c, const void* logits, size_t stride, void* out,
         a.n_allowed = (uint32_t)r.n_allowed;
         a.allowed_row = r.allowed_row;
     }
+    const char* too_many = "with next, 16384 rows at most, and 2^21 slices of 4096 logits in all of them";
+    if (next && (rows > LOGIT_NEXT_ROWS || rows * logit_slices(vocab) > LOGIT_NEXT_SLICES)) return refuse(who, too_many);
     if (!c) return refuse(who, "null context");
     if (!rows) return 1;
     OnDevice on(c->device);
@@ -203,7 +205,7 @@ int oxhip_dev_logits(oxhip_ctx* c, const void* logits, size_t stride, void* out,
     if (next) {
         DecodeScratch* sc = parts(c, s, who);
         if (!sc) return 0;
-        if (rows * CTR_STRIDE > sc->ncounters || rows * logit_slices(vocab) * 2 > sc->partial_floats) return refuse(who, "too many rows for `next` in one call (16384 at most)");
+        if (rows * CTR_STRIDE > sc->ncounters || rows * logit_slices(vocab) * 2 > sc->partial_floats) return refuse(who, too_many);
         a.best = reinterpret_cast<uint64_t*>(sc->partial);
         a.counters = sc->counters;
     }

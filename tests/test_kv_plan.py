@@ -246,3 +246,15 @@ def test_the_bindings_own_checks():
         hip.KvBatch(z(3), z(3, 4, t=torch.int32))
     with pytest.raises(ValueError, match="wanted"):
         hip.Rope(z(3, 4, 2, t=torch.float64))
+
+
+def test_how_many_rows_have_a_best_token(lib):
+    """With `next`, rows and their slices of 4096 logits have to fit the stream's scratch; the refusal names both bounds."""
+    def logits(rows, vocab, next=P):
+        return said(lib, lib.oxhip_dev_logits(None, P, 0, P, 0, rows, vocab, 0, None, next, None))
+
+    for rows, vocab in ((16384, 1), (16384, 524288), (8192, 2**20), (4, 2**31 - 4096)):
+        assert "null context" in logits(rows, vocab), (rows, vocab)
+    for rows, vocab in ((16385, 1), (16384, 524289), (8193, 2**20), (5, 2**31 - 4096)):
+        assert "16384 rows" in logits(rows, vocab) and "2^21 slices" in logits(rows, vocab), (rows, vocab)
+    assert "2^31 - 4096" in logits(1, 2**31 - 4095) and "null context" in logits(16385, 5, next=None)

@@ -528,8 +528,7 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
         if (e != hipSuccess || b.n_seqs == 1) return e;
     }
     a.cols = b.row_start ? 16u : min(16u, a.g);
-    const uint64_t tiles = b.row_start ? kv_places((uint64_t)b.rows * a.g, b.n_seqs, 16, 1) : (uint64_t)b.n_seqs * ((a.g + 15) / 16);
-    const uint64_t units = tiles * kv.n_kv, most = (uint64_t)b.max_pages << kv.shift;  // (at most that many)
+    const uint64_t units = kv_units(b.row_start, b.rows, b.n_seqs, a.g, kv.n_kv), most = (uint64_t)b.max_pages << kv.shift;  // (at most that many)
     a.quantum = kv_quantum(units, most);
     if (!a.quantum) return hipErrorInvalidValue;
     a.many = 256 * split_places((int)kv.d / 32);
@@ -538,7 +537,7 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     a.least = a.quantum < least ? least / a.quantum : 1;
     const uint64_t weight = (most + a.quantum - 1) / a.quantum, parts = (weight + a.least - 1) / a.least;  // of a tile, at most
     uint64_t grid = units * parts < units + a.many ? units * parts : units + a.many;
-    if (a.many > MOST_SPLITS || 2 * a.many * CTR_STRIDE > sc.ncounters || 2 * (uint64_t)a.many * a.cols * (kv.d + 2) > sc.partial_floats || grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
+    if (a.many > MOST_SPLITS || 2 * a.many * CTR_STRIDE > sc.ncounters || 2 * (uint64_t)a.many * a.cols * (kv.d + 2) > sc.partial_floats || !kv_launch_fits(grid, 64 * split_waves((int)kv.d / 32))) return hipErrorInvalidValue;
     // Where a sequence's entries make one tile (all sequences' on average), a block is read once; a second tile finds it in the L2. 64 sequences of
     // 8 heads to a key head, 8192 tokens at most: 74.5 us through the L2, 69.1 past it; 16 sequences of 8 rows of 4: 36.5 and 42.7.
     const bool once = b.row_start ? (uint64_t)b.rows * a.g <= (uint64_t)b.n_seqs * 16 : a.g <= 16;

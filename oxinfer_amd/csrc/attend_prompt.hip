@@ -362,7 +362,7 @@ template <int KD, int WAVES, bool F32, bool RULES>
 static hipError_t launch_waves(const AttendArgs& a, hipStream_t s) {
     constexpr int PLACES = (F32 && KD > 4) || KD > 5 ? 1 : 2;  // waves on a SIMD: two where half of its registers do
     const uint64_t grid = kv_places((uint64_t)a.b.rows * a.g, a.b.n_seqs, 32 * WAVES, 1) * a.kv.n_kv;
-    if (grid > 0x7FFFFFFFu) return hipErrorInvalidValue;
+    if (!kv_launch_fits(grid, 64 * WAVES)) return hipErrorInvalidValue;
     attend_prompt_kernel<KD, WAVES, (WAVES == 8 ? 2 : PLACES), F32, RULES><<<(unsigned)grid, 64 * WAVES, 0, s>>>(a);
     return hipGetLastError();
 }

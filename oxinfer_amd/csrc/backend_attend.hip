@@ -78,6 +78,9 @@ int oxhip_dev_kv_append(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_b
             return refuse(who, "a table of angles at a multiple of 8 bytes, an even number of rotated channels, at most d");
         r = RopeView{rope->table, (uint32_t)rope->n_pos, (uint32_t)(rope->n_rot / 2), rope->interleaved ? 1u : 0u};
     }
+    const size_t heads = 2 * kv->n_kv + n_q;
+    if (!kv_launch_fits(kv_append_workgroups(b->row_start, b->rows, b->n_seqs, heads), 256, b->row_start ? heads : 1))
+        return refuse(who, "more rows, sequences or heads than one launch takes (2^24 workgroups; with row_start 65535 heads)");
     if (!c) return refuse(who, "null context");
     if (!b->rows) return 1;
     OnDevice on(c->device);
@@ -97,7 +100,7 @@ int oxhip_dev_kv_read(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_bat
     if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "values are f32 or bf16");
     const size_t size = dtype == OXHIP_BF16 ? 2 : 4;
     if (!aligned(k_out, size) || !aligned(v_out, size)) return refuse(who, "values begin at multiples of their size");
-    if (count > 0x7FFFFFC0u || (count / KV_BLOCK + 2) * b->n_seqs > 0x7FFFFFFFu) return refuse(who, "too many tokens for one call");
+    if (count > 0x7FFFFFC0u || !kv_launch_fits(kv_read_blocks(count) * b->n_seqs, 256)) return refuse(who, "more tokens than one launch takes (2^24 blocks)");
     if (!c) return refuse(who, "null context");
     if (!count) return 1;
     OnDevice on(c->device);
@@ -120,6 +123,10 @@ int oxhip_dev_attend(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batc
     if (!aligned(q, size) || !aligned(out, size)) return refuse(who, "rows begin at multiples of their values' size");
     if ((q_stride && q_stride < width) || (out_stride && out_stride < width)) return refuse(who, "rows lie at least a row apart");
     if (q == out) return refuse(who, "out lies apart from q");
+    const size_t g = n_q / kv->n_kv;
+    if (b->row_start && b->n_seqs == 1 ? !kv_launch_fits(kv_places(b->rows * g, 1, 128, 1) * kv->n_kv, 256)
+                                       : !kv_launch_fits(kv_units(b->row_start, b->rows, b->n_seqs, g, kv->n_kv), 512))
+        return refuse(who, "more rows, sequences or heads than one launch takes");
     AttendCall call{};
     if (rules) {
         if (!(rules->cap == 0.0f || (rules->cap >= 0x1p-60f && rules->cap <= 0x1p60f))) return refuse(who, "a cap lies within 2^-60 and 2^60, or is 0 for none");
@@ -195,6 +202,7 @@ int oxhip_dev_logits(oxhip_ctx* c, const void* logits, size_t stride, void* out,
         a.n_allowed = (uint32_t)r.n_allowed;
         a.allowed_row = r.allowed_row;
     }
+    if (!kv_launch_fits(rows * logit_slices(vocab), LOGIT_THREADS)) return refuse(who, "more logits than one launch takes (2^23 slices of 4096)");
     const char* too_many = "with next, 16384 rows at most, and 2^21 slices of 4096 logits in all of them";
     if (next && (rows > LOGIT_NEXT_ROWS || rows * logit_slices(vocab) > LOGIT_NEXT_SLICES)) return refuse(who, too_many);
     if (!c) return refuse(who, "null context");

@@ -445,14 +445,12 @@ hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeVi
     a.vec = (vec(k, k_stride) ? 1u : 0u) | (vec(v, v_stride) ? 2u : 0u) | (vec(q, q_stride) ? 4u : 0u) | (vec(q_out, q_out_stride) ? 8u : 0u);
     a.even = rope.half % 8 == 0;
     if (!b.row_start) {
-        const uint64_t tasks = (uint64_t)b.n_seqs * a.tasks;
-        if (tasks > 0x7FFFFFFFu) return hipErrorInvalidValue;
-        const unsigned grid = (unsigned)((tasks + 3) / 4);
+        const unsigned grid = (unsigned)kv_append_workgroups(false, b.rows, b.n_seqs, a.tasks);
         if (bf16) kv_append_step_kernel<true><<<grid, 256, 0, s>>>(a);
         else kv_append_step_kernel<false><<<grid, 256, 0, s>>>(a);
         return hipGetLastError();
     }
-    const dim3 grid((unsigned)kv_places(b.rows, b.n_seqs, KV_BLOCK, 2), a.tasks);
+    const dim3 grid((unsigned)kv_append_workgroups(true, b.rows, b.n_seqs, a.tasks), a.tasks);
     auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
     if (kv.d <= 64) bf16 ? go(kv_append_kernel<true, 1>) : go(kv_append_kernel<false, 1>);
     else if (kv.d <= 128) bf16 ? go(kv_append_kernel<true, 2>) : go(kv_append_kernel<false, 2>);
@@ -461,7 +459,7 @@ hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeVi
 }
 
 hipError_t launch_kv_read(const KvView& kv, const KvBatchView& b, size_t count, void* k_out, void* v_out, bool bf16, hipStream_t s) {
-    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)((count + 2 * KV_BLOCK - 2) / KV_BLOCK), (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0};
+    const ReadArgs a{kv, b, k_out, v_out, (int32_t)count, (uint32_t)kv_read_blocks(count), (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0};
     const dim3 grid(a.blocks * b.n_seqs, 2 * kv.n_kv);
     if (bf16) kv_read_kernel<true><<<grid, 256, 0, s>>>(a);
     else kv_read_kernel<false><<<grid, 256, 0, s>>>(a);

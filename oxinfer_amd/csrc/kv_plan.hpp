@@ -36,6 +36,19 @@ constexpr float KV_SCALE_MIN = 0x1p-60f, KV_SCALE_MAX = 0x1p60f;
 OXHIP_HD uint64_t kv_first_place(uint64_t start, uint64_t s, uint32_t unit, uint32_t more) { return start / unit + more * s; }
 inline uint64_t kv_places(uint64_t entries, uint64_t n_seqs, uint32_t unit, uint32_t more) { return entries / unit + more * n_seqs; }
 
+// A launch has fewer than 2^32 threads, and 65535 workgroups at most in its second direction.
+inline bool kv_launch_fits(uint64_t workgroups, uint32_t threads, uint64_t second = 1) { return workgroups <= 0xFFFFFFFFu / threads && second <= 65535; }
+// The workgroups along an append's launch: the blocks that its rows touch (and heads in the second direction), or, of single tokens, four heads each.
+inline uint64_t kv_append_workgroups(bool ragged, uint64_t rows, uint64_t n_seqs, uint64_t heads) {
+    return ragged ? kv_places(rows, n_seqs, KV_BLOCK, 2) : (n_seqs * heads + 3) / 4;
+}
+// The blocks that `count` consecutive tokens touch, wherever they begin.
+inline uint64_t kv_read_blocks(uint64_t count) { return (count + 2 * KV_BLOCK - 2) / KV_BLOCK; }
+// Tiles of 16 entries x key heads that the attention for few rows may have.
+inline uint64_t kv_units(bool ragged, uint64_t rows, uint64_t n_seqs, uint64_t g, uint64_t n_kv) {
+    return (ragged ? kv_places(rows * g, n_seqs, 16, 1) : n_seqs * ((g + 15) / 16)) * n_kv;
+}
+
 // A sequence's part of a batch, as far as it is sound: rows of the batch, tokens that a table of max_pages pages can hold.
 struct KvSeq {
     int32_t s, row0, n, len;

@@ -261,7 +261,6 @@ hipError_t launch_logits(const LogitArgs& args, bool bf16, hipStream_t s) {
     auto vec = [&](const void* p, size_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; };
     a.vec = (vec(a.x, a.x_stride) ? 1u : 0u) | (vec(a.out, a.out_stride) ? 2u : 0u);
     a.slices = (uint32_t)logit_slices(a.vocab);
-    if ((uint64_t)a.slices * a.rows > 0x7FFFFFFFu) return hipErrorInvalidValue;
     const unsigned grid = a.slices * a.rows;
     if (bf16) logits_kernel<true><<<grid, LOGIT_THREADS, 0, s>>>(a);
     else logits_kernel<false><<<grid, LOGIT_THREADS, 0, s>>>(a);

@@ -258,3 +258,30 @@ def test_how_many_rows_have_a_best_token(lib):
     for rows, vocab in ((16385, 1), (16384, 524289), (8193, 2**20), (5, 2**31 - 4096)):
         assert "16384 rows" in logits(rows, vocab) and "2^21 slices" in logits(rows, vocab), (rows, vocab)
     assert "2^31 - 4096" in logits(1, 2**31 - 4095) and "null context" in logits(16385, 5, next=None)
+
+
+def test_calls_of_more_than_one_launch_takes(lib):
+    """A launch has fewer than 2^32 threads, and 65535 workgroups at most in its second direction: the calls on either side of that."""
+    from oxinfer_amd import hip
+
+    def batch(n_seqs, rows=None, ragged=False, **kv):
+        return structs(hip, kv, dict(n_seqs=n_seqs, rows=n_seqs if rows is None else rows, row_start=P if ragged else None))
+
+    def append(s, n_q=4):
+        return said(lib, lib.oxhip_dev_kv_append(None, C.byref(s[0]), C.byref(s[1]), P, 0, P, 0, P, 0, P, 0, n_q, 0, None, None))
+
+    def read(s, count):
+        return said(lib, lib.oxhip_dev_kv_read(None, C.byref(s[0]), C.byref(s[1]), count, P, P, 0, None))
+
+    def attend(s, n_q=4):
+        return said(lib, lib.oxhip_dev_attend(None, C.byref(s[0]), C.byref(s[1]), P, 0, n_q, 0, 1.0, None, 2 * P, 0, None))
+
+    def logits(rows, vocab):
+        return said(lib, lib.oxhip_dev_logits(None, P, 0, P, 0, rows, vocab, 0, None, None, None))
+
+    m = 2**20
+    wide = dict(n_kv=16384, n_pages=9)
+    for good, bad in ((append(batch(8 * m - 1)), append(batch(8 * m))), (append(batch(8 * m - 1, 5, True)), append(batch(8 * m, 5, True))), (append(batch(1, 9, True, **wide), 32766), append(batch(1, 9, True, **wide), 32768)),
+                      (read(batch(8 * m - 1), 33), read(batch(8 * m - 1), 65)), (attend(batch(4 * m - 1)), attend(batch(4 * m))), (attend(batch(m, 2 * m, True), 2 * 16), attend(batch(m, 4 * m, True), 2 * 16)),
+                      (attend(batch(1, 2**28, True), 2 * 3), attend(batch(1, 2**28, True), 2 * 4)), (logits(8 * m - 1, 4096), logits(8 * m, 4096)), (logits(4 * m - 1, 4097), logits(4 * m, 4097))):
+        assert "null context" in good and "one launch" in bad, (good, bad)

@@ -367,7 +367,8 @@ typedef struct {
  * tokens come in one call. Tokens that come later and do not fit double it until they do, and the codes that are there are rounded to the new scale:
  * none is further than a scale from its value, however many calls fill a block (half a scale where it did not grow). Scales stay within 2^-60 and
  * 2^61, larger values are cut to 127 * 2^60; NaN is stored as 0. A row whose position the table does not hold: q NaN, the key's rotated
- * channels 0. A page number outside the cache: that token is not stored. A page that a call appends to stands once in one sequence's table;
+ * channels 0. Rows before a sequence's first token (more rows than kv_len says tokens) are left out: nothing of them is stored, and q_out keeps what it
+ * has there. A page number outside the cache: that token is not stored. A page that a call appends to stands once in one sequence's table;
  * pages that are only read may be shared. */
 int oxhip_dev_kv_append(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* k, size_t k_stride, const void* v, size_t v_stride,
                         const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream);

@@ -652,7 +652,8 @@ class HipBackend:
 
     def kv_append(self, cache, batch, k, v, q=None, rope=None, q_out=None):
         """The rows' keys and values [rows, n_kv * d] (f32 or bf16; any row stride) into the cache; the keys, and the queries [rows, n_q * d],
-        rotated by `rope`. Returns the rotated queries (`q_out`, which may be q) or None."""
+        rotated by `rope`. Returns the rotated queries (`q_out`, which may be q) or None. Rows behind the last sequence, and rows before a
+        sequence's first token, are left as `q_out` has them: in a new one they may hold anything."""
         self._held(cache, batch)
         dev, rows, width = self.device, batch.rows, cache.n_kv * cache.d
         kp, ks, kd = _rows("k", k, width, rows, dev)
@@ -694,7 +695,8 @@ class HipBackend:
 
     def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
         """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of
-        `oxhip_attend_rules`. Returns out, of q's shape and type."""
+        `oxhip_attend_rules`. Returns out, of q's shape and type; rows behind the last sequence are left as `out` has them: in a new one they
+        may hold anything."""
         self._held(cache, batch)
         dev, width = self.device, math.prod(q.shape[1:])
         n_q = width // cache.d

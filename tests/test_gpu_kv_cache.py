@@ -223,3 +223,18 @@ def test_the_bindings_refusals(be):
         be.kv_read(cache, batch, 4, dtype=torch.float16)
     new = be.kv_cache(3, 2, 64, page_tokens=128)
     assert new.k.shape == (3, 2, 4, 2048) and be.kv_read(new, hip.KvBatch(batch.kv_len, torch.zeros((2, 1), dtype=torch.int32, device="cuda")), 9)[0].abs().max() == 0
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("n,lens", [([1, 1, 1], [0, 5, 0]), ([7, 2, 40], [3, 0, 40])])
+def test_queries_before_the_first_token_are_left_as_they_are(be, n, lens, inplace):
+    from oxinfer_amd import hip
+    w = kv_ref.World(lens, 2, 64, seed=1, n=n)
+    cache, batch = w.tensors(hip)
+    k = torch.randn(w.rows, 128, device="cuda")
+    q = torch.randn(w.rows, 256, device="cuda")
+    out = q if inplace else torch.full_like(q, 9.0)
+    was = out.clone()
+    be.kv_append(cache, batch, k, k, q=q, q_out=out, rope=hip.Rope(torch.from_numpy(angles(50, 64)).cuda()))
+    pos = np.concatenate([w.lens[s] - w.n[s] + np.arange(w.n[s]) for s in range(3)])
+    assert torch.equal(out[torch.from_numpy(pos < 0).cuda()], was[torch.from_numpy(pos < 0).cuda()]) and not (out == was)[torch.from_numpy(pos > 0).cuda()].all()

@@ -386,8 +386,9 @@ typedef struct {
     const int32_t* first;  /* [rows]: the first key of the row's document */
 } oxhip_attend_rules;
 /* out [rows, n_q, d] = softmax(scale * q K^T, as the rules have it) V over the cache, query head h reading key head h * n_kv / n_q (n_q a
- * multiple of n_kv); q and out (apart from each other) of `dtype`, rows *_stride values apart (0 = dense); |scale| <= 2^120. Scores, weights' sums and results are formed in
- * f32; f32 rows enter as two f16 values each (22 bits), bf16 rows as one. A row that sees no key gives zeros; one that would see a token of a page
+ * multiple of n_kv); q and out (apart from each other) of `dtype`, rows *_stride values apart (0 = dense); |scale| <= 2^120. Scores (below 2^125 in
+ * magnitude), weights' sums and results are formed in f32. f32 rows, and their weights in the product with the values, enter as two f16 values each (22 bits),
+ * bf16 rows and theirs as one (11 bits; the sum takes weights unrounded). A row that sees no key gives zeros; one that would see a token of a page
  * outside the cache NaN. The stream's scratch (as oxhip_dev_decode_batch's) is made with the first call on it. */
 int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* q, size_t q_stride, size_t n_q, int dtype, float scale,
                      const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
@@ -402,7 +403,7 @@ int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_ba
  *            number of n_allowed or more allows nothing. */
 typedef struct {
     const int32_t* history;     /* [rows, history_stride] */
-    size_t history_stride;
+    size_t history_stride;      /* 1 at least, with a history */
     const int32_t* history_len; /* [rows] */
     const int32_t* prompt_len;  /* [rows]; NULL: no prompt */
     const float *repetition, *presence, *frequency; /* [rows] each, not zero the first */

@@ -518,8 +518,9 @@ hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCal
     // Sequences of many query entries go to the kernel that is bound by the matrix cores, those of few to this file's; which of them a batch
     // has is known on the device alone, but where all rows together are few, or all one sequence's.
     // It has tiles of 128 entries and takes a tile's keys one after the other, so it pays where its tiles fill the chip: 1024 rows alone or behind 8192
-    // tokens (32 heads of 128 over 8, bf16: 256 tiles) 33 and 238 us, here 45 and 306; 512 rows 21 and 208, here 22 and 155; of heads of 64 channels
-    // (8 over 4) 4096 rows 76 and 226, here 62 and 222.
+    // tokens (32 heads of 128 over 8, bf16: 256 tiles) 36 and 216 us, here 43 and 291; 512 rows 22 and 198, here 21 and 153; of heads of 64 channels
+    // (8 over 4) 4096 rows 82 and 232, here 58 and 205. The same 1024 rows in f32: 50 and 309, here 48 and 368; capped bf16: 80 and 624, here 50 and 362
+    // (2048 rows: 128 and 590, here 131 and 733): for capped scores the border lies too low.
     const uint64_t all = (uint64_t)b.rows * a.g, fill = all * kv.n_kv / 128;
     const bool prompts = b.row_start && all >= PROMPT_ENTRIES && fill >= 256 && fill * kv.d >= 256 * 128;
     a.prompt = !prompts ? 0xFFFFFFFFu : b.n_seqs > 1 ? PROMPT_ENTRIES : 1;

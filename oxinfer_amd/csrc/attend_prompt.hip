@@ -367,7 +367,7 @@ static hipError_t launch_waves(const AttendArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 // Eight waves turn the codes into operands half as often as four, where their tiles still fill the chip and are filled themselves: prompts of 2048
-// and 4096 rows (32 heads over 8, bf16) 64 and 177 us with four, 73 and 157 with eight; 4096 rows behind 8192 tokens 725 and 683.
+// and 4096 rows (32 heads over 8, bf16) 68 and 187 us with four, 76 and 173 with eight; 4096 rows behind 8192 tokens 741 and 683.
 template <int KD, bool F32, bool RULES>
 static hipError_t launch_prompt(const AttendArgs& a, hipStream_t s) {
     const uint64_t entries = (uint64_t)a.b.rows * a.g;

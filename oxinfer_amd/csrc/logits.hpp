@@ -25,7 +25,7 @@ struct LogitArgs {
 };
 
 // Logits of a row that a workgroup takes, and its threads. (Slices of 2048 by 256 threads, 4096 by 256, 4096 by 512 and 8192 by 1024: 64 rows of 151936 bf16
-// with 2000 tokens of history 26.4, 27.4, 28.2 and 39 us a call, nine rows of 32003 with 9000 tokens 19.0, 20.6, 15.1 and 15.2, one of 128256 12.6 each.)
+// with 2000 tokens of history 26.4, 28.0, 25.8 and 27.3 us a call, nine rows of 32003 with 9000 tokens 19.9, 21.4, 15.3 and 15.3, one of 128256 13.2 each.)
 constexpr uint32_t LOGIT_SLICE = 4096, LOGIT_THREADS = 512;
 // What a stream's scratch holds of rows and of their slices' best.
 constexpr size_t LOGIT_NEXT_ROWS = 16384, LOGIT_NEXT_SLICES = (size_t)1 << 21;

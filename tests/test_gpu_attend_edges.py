@@ -155,3 +155,48 @@ def test_steep_slopes(be, n, n_kv, d, g, slope, dtype):
     """A row's own key is what is left."""
     w = kv_ref.World([90, 301] if d == 64 else [400, 64], n_kv, d, page=32, seed=5, n=n)
     one_key(be, w, g, dtype, d**-0.5, slopes=np.full(n_kv * g, slope), heads=None if d == 64 else [0, 60, 127])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [2.0**22, 2.0**39, -(2.0**60)])
+def test_scores_far_from_zero_in_parts_that_meet(be, scale, dtype):
+    """Sequences whose blocks several workgroups share."""
+    one_key(be, kv_ref.World([9000, 4500], 2, 64, page=64, seed=5), 3, dtype, scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("slope", [1e7, 1e30])
+def test_steep_slopes_in_parts_that_meet(be, slope, dtype):
+    w = kv_ref.World([9000, 4500], 2, 64, page=64, seed=5)
+    one_key(be, w, 3, dtype, 0.125, slopes=np.full(6, slope))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scales_of_zero_in_parts_that_meet(be, dtype):
+    """Most blocks of one sequence, and all of the other, hold zeros."""
+    w = kv_ref.World([9000, 4500], 2, 64, page=64, seed=5)
+    at = np.concatenate([w.table[0, 3:140], w.table[1, : -(-4500 // 64)]])
+    w.vs[at] = 0.0
+    w.ks[at[::2]] = 0.0
+    check(be, w, 3, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,n_kv", [([5, 3], 2), ([300, 5], 16)], ids=["few", "prompt"])
+@pytest.mark.parametrize("factor", [2.0**20, 2.0**40, 2.0**-40, 0.0])
+def test_a_rows_bits_beside_rows_of_another_size(be, n, n_kv, factor, dtype):
+    """Rows whose scores are far from zero, or all alike, leave the rows of their tile as they are; blocks without values among them."""
+    from oxinfer_amd import hip
+    w = kv_ref.World([900, 64], n_kv, 128, page=32, seed=3, n=n)
+    w.vs[w.table[0, 7]] = 0.0
+    cache, batch = w.tensors(hip)
+    q = torch.randn(w.rows, n_kv * 8 * 128, device="cuda").to(dtype)
+    for rules in (dict(), dict(cap=1e12)):
+        want = be.attend(cache, batch, q, **rules)
+        for part in (slice(0, None, 3), slice(1, None, 2)):
+            other = q.clone()
+            other[part] *= factor
+            kept = torch.ones(w.rows, dtype=torch.bool)
+            kept[part] = False
+            got = be.attend(cache, batch, other, **rules)
+            assert torch.equal(got[kept], want[kept]) and got.isfinite().all() and not torch.equal(got, want)

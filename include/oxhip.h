@@ -393,6 +393,47 @@ typedef struct {
 int oxhip_dev_attend(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* q, size_t q_stride, size_t n_q, int dtype, float scale,
                      const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
 
+/* A batch whose sequences begin with the same tokens, group by group: those of group i are group_start[i] .. group_start[i + 1] - 1 and share their first common[i]
+ * tokens. Both arrays are on the device, group_start ascends; sequences outside of all groups share nothing. */
+typedef struct {
+    const int32_t* group_start; /* [n_groups + 1] */
+    const int32_t* common;      /* [n_groups] */
+    size_t n_groups;
+} oxhip_kv_shared;
+/* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence:
+ * token j < common of a sequence lies in the page that the table of its group's FIRST sequence names, any other in its own table's. (Tables that all name
+ * the shared pages, as appending sequences' do, fit both calls.) Everything else is oxhip_dev_attend's: rules, types, rows that see nothing, pages outside the cache;
+ * rows that are no sequence's (also of row numbers that do not ascend) are left as they are. For batches of few rows a sequence: a prompt's are
+ * oxhip_dev_attend's. */
+int oxhip_dev_attend_shared(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_shared* shared, const void* q, size_t q_stride, size_t n_q,
+                            int dtype, float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
+
+/* Attention over the parts of a long cache that matter to a row: mean keys of its spans, a choice among them by a cheap score, the attention over the choice.
+ * A span is `span` tokens (a power of two, 32 at least and a page at most); a summary holds, for every span of the cache and key head, the mean m of
+ * its keys as bytes c with a scale s = max |m| / 127, c = rint(m / s), both on the device; `code` begins at a multiple of 16 bytes. */
+typedef struct {
+    int8_t* code; /* [n_pages, n_kv, page_tokens / span, d] */
+    float* scale; /* [n_pages, n_kv, page_tokens / span] */
+    size_t span;
+} oxhip_kv_summary;
+/* The spans that the batch's rows touch (after their append), over the tokens that the cache then holds of them. Keys whose scale is under 2^-60 count as 0. A
+ * span of a page outside the cache is left out. A page that a call appended to stands once in one table, as for the append. */
+int oxhip_dev_kv_summarize(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, void* stream);
+/* The mean keys that the last `count` spans of every sequence stand for, out [n_seqs, count, n_kv, d] f32 at a multiple of 16 bytes; places before a sequence's
+ * first span are zeros, spans of a page outside the cache NaN. */
+int oxhip_dev_kv_summary_read(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, size_t count, float* out, void* stream);
+/* `count` spans for every row and key head, chosen [rows, n_kv, count]: of the spans 0 .. p / span (p the row's position) the first `first`, the last `last`, and of
+ * the others those of the highest score, of equal ones the lower; ascending, -1 behind the last (all spans, where there are no more than count). The score of
+ * a span is max over the key head's query heads of (sum of products of bytes) * its scale * the query's, the query being made bytes as a mean
+ * key is (its scale max |q| times the f32 nearest to 1 / 127; NaN as 0, infinity as the largest value); the sum is exact and the products are formed in f64. A span of a page outside the cache has the lowest score.
+ * q [rows, n_q, d] as oxhip_dev_attend's. A sequence's table has room for 16384 spans at most (max_pages * page_tokens / span). */
+int oxhip_dev_kv_select(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, const void* q, size_t q_stride, size_t n_q, int dtype,
+                        size_t count, size_t first, size_t last, int32_t* chosen, void* stream);
+/* oxhip_dev_attend over the spans alone that `chosen` [rows, n_kv, count] names for a row and key head (of those keys, what the rules let the row see). Numbers that are
+ * negative, past the row's own span, or not above the one before them name nothing. */
+int oxhip_dev_attend_selected(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const int32_t* chosen, size_t count, size_t span, const void* q, size_t q_stride,
+                              size_t n_q, int dtype, float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
+
 /* ---- the logits' rules (behind the head's linear) ------------------------------------------------------------------
  * In this order, for every row; a NULL array sets no such rule. All arrays are on the device.
  *   history: ids of the row's tokens so far, the first prompt_len[row] of them its prompt. An id that occurs: l > 0 ? l / repetition[row] : l *
@@ -421,6 +462,25 @@ typedef struct {
  * oxhip_dev_attend's. */
 int oxhip_dev_logits(oxhip_ctx* ctx, const void* logits, size_t stride, void* out, size_t out_stride, size_t rows, size_t vocab, int dtype,
                      const oxhip_logit_rules* rules, int32_t* next, void* stream);
+
+/* The draw of the rows' next tokens, behind the rules above. All arrays are on the device, one value for each row; a NULL array sets no such limit.
+ * A token's weight is w = exp((l - max l) / temperature) (no array: 1; 0, a negative one or NaN: the best token is taken, of equal ones the lowest); NaN and
+ * -infinity weigh nothing; where the largest logit is infinite, those alone weigh. In the order of their logits, of equal ones the lower id first, there remain
+ *   top_k: the first top_k tokens (0 or less: all); then
+ *   top_p: the fewest first tokens that weigh top_p and more of what remains, at least one (1 and above, or NaN: all); then
+ *   min_p: tokens with w >= min_p (above 1: as 1; 0 and below, or NaN: all).
+ * next: the first id up to which what remains, in the order of the ids, weighs more than u times all of it, u in [0, 1) being the row's random number (what is
+ * below 0 or NaN is 0, 1 and above gives the last one); -1 where nothing weighs. logp (or NULL): the logarithm of the token's share of what remains (-infinity for -1).
+ * Weights are held as whole numbers of 2^-(62 - ceil(log2 vocab)) of the largest: their sums are exact, the same numbers draw the same token. */
+typedef struct {
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+} oxhip_sample_rules;
+/* logits [rows, vocab] of `dtype`, rows `stride` values apart (0 = dense); a vocabulary has 2^31 - 4096 ids at most. */
+int oxhip_dev_sample(oxhip_ctx* ctx, const void* logits, size_t stride, size_t rows, size_t vocab, int dtype, const oxhip_sample_rules* rules, const float* u, int32_t* next,
+                     float* logp, void* stream);
 
 /* ---- a recorded chain of device-pointer ops, replayed with one call ---------------------------------------------
  * The matmul side of DecodePlan::step (src/gpu_decode.rs:572-587; CUDA's per-graph launch list, src/cuda_decode.rs:1044-1049):

@@ -21,6 +21,12 @@ struct AttendArgs {
     float scale, cap;  // scale: the mantissa of the call's, times log2 e
     int32_t power;     // the call's scale's
     uint32_t g, window, cols, vec, quantum, many, least, prompt;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
+    // of a shared prefix, and of chosen spans (attend_lists.hip): tiles x key heads, parts of one at most
+    uint32_t units, parts;
+    const int32_t *group_start, *common;
+    uint32_t n_groups;
+    const int32_t* chosen;
+    uint32_t count, span_shift;  // spans of a row and key head; blocks of a span: 1 << span_shift
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -41,6 +47,12 @@ __device__ __forceinline__ float key_scale(float held) { return held < KV_SCALE_
 constexpr float NO_VALUES = -61.0f;
 __device__ __forceinline__ float value_log(float held) { return held < KV_SCALE_MIN ? NO_VALUES : __builtin_amdgcn_logf(held); }
 __device__ __forceinline__ bool no_values(float log) { return __float_as_uint(log) == __builtin_bit_cast(uint32_t, NO_VALUES); }
+
+// A sum of weights (in units of which the values' scale is no part) under another maximum, 2^apart of it. Between maxima of blocks whose value scales lie as far
+// apart as scales may, 2^apart alone would be below what f32 holds, where the sum, 2^61 and more, is not.
+__device__ __forceinline__ float lowered(float sum, float apart) {
+    return apart < -100.0f ? sum * 0x1p-100f * __builtin_amdgcn_exp2f(apart + 100.0f) : sum * __builtin_amdgcn_exp2f(apart);
+}
 
 // What makes a score, times log2 e, of the product of a row's operands and a block's codes: the call's scale (its mantissa times log2 e, which the key scales
 // are multiplied with) and two powers of two, the call's and the one that the row's operands were divided by. Either may lie outside f32, so they are added first. A masked
@@ -147,6 +159,8 @@ __device__ __forceinline__ void load_query(const void* q, size_t at, bool vec, f
 
 // Entries (rows x heads of a group) of a sequence from which on attend_prompt_kernel takes it.
 constexpr uint32_t PROMPT_ENTRIES = 128;
+// What the launches of one call have alike; whether the kernels with rules are to run.
+AttendArgs attend_args(const KvView& kv, const KvBatchView& b, const AttendCall& call, const DecodeScratch& sc, bool* rules);
 hipError_t launch_attend_prompt(const AttendArgs& a, bool bf16, bool rules, hipStream_t s);
 
 }  // namespace oxhip

@@ -1,0 +1,55 @@
+// Attention over a prefix that a batch's sequences share, and over chosen spans of a cache: what attend.hip computes, over other lists of blocks.
+//
+// A tile is 16 query entries of one key head. Of a shared prefix they may come from several sequences, so that a shared block is read, and its codes are made
+// f16 values, once for 16 entries; behind the shared tokens a tile's list names each sequence's own blocks, whose keys the other sequences' entries do not see.
+// Of chosen spans a tile is one row's group of heads, for which the spans were chosen together.
+#include <cmath>
+
+#include "attend_split.hpp"
+
+namespace oxhip {
+
+// How many tiles a batch has, and parts of each: `target` workgroups in all, where lists of `blocks` blocks at most have parts of a.least blocks for them.
+static hipError_t spread(AttendArgs& a, const DecodeScratch& sc, bool several, uint64_t blocks, uint32_t target, unsigned* grid) {
+    const uint64_t units = kv_row_tiles(a.b.rows, a.g, several) * a.kv.n_kv;
+    a.cols = several ? 16u : std::min(16u, a.g);
+    a.least = a.kv.d > 128 ? KV_LEAST / 2 : KV_LEAST;
+    const uint64_t room = std::min<uint64_t>(sc.partial_floats / ((uint64_t)a.cols * (a.kv.d + 2)), sc.ncounters / CTR_STRIDE);  // parts that the scratch holds
+    uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>((target + units - 1) / units, (blocks + a.least - 1) / a.least));
+    parts = std::min<uint64_t>(parts, MOST_SPLITS);
+    if (units * parts > room) parts = std::max<uint64_t>(1, room / units);
+    if (!kv_launch_fits(units * parts, 64 * split_waves((int)a.kv.d / 32))) return hipErrorInvalidValue;
+    a.units = (uint32_t)units;
+    a.parts = (uint32_t)parts;
+    *grid = (unsigned)(units * parts);
+    return hipSuccess;
+}
+template <int KIND>
+static hipError_t go(const AttendArgs& a, bool bf16, bool rules, unsigned grid, hipStream_t s) {
+    if (bf16) return rules ? launch_split<false, true, false, KIND>(a, grid, s) : launch_split<false, false, false, KIND>(a, grid, s);
+    return rules ? launch_split<true, true, false, KIND>(a, grid, s) : launch_split<true, false, false, KIND>(a, grid, s);
+}
+
+hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const SharedView& shared, const AttendCall& call, const DecodeScratch& sc, hipStream_t s) {
+    bool rules;
+    AttendArgs a = attend_args(kv, b, call, sc, &rules);
+    a.group_start = shared.group_start;
+    a.common = shared.common;
+    a.n_groups = shared.n_groups;
+    unsigned grid;
+    const hipError_t e = spread(a, sc, true, (uint64_t)b.max_pages << kv.shift, 256 * split_places((int)kv.d / 32), &grid);
+    return e != hipSuccess ? e : go<SHARED>(a, call.bf16, rules, grid, s);
+}
+
+hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const ChosenView& chosen, const AttendCall& call, const DecodeScratch& sc, hipStream_t s) {
+    bool rules;
+    AttendArgs a = attend_args(kv, b, call, sc, &rules);
+    a.chosen = chosen.chosen;
+    a.count = chosen.count;
+    while ((1u << a.span_shift) < chosen.span_blocks) a.span_shift++;
+    unsigned grid;
+    const hipError_t e = spread(a, sc, false, std::min<uint64_t>((uint64_t)chosen.count << a.span_shift, (uint64_t)b.max_pages << kv.shift), 256 * split_places((int)kv.d / 32), &grid);
+    return e != hipSuccess ? e : go<CHOSEN>(a, call.bf16, rules, grid, s);
+}
+
+}  // namespace oxhip

@@ -271,9 +271,9 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
             float shift = lv + HEAD_ROOM - m;
             if (__builtin_amdgcn_ballot_w64(top + lv > bar)) {
                 // (an entry whose own scores need it: another row's do not change a row's bits)
-                const float own = half_max(top) + lv, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
+                const float own = half_max(top) + lv, before = m, to = own > m + (MOST_ROOM - HEAD_ROOM) ? own : m, down = __builtin_amdgcn_exp2f(m - to);
                 m = to;
-                l *= down;
+                l = lowered(l, before - to);
 #pragma unroll
                 for (int c = 0; c < KD; c++) acc[c] *= down;
                 shift = lv + HEAD_ROOM - m;
@@ -291,10 +291,10 @@ __global__ __launch_bounds__(64 * WAVES, PLACES) void attend_prompt_kernel(Atten
                     float sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        sum += __builtin_amdgcn_exp2f(RULES ? sc[r] + shift : fmaf(sc[r], f, shift));
+                        sum += __builtin_amdgcn_exp2f((RULES ? sc[r] + shift : fmaf(sc[r], f, shift)) - lv);
                         sc[r] = -__builtin_inff();
                     }
-                    l += sum * __builtin_amdgcn_exp2f(-lv);
+                    l += sum;
                 }
             }
             // keys of block i + 1; the weights of block i

@@ -1,7 +1,8 @@
-// The C entry points of the 8-bit key / value cache, the attention over it and the logits' rules: the checks of their arguments.
+// The C entry points of the 8-bit key / value cache, the attention over it, the logits' rules and the draw: the checks of their arguments.
 #include "backend.hpp"
 #include "kv.hpp"
 #include "logits.hpp"
+#include "sample.hpp"
 
 using namespace oxhip;
 
@@ -50,6 +51,46 @@ DecodeScratch* parts(oxhip_ctx* c, hipStream_t s, const char* who) {
     StreamScratch* sc = scratch_for(c, s, true);
     if (sc) return &sc->dec;
     set_error(std::string(who) + (stream_recording(s) ? ": the stream's scratch does not exist yet and a plan records on it (run the chain once before recording)" : ": device memory short"));
+    return nullptr;
+}
+
+// What the calls of the attention have alike: the checks, and what the kernels get. nullptr, or what is wrong.
+const char* check_attend(const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* q, size_t q_stride, size_t n_q, int dtype, float scale, const oxhip_attend_rules* rules,
+                         void* out, size_t out_stride, KvView* kvv, KvBatchView* bv, AttendCall* call) {
+    if (!q || !out) return "null argument";
+    if (const char* why = check(kv, b, kvv, bv)) return why;
+    if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return "rows are f32 or bf16";
+    if (!n_q || n_q % kv->n_kv || n_q > 65536) return "the query heads are a multiple of the key heads, 65536 at most";
+    if (!(std::fabs(scale) <= 0x1p120f)) return "the scale lies within -2^120 and 2^120";
+    const size_t size = dtype == OXHIP_BF16 ? 2 : 4, width = n_q * kv->d;
+    if (!aligned(q, size) || !aligned(out, size)) return "rows begin at multiples of their values' size";
+    if ((q_stride && q_stride < width) || (out_stride && out_stride < width)) return "rows lie at least a row apart";
+    if (q == out) return "out lies apart from q";
+    if (rules) {
+        if (!(rules->cap == 0.0f || (rules->cap >= 0x1p-60f && rules->cap <= 0x1p60f))) return "a cap lies within 2^-60 and 2^60, or is 0 for none";
+        if (!aligned(rules->slopes, 4) || !aligned(rules->prefix, 4) || !aligned(rules->first, 4)) return "an array of 4-byte values at an odd address";
+        call->cap = rules->cap;
+        call->slopes = rules->slopes;
+        call->window = rules->window < 0x7FFFFFFFu ? (uint32_t)rules->window : 0;  // (no sequence is that long)
+        call->prefix = rules->prefix;
+        call->first = rules->first;
+    }
+    call->q = q;
+    call->out = out;
+    call->q_stride = q_stride ? q_stride : width;
+    call->out_stride = out_stride ? out_stride : width;
+    call->scale = scale;
+    call->n_q = (uint32_t)n_q;
+    call->bf16 = dtype == OXHIP_BF16;
+    return nullptr;
+}
+// A summary of a cache, or nullptr and what is wrong.
+const char* check_summary(const oxhip_kv_cache* kv, const oxhip_kv_summary* sum, uint32_t* span_shift) {
+    if (!sum || !sum->code || !sum->scale) return "null argument";
+    if (!aligned(sum->code, 16) || !aligned(sum->scale, 4)) return "code begins at a multiple of 16 bytes, scale of 4";
+    if (sum->span < KV_BLOCK || (sum->span & (sum->span - 1)) || sum->span > kv->page_tokens) return "a span is a power of two of tokens, 32 at least and a page at most";
+    *span_shift = 0;
+    while (((size_t)KV_BLOCK << *span_shift) < sum->span) ++*span_shift;
     return nullptr;
 }
 
@@ -114,44 +155,163 @@ int oxhip_dev_attend(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batc
     const char* who = "attend";
     KvView kvv;
     KvBatchView bv;
-    if (!q || !out) return refuse(who, "null argument");
-    if (const char* why = check(kv, b, &kvv, &bv)) return refuse(who, why);
-    if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "rows are f32 or bf16");
-    if (!n_q || n_q % kv->n_kv || n_q > 65536) return refuse(who, "the query heads are a multiple of the key heads, 65536 at most");
-    if (!(std::fabs(scale) <= 0x1p120f)) return refuse(who, "the scale lies within -2^120 and 2^120");
-    const size_t size = dtype == OXHIP_BF16 ? 2 : 4, width = n_q * kv->d;
-    if (!aligned(q, size) || !aligned(out, size)) return refuse(who, "rows begin at multiples of their values' size");
-    if ((q_stride && q_stride < width) || (out_stride && out_stride < width)) return refuse(who, "rows lie at least a row apart");
-    if (q == out) return refuse(who, "out lies apart from q");
+    AttendCall call{};
+    if (const char* why = check_attend(kv, b, q, q_stride, n_q, dtype, scale, rules, out, out_stride, &kvv, &bv, &call)) return refuse(who, why);
     const size_t g = n_q / kv->n_kv;
     if (b->row_start && b->n_seqs == 1 ? !kv_launch_fits(kv_places(b->rows * g, 1, 128, 1) * kv->n_kv, 256)
                                        : !kv_launch_fits(kv_units(b->row_start, b->rows, b->n_seqs, g, kv->n_kv), 512))
         return refuse(who, "more rows, sequences or heads than one launch takes");
-    AttendCall call{};
-    if (rules) {
-        if (!(rules->cap == 0.0f || (rules->cap >= 0x1p-60f && rules->cap <= 0x1p60f))) return refuse(who, "a cap lies within 2^-60 and 2^60, or is 0 for none");
-        if (!aligned(rules->slopes, 4) || !aligned(rules->prefix, 4) || !aligned(rules->first, 4)) return refuse(who, "an array of 4-byte values at an odd address");
-        call.cap = rules->cap;
-        call.slopes = rules->slopes;
-        call.window = rules->window < 0x7FFFFFFFu ? (uint32_t)rules->window : 0;  // (no sequence is that long)
-        call.prefix = rules->prefix;
-        call.first = rules->first;
-    }
     if (!c) return refuse(who, "null context");
     if (!b->rows) return 1;
-    call.q = q;
-    call.out = out;
-    call.q_stride = q_stride ? q_stride : width;
-    call.out_stride = out_stride ? out_stride : width;
-    call.scale = scale;
-    call.n_q = (uint32_t)n_q;
-    call.bf16 = dtype == OXHIP_BF16;
     OnDevice on(c->device);
     if (!on.ok) return refuse(who, "hipSetDevice failed");
     hipStream_t s = static_cast<hipStream_t>(stream);
     DecodeScratch* sc = parts(c, s, who);
     if (!sc) return 0;
     HIP_TRY(launch_attend(kvv, bv, call, *sc, s), "attend launch");
+    return 1;
+}
+
+int oxhip_dev_attend_shared(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_shared* shared, const void* q, size_t q_stride, size_t n_q, int dtype,
+                            float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream) {
+    const char* who = "attend_shared";
+    KvView kvv;
+    KvBatchView bv;
+    AttendCall call{};
+    if (const char* why = check_attend(kv, b, q, q_stride, n_q, dtype, scale, rules, out, out_stride, &kvv, &bv, &call)) return refuse(who, why);
+    if (!shared || !shared->group_start || !shared->common) return refuse(who, "null argument");
+    if (!aligned(shared->group_start, 4) || !aligned(shared->common, 4)) return refuse(who, "an array of 4-byte values at an odd address");
+    if (!shared->n_groups || shared->n_groups > ((size_t)1 << 24)) return refuse(who, "1 to 2^24 groups");
+    if (!kv_launch_fits(kv_row_tiles(b->rows, n_q / kv->n_kv, true) * kv->n_kv, 512)) return refuse(who, "more rows or heads than one launch takes");
+    if (!c) return refuse(who, "null context");
+    if (!b->rows) return 1;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DecodeScratch* sc = parts(c, s, who);
+    if (!sc) return 0;
+    HIP_TRY(launch_attend_shared(kvv, bv, SharedView{shared->group_start, shared->common, (uint32_t)shared->n_groups}, call, *sc, s), "attend_shared launch");
+    return 1;
+}
+
+int oxhip_dev_kv_summarize(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, void* stream) {
+    const char* who = "kv_summarize";
+    SummaryArgs a{};
+    if (const char* why = check(kv, b, &a.kv, &a.b)) return refuse(who, why);
+    if (const char* why = check_summary(kv, sum, &a.span_shift)) return refuse(who, why);
+    if (!kv_launch_fits((b->row_start ? kv_places(b->rows, b->n_seqs, (uint32_t)sum->span, 2) : b->n_seqs) * kv->n_kv, 256)) return refuse(who, "more rows, sequences or heads than one launch takes");
+    if (!c) return refuse(who, "null context");
+    if (!b->rows) return 1;
+    a.code = sum->code;
+    a.scale = sum->scale;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    HIP_TRY(launch_kv_summarize(a, static_cast<hipStream_t>(stream)), "kv_summarize launch");
+    return 1;
+}
+
+int oxhip_dev_kv_summary_read(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, size_t count, float* out, void* stream) {
+    const char* who = "kv_summary_read";
+    SummaryArgs a{};
+    if (!out) return refuse(who, "null argument");
+    if (const char* why = check(kv, b, &a.kv, &a.b)) return refuse(who, why);
+    if (const char* why = check_summary(kv, sum, &a.span_shift)) return refuse(who, why);
+    if (!aligned(out, 16)) return refuse(who, "out begins at a multiple of 16 bytes");
+    if (count > 0x7FFFFFFFu || (count && b->n_seqs * kv->n_kv > 0xFFFFFFFFu / (kv->d / 4) / count)) return refuse(who, "more spans than one launch takes");
+    if (!c) return refuse(who, "null context");
+    if (!count) return 1;
+    a.code = sum->code;
+    a.scale = sum->scale;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    HIP_TRY(launch_kv_summary_read(a, count, out, static_cast<hipStream_t>(stream)), "kv_summary_read launch");
+    return 1;
+}
+
+int oxhip_dev_kv_select(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, const void* q, size_t q_stride, size_t n_q, int dtype,
+                        size_t count, size_t first, size_t last, int32_t* chosen, void* stream) {
+    const char* who = "kv_select";
+    SelectArgs a{};
+    if (!q || !chosen) return refuse(who, "null argument");
+    if (const char* why = check(kv, b, &a.kv, &a.b)) return refuse(who, why);
+    if (const char* why = check_summary(kv, sum, &a.span_shift)) return refuse(who, why);
+    if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "rows are f32 or bf16");
+    if (!n_q || n_q % kv->n_kv || n_q > 65536) return refuse(who, "the query heads are a multiple of the key heads, 65536 at most");
+    const size_t width = n_q * kv->d;
+    if (!aligned(q, dtype == OXHIP_BF16 ? 2 : 4) || !aligned(chosen, 4)) return refuse(who, "rows begin at multiples of their values' size");
+    if (q_stride && q_stride < width) return refuse(who, "rows lie at least a row apart");
+    if (!count || count > SELECT_SPANS || first > count || last > count - first) return refuse(who, "1 to 16384 spans of a row, the first and the last ones among them");
+    if (b->max_pages > SELECT_SPANS / (kv->page_tokens / sum->span)) return refuse(who, "a sequence's table has room for 16384 spans at most");
+    if (!kv_launch_fits((uint64_t)b->rows * kv->n_kv, 512)) return refuse(who, "more rows or heads than one launch takes");
+    if (!c) return refuse(who, "null context");
+    if (!b->rows) return 1;
+    a.code = sum->code;
+    a.scale = sum->scale;
+    a.q = q;
+    a.q_stride = q_stride ? q_stride : width;
+    a.out = chosen;
+    a.g = (uint32_t)(n_q / kv->n_kv);
+    a.count = (uint32_t)count;
+    a.first = (uint32_t)first;
+    a.last = (uint32_t)last;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    HIP_TRY(launch_kv_select(a, dtype == OXHIP_BF16, static_cast<hipStream_t>(stream)), "kv_select launch");
+    return 1;
+}
+
+int oxhip_dev_attend_selected(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const int32_t* chosen, size_t count, size_t span, const void* q, size_t q_stride,
+                              size_t n_q, int dtype, float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream) {
+    const char* who = "attend_selected";
+    KvView kvv;
+    KvBatchView bv;
+    AttendCall call{};
+    if (const char* why = check_attend(kv, b, q, q_stride, n_q, dtype, scale, rules, out, out_stride, &kvv, &bv, &call)) return refuse(who, why);
+    if (!chosen) return refuse(who, "null argument");
+    if (!aligned(chosen, 4)) return refuse(who, "an array of 4-byte values at an odd address");
+    if (span < KV_BLOCK || (span & (span - 1)) || span > kv->page_tokens) return refuse(who, "a span is a power of two of tokens, 32 at least and a page at most");
+    if (!count || count > ((size_t)1 << 26) / (span / KV_BLOCK)) return refuse(who, "1 span of a row at least, 2^31 tokens of them at most");
+    if (!kv_launch_fits(kv_row_tiles(b->rows, n_q / kv->n_kv, false) * kv->n_kv, 512)) return refuse(who, "more rows or heads than one launch takes");
+    if (!c) return refuse(who, "null context");
+    if (!b->rows) return 1;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DecodeScratch* sc = parts(c, s, who);
+    if (!sc) return 0;
+    HIP_TRY(launch_attend_selected(kvv, bv, ChosenView{chosen, (uint32_t)count, (uint32_t)(span / KV_BLOCK)}, call, *sc, s), "attend_selected launch");
+    return 1;
+}
+
+int oxhip_dev_sample(oxhip_ctx* c, const void* logits, size_t stride, size_t rows, size_t vocab, int dtype, const oxhip_sample_rules* rules, const float* u, int32_t* next,
+                     float* logp, void* stream) {
+    const char* who = "sample";
+    if (!logits || !u || !next) return refuse(who, "null argument");
+    if (dtype != OXHIP_F32 && dtype != OXHIP_BF16) return refuse(who, "logits are f32 or bf16");
+    if (!vocab || vocab > 0x7FFFF000u || rows > ((size_t)1 << 22) - 1) return refuse(who, "a vocabulary of 1 to 2^31 - 4096, fewer than 2^22 rows");
+    if (!aligned(logits, dtype == OXHIP_BF16 ? 2 : 4) || !aligned(u, 4) || !aligned(next, 4) || !aligned(logp, 4)) return refuse(who, "rows begin at multiples of their values' size");
+    if (stride && stride < vocab) return refuse(who, "rows lie at least a row apart");
+    SampleArgs a{};
+    a.x = logits;
+    a.stride = stride ? stride : vocab;
+    a.rows = (uint32_t)rows;
+    a.vocab = (uint32_t)vocab;
+    a.u = u;
+    a.next = next;
+    a.logp = logp;
+    if (rules) {
+        for (const void* p : {(const void*)rules->temperature, (const void*)rules->top_k, (const void*)rules->top_p, (const void*)rules->min_p})
+            if (!aligned(p, 4)) return refuse(who, "an array of 4-byte values at an odd address");
+        a.temperature = rules->temperature;
+        a.top_k = rules->top_k;
+        a.top_p = rules->top_p;
+        a.min_p = rules->min_p;
+    }
+    if (!c) return refuse(who, "null context");
+    if (!rows) return 1;
+    OnDevice on(c->device);
+    if (!on.ok) return refuse(who, "hipSetDevice failed");
+    HIP_TRY(launch_sample(a, dtype == OXHIP_BF16, static_cast<hipStream_t>(stream)), "sample launch");
     return 1;
 }
 

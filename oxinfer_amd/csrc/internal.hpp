@@ -284,8 +284,22 @@ struct AttendCall {
     bool bf16;
 };
 hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
+// The sequences whose first tokens are the same: those of group i are group_start[i] .. group_start[i + 1] - 1, and they share common[i] tokens.
+struct SharedView {
+    const int32_t *group_start, *common;
+    uint32_t n_groups;
+};
+hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const SharedView& shared, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
+// The spans of `span_blocks` blocks that were chosen for each row and key head: [rows][n_kv][count].
+struct ChosenView {
+    const int32_t* chosen;
+    uint32_t count, span_blocks;
+};
+hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const ChosenView& chosen, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
 struct LogitArgs;
 hipError_t launch_logits(const LogitArgs& a, bool bf16, hipStream_t s);
+struct SampleArgs;
+hipError_t launch_sample(const SampleArgs& a, bool bf16, hipStream_t s);
 
 hipError_t launch_fill_zero(uint32_t* p, size_t n, hipStream_t s);  // n dwords, by a kernel on `s`
 

@@ -14,6 +14,29 @@ struct KvBatchView {
     const int32_t *row_start, *kv_len, *pages;
     uint32_t n_seqs, rows, max_pages;
 };
+// The mean keys of the cache's spans of 1 << span_shift blocks: signed bytes [page][head][span of the page][d], and a scale for each.
+struct SummaryArgs {
+    KvView kv;
+    KvBatchView b;
+    int8_t* code;
+    float* scale;
+    uint32_t span_shift;
+};
+struct SelectArgs {
+    KvView kv;
+    KvBatchView b;
+    const int8_t* code;
+    const float* scale;
+    const void* q;
+    size_t q_stride;
+    int32_t* out;  // [rows][n_kv][count]
+    uint32_t span_shift, g, count, first, last;
+};
+// The spans that a sequence's table may hold: their scores lie in LDS.
+constexpr uint32_t SELECT_SPANS = 16384;
+hipError_t launch_kv_summarize(const SummaryArgs& a, hipStream_t s);
+hipError_t launch_kv_summary_read(const SummaryArgs& a, size_t count, float* out, hipStream_t s);
+hipError_t launch_kv_select(const SelectArgs& a, bool bf16, hipStream_t s);
 struct RopeView {
     const float* table;
     uint32_t n_pos, half;  // positions, pairs per head

@@ -48,6 +48,12 @@ inline uint64_t kv_read_blocks(uint64_t count) { return (count + 2 * KV_BLOCK - 
 inline uint64_t kv_units(bool ragged, uint64_t rows, uint64_t n_seqs, uint64_t g, uint64_t n_kv) {
     return (ragged ? kv_places(rows * g, n_seqs, 16, 1) : n_seqs * ((g + 15) / 16)) * n_kv;
 }
+// Tiles of rows of a batch, whatever sequences they are of, for one key head: of 16 / g rows where several may share a tile, of one row otherwise, of 16 heads where
+// a row's group has more.
+inline uint64_t kv_row_tiles(uint64_t rows, uint64_t g, bool several) {
+    const uint64_t of = several && g < 16 ? 16 / g : 1;
+    return (rows + of - 1) / of * ((g + 15) / 16);
+}
 
 // A sequence's part of a batch, as far as it is sound: rows of the batch, tokens that a table of max_pages pages can hold.
 struct KvSeq {
@@ -76,6 +82,15 @@ OXHIP_HD KvSpan kv_span(int64_t prefix, int64_t lo, int64_t hi) {
     const uint32_t first = lo > 0 ? (uint32_t)(lo / KV_BLOCK) : 0u, end = hi > 0 ? (uint32_t)((hi + KV_BLOCK - 1) / KV_BLOCK) : 0u;
     s.lo = first > s.pre ? first : s.pre;
     s.count = s.pre + (hi > lo && end > s.lo ? end - s.lo : 0u);
+    return s;
+}
+// The same of the blocks from `base` on alone: those of the prefix from there on are the first `pre` of them.
+OXHIP_HD KvSpan kv_span_from(uint32_t base, int64_t prefix, int64_t lo, int64_t hi) {
+    KvSpan s = kv_span(prefix, lo, hi);
+    const uint32_t end = s.count > s.pre ? s.lo + (s.count - s.pre) : 0u, first = s.lo > base ? s.lo : base;
+    s.pre = s.pre > base ? s.pre - base : 0u;
+    s.lo = first;
+    s.count = s.pre + (end > first ? end - first : 0u);
     return s;
 }
 OXHIP_HD uint32_t kv_span_block(const KvSpan& s, uint32_t i) { return i < s.pre ? i : s.lo + (i - s.pre); }

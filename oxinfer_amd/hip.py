@@ -76,6 +76,18 @@ class LogitRulesC(C.Structure):
                 ("allowed_stride", C.c_size_t), ("allowed_row", C.c_void_p)]
 
 
+class KvSharedC(C.Structure):
+    _fields_ = [("group_start", C.c_void_p), ("common", C.c_void_p), ("n_groups", C.c_size_t)]
+
+
+class KvSummaryC(C.Structure):
+    _fields_ = [("code", C.c_void_p), ("scale", C.c_void_p), ("span", C.c_size_t)]
+
+
+class SampleRulesC(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+
 _lib = None
 _torch = None
 
@@ -143,6 +155,12 @@ def load_library():
         "oxhip_dev_kv_read": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), sz, vp, vp, C.c_int, vp]),
         "oxhip_dev_attend": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
         "oxhip_dev_logits": (C.c_int, [vp, vp, sz, vp, sz, sz, sz, C.c_int, C.POINTER(LogitRulesC), vp, vp]),
+        "oxhip_dev_attend_shared": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSharedC), vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
+        "oxhip_dev_kv_summarize": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSummaryC), vp]),
+        "oxhip_dev_kv_summary_read": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSummaryC), sz, vp, vp]),
+        "oxhip_dev_kv_select": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSummaryC), vp, sz, sz, C.c_int, sz, sz, sz, vp, vp]),
+        "oxhip_dev_attend_selected": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), vp, sz, sz, vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
+        "oxhip_dev_sample": (C.c_int, [vp, vp, sz, sz, sz, C.c_int, C.POINTER(SampleRulesC), vp, vp, vp, vp]),
         "oxhip_plan_begin": (vp, [vp, vp]),
         "oxhip_plan_end": (C.c_int, [vp]),
         "oxhip_plan_launches": (sz, [vp]),
@@ -335,6 +353,35 @@ class Rope:
         self.table = table
         self.c = RopeC(_array("table", table, torch.float32), table.shape[0], 2 * table.shape[1], int(interleaved))
         self.ref, self.device = C.byref(self.c), table.get_device()
+
+
+class KvShared:
+    """`oxhip_kv_shared`: group_start int32 [n_groups + 1], common int32 [n_groups]: the sequences of a batch that begin with the same tokens. Their
+    contents may change between calls."""
+
+    def __init__(self, group_start, common):
+        import torch
+        n, dev = common.numel(), common.get_device() if common.is_cuda else None
+        p = _array("group_start", group_start, torch.int32, dev, n + 1), _array("common", common, torch.int32, dev)
+        self.group_start, self.common, self.device = group_start, common, dev
+        self.c = KvSharedC(*p, n)
+        self.ref = C.byref(self.c)
+
+
+class KvSummary:
+    """`oxhip_kv_summary`: the mean keys of a cache's spans, codes int8 [n_pages, n_kv, page_tokens / span, d] and f32 scales [n_pages, n_kv, page_tokens /
+    span]. `HipBackend.kv_summary` makes a new one."""
+
+    def __init__(self, code, scale, span):
+        import torch
+        dev = code.get_device() if code.is_cuda else None
+        if code.dim() != 4:
+            raise ValueError(f"code: shape {tuple(code.shape)}, wanted [n_pages, n_kv, page_tokens / span, d]")
+        p = _array("code", code, torch.int8, dev), _array("scale", scale, torch.float32, dev, math.prod(code.shape[:3]))
+        self.code, self.scale, self.span, self.device = code, scale, span, dev
+        self.shape = tuple(code.shape)
+        self.c = KvSummaryC(*p, span)
+        self.ref = C.byref(self.c)
 
 
 class HipBackend:
@@ -693,10 +740,8 @@ class HipBackend:
             raise RuntimeError(self.last_error())
         return both.unbind(0)
 
-    def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
-        """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of
-        `oxhip_attend_rules`. Returns out, of q's shape and type; rows behind the last sequence are left as `out` has them: in a new one they
-        may hold anything."""
+    def _attend_call(self, cache, batch, q, cap, slopes, window, prefix, first, out):
+        """What the attention's calls have alike: (q's pointer and stride, n_q, type, rules, out's pointer and stride, out)."""
         self._held(cache, batch)
         dev, width = self.device, math.prod(q.shape[1:])
         n_q = width // cache.d
@@ -716,10 +761,97 @@ class HipBackend:
                 raise ValueError("first: one for each row")
             rules = C.byref(AttendRulesC(cap, _array("slopes", slopes, _torch.float32, dev, n_q), window, _array("prefix", prefix, _torch.int32, dev, batch.n_seqs),
                                          _array("first", first, _torch.int32, dev)))
+        return qp, qs, n_q, qd, rules, op, os_, out
+
+    def attend(self, cache, batch, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
+        """Attention of q [rows, n_q * d] (f32 or bf16; any row stride) over the cache; scale: 1 / sqrt(d) by default. The rules are those of
+        `oxhip_attend_rules`. Returns out, of q's shape and type; rows behind the last sequence are left as `out` has them: in a new one they
+        may hold anything."""
+        qp, qs, n_q, qd, rules, op, os_, out = self._attend_call(cache, batch, q, cap, slopes, window, prefix, first, out)
         if batch.rows and not self.lib.oxhip_dev_attend(self.ctx, cache.ref, batch.ref, qp, qs, n_q, qd, cache.d**-0.5 if scale is None else scale, rules, op, os_,
                                                         self._stream_here()):
             raise RuntimeError(self.last_error())
         return out
+
+    def attend_shared(self, cache, batch, shared, q, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
+        """`attend` of a batch whose sequences begin, group by group, with the same tokens (`KvShared`): these are read where the table of a group's
+        first sequence names them, once for several rows."""
+        qp, qs, n_q, qd, rules, op, os_, out = self._attend_call(cache, batch, q, cap, slopes, window, prefix, first, out)
+        if shared.device != self.device:
+            raise ValueError(f"shared: wanted on cuda:{self.device}")
+        if batch.rows and not self.lib.oxhip_dev_attend_shared(self.ctx, cache.ref, batch.ref, shared.ref, qp, qs, n_q, qd, cache.d**-0.5 if scale is None else scale, rules,
+                                                               op, os_, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out
+
+    def kv_summary(self, cache, span=64):
+        """A new summary of a cache: the mean keys of its spans of `span` tokens (a power of two, 32 at least and a page at most)."""
+        import torch
+        if span < 32 or cache.page_tokens % span:
+            raise ValueError(f"span: {span}, wanted a power of two, 32 at least and {cache.page_tokens} at most")
+        shape, dev = (cache.k.shape[0], cache.n_kv, cache.page_tokens // span), cache.k.device
+        return KvSummary(torch.zeros((*shape, cache.d), dtype=torch.int8, device=dev), torch.zeros(shape, dtype=torch.float32, device=dev), span)
+
+    def _summed(self, cache, batch, summary):
+        self._held(cache, batch)
+        if summary.device != self.device or summary.shape != (cache.k.shape[0], cache.n_kv, cache.page_tokens // summary.span, cache.d):
+            raise ValueError(f"summary: {summary.shape} of spans of {summary.span} on cuda:{summary.device} is not one of this cache on cuda:{self.device}")
+
+    def kv_summarize(self, cache, batch, summary):
+        """The mean keys of the spans that the batch's rows touch, made anew (behind their append)."""
+        self._summed(cache, batch, summary)
+        if batch.rows and not self.lib.oxhip_dev_kv_summarize(self.ctx, cache.ref, batch.ref, summary.ref, self._stream_here()):
+            raise RuntimeError(self.last_error())
+
+    def kv_summary_read(self, cache, batch, summary, count):
+        """The mean keys that the last `count` spans of every sequence stand for: f32 [n_seqs, count, n_kv, d]."""
+        self._summed(cache, batch, summary)
+        out = cache.k_scale.new_empty((batch.n_seqs, count, cache.n_kv, cache.d))
+        if count and not self.lib.oxhip_dev_kv_summary_read(self.ctx, cache.ref, batch.ref, summary.ref, count, out.data_ptr(), self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out
+
+    def kv_select(self, cache, batch, summary, q, count, first=1, last=1, out=None):
+        """For every row of q [rows, n_q * d] and key head, `count` spans of the cache: the first and last ones, and those whose mean keys score best.
+        int32 [rows, n_kv, count], ascending, -1 behind the last; rows behind the last sequence are left as `out` has them."""
+        self._summed(cache, batch, summary)
+        dev, n_q = self.device, math.prod(q.shape[1:]) // cache.d
+        qp, qs, qd = _rows("q", q, n_q * cache.d, batch.rows, dev)
+        if out is None:
+            out = batch.kv_len.new_empty((q.shape[0], cache.n_kv, count))
+        elif tuple(out.shape[1:]) != (cache.n_kv, count) or out.shape[0] < batch.rows:
+            raise ValueError(f"out: shape {tuple(out.shape)}, wanted [{batch.rows}, {cache.n_kv}, {count}]")
+        if batch.rows and not self.lib.oxhip_dev_kv_select(self.ctx, cache.ref, batch.ref, summary.ref, qp, qs, n_q, qd, count, first, last, _array("out", out, _torch.int32, dev),
+                                                           self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out
+
+    def attend_selected(self, cache, batch, q, chosen, span, scale=None, cap=0.0, slopes=None, window=0, prefix=None, first=None, out=None):
+        """`attend` over the spans of `span` tokens alone that `chosen` int32 [rows, n_kv, count] names (`kv_select`)."""
+        qp, qs, n_q, qd, rules, op, os_, out = self._attend_call(cache, batch, q, cap, slopes, window, prefix, first, out)
+        if chosen.dim() != 3 or chosen.shape[0] < batch.rows or chosen.shape[1] != cache.n_kv:
+            raise ValueError(f"chosen: shape {tuple(chosen.shape)}, wanted [{batch.rows}, {cache.n_kv}, count]")
+        if batch.rows and not self.lib.oxhip_dev_attend_selected(self.ctx, cache.ref, batch.ref, _array("chosen", chosen, _torch.int32, self.device), chosen.shape[2], span, qp, qs, n_q,
+                                                                 qd, cache.d**-0.5 if scale is None else scale, rules, op, os_, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return out
+
+    def sample(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, want_logp=True):
+        """The draw of `oxhip_dev_sample` from rows of logits [rows, vocab] (f32 or bf16; any row stride) by the random numbers u f32 [rows]: (next int32
+        [rows], logp f32 [rows] or None). temperature, top_p, min_p f32 [rows], top_k int32 [rows]."""
+        t, vocab = logits.shape
+        dev, f32 = self.device, _torch.float32
+        lp, ls, ld = _rows("logits", logits, vocab, t, dev)
+        rules = None
+        if temperature is not None or top_k is not None or top_p is not None or min_p is not None:
+            rules = C.byref(SampleRulesC(_array("temperature", temperature, f32, dev, t), _array("top_k", top_k, _torch.int32, dev, t), _array("top_p", top_p, f32, dev, t),
+                                         _array("min_p", min_p, f32, dev, t)))
+        up = _array("u", u, f32, dev, t)
+        both = u.new_empty((2, t))
+        at = both.data_ptr()
+        if t and not self.lib.oxhip_dev_sample(self.ctx, lp, ls, t, vocab, ld, rules, up, at, at + 4 * t if want_logp else None, self._stream_here()):
+            raise RuntimeError(self.last_error())
+        return both[0].view(_torch.int32), both[1] if want_logp else None
 
     def adjust_logits(self, logits, out=None, want_out=True, want_next=True, history=None, history_len=None, prompt_len=None, repetition=None,
                       presence=None, frequency=None, bias_start=None, bias_id=None, bias=None, allowed=None, allowed_row=None):

@@ -1,0 +1,214 @@
+"""The draw of next tokens against the same in 64 bits (lists_ref.sample): the token is the same, its log-probability within the roundings of f32."""
+import numpy as np
+import pytest
+import torch
+
+from tests.lists_ref import sample
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be():
+    from oxinfer_amd import HipBackend
+    b = HipBackend(0)
+    yield b
+    b.close()
+
+
+def rules_of(t, rng, names):
+    made = dict(temperature=rng.uniform(0.3, 1.5, t).astype(np.float32), top_k=rng.integers(0, 60, t).astype(np.int32), top_p=rng.uniform(0.2, 1.05, t).astype(np.float32), min_p=rng.uniform(-0.05, 0.3, t).astype(np.float32))
+    return {k: made[k] for k in names}
+
+
+def check(be, x, u, strided=False, **rules):
+    """x: a torch tensor of logits on the device. logp: weights are off by 2^-(62 - log2 vocab) of the largest at most, their sums by as many; then one
+    rounding to f32, and one of the logarithm's argument."""
+    t, vocab = x.shape
+    up = {k: torch.from_numpy(v).cuda() for k, v in rules.items()}
+    got, logp = be.sample(x, torch.from_numpy(u).cuda(), **up)
+    want, logs = sample(x.double().cpu().numpy(), u, **rules)
+    assert got.tolist() == want.tolist()
+    logp = logp.double().cpu().numpy()
+    live = want >= 0
+    assert (logp[~live] == -np.inf).all()
+    bits = max(1, (vocab - 1).bit_length())
+    with np.errstate(over="ignore"):
+        share = 2.0 ** (bits - 61) * (1 + np.exp(-logs[live]))  # (the token's own weight may be small beside the largest)
+    assert (np.abs(logp[live] - logs[live]) <= 2.0**-24 * np.abs(logs[live]) + vocab * share + 2.0**-50).all()
+    return got
+
+
+NAMES = ("temperature", "top_k", "top_p", "min_p")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 4095, 4096, 4097, 32003, 128256])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_sizes(be, rows, vocab, dtype):
+    rng = np.random.default_rng(vocab + rows)
+    x = torch.from_numpy(3 * rng.normal(size=(rows, vocab))).cuda().to(dtype)
+    check(be, x, rng.random(rows).astype(np.float32), **rules_of(rows, rng, NAMES))
+
+
+@pytest.mark.parametrize("names", [(), ("temperature",), ("top_k",), ("top_p",), ("min_p",), ("top_k", "top_p"), ("top_k", "min_p"), ("top_p", "min_p"), NAMES], ids=str)
+@pytest.mark.parametrize("spread", [0.01, 1.0, 5.0, 100.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rules(be, names, spread, dtype):
+    """Logits that hardly differ, ordinary ones, and ones of which one is all."""
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(spread * rng.normal(size=(40, 20011))).cuda().to(dtype)
+    check(be, x, rng.random(40).astype(np.float32), **rules_of(40, rng, names))
+
+
+def test_many_rows_and_shares(be):
+    """The same row with random numbers from 0 to 1: each token comes as often as its weight says."""
+    rng = np.random.default_rng(1)
+    row = 2 * rng.normal(size=3001)
+    n = 4096
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    x = torch.from_numpy(np.repeat(row[None], n, 0)).cuda().float()
+    got = check(be, x, u, top_k=np.full(n, 50, np.int32), top_p=np.full(n, 0.8, np.float32)).cpu().numpy()
+    assert (np.diff(got) >= 0).all()  # (in the order of the ids)
+    w = np.exp(x[0].double().cpu().numpy())
+    order = np.argsort(-w, kind="stable")[:50]
+    kept = order[: 1 + int((np.cumsum(w[order])[:-1] < 0.8 * w[order].sum()).sum())]
+    count = np.bincount(got, minlength=3001)
+    share = np.zeros(3001)
+    share[kept] = w[kept] / w[kept].sum()
+    assert (np.abs(count - n * share) <= 1.001).all() and set(np.flatnonzero(count)) <= set(kept.tolist())
+
+
+def test_equal_logits_go_by_their_ids(be):
+    """Whole rows alike, and few different values, so that the limits fall among equal ones."""
+    rng = np.random.default_rng(2)
+    x = np.zeros((12, 9000))
+    x[4:8] = rng.integers(-3, 3, (4, 9000))
+    x[8:] = rng.integers(0, 2, (4, 9000)) * 1e-30
+    u = np.linspace(0, 0.999, 12).astype(np.float32)
+    for rules in (dict(), dict(top_k=np.full(12, 7, np.int32)), dict(top_k=np.full(12, 5000, np.int32)), dict(top_p=np.full(12, 0.3, np.float32)), dict(top_k=np.full(12, 100, np.int32), top_p=np.full(12, 0.255, np.float32)),
+                  dict(min_p=np.full(12, 1.0, np.float32)), dict(min_p=np.full(12, 0.3, np.float32), top_k=np.full(12, 4000, np.int32))):
+        for dtype in (torch.float32, torch.bfloat16):
+            check(be, torch.from_numpy(x).cuda().to(dtype), u, **rules)
+
+
+def test_values_a_hairs_breadth_apart(be):
+    """f32 values next to each other, around zero and around a large one, that the limits tell apart."""
+    rng = np.random.default_rng(2)
+    near = np.float32(1000.0) + np.arange(-300, 300).astype(np.float32) * np.float32(2.0**-14)
+    tiny = rng.integers(-300, 300, 600).astype(np.float32) * np.float32(1e-45)
+    mixed = np.concatenate([tiny[:300], np.float32(8.0) + np.arange(300).astype(np.float32) * np.float32(2.0**-20)])
+    x = torch.from_numpy(np.stack([rng.permutation(v) for v in (near, tiny, mixed)])).cuda()
+    for k in (1, 2, 299, 300, 301, 450, 599):
+        check(be, x, np.array([0.999, 0.5, 0.9999], np.float32), top_k=np.full(3, k, np.int32))
+        check(be, x, np.array([0.1, 0.7, 0.99], np.float32), top_k=np.full(3, k, np.int32), temperature=np.array([1e-3, 1e30, 0.01], np.float32), top_p=np.full(3, 0.9, np.float32))
+
+
+def test_temperatures_at_their_ends(be):
+    rng = np.random.default_rng(4)
+    heats = np.array([0.0, -1.0, np.nan, 1e-45, 1e-38, 1e-3, 1e3, 1e30, 3e38, np.inf, -0.0, -np.inf], np.float32)
+    x = torch.from_numpy(3 * rng.normal(size=(12, 5000))).cuda().float()
+    x[:, 77] = x.amax(1)  # (two best ones)
+    for rules in (dict(), dict(top_k=np.full(12, 20, np.int32)), dict(top_p=np.full(12, 0.5, np.float32))):
+        check(be, x, rng.random(12).astype(np.float32), temperature=heats, **rules)
+
+
+def test_limits_at_their_ends(be):
+    rng = np.random.default_rng(4)
+    x = torch.from_numpy(3 * rng.normal(size=(10, 5000))).cuda().float()
+    u = rng.random(10).astype(np.float32)
+    check(be, x, u, top_p=np.array([0.0, -1.0, 1.0, 2.0, np.nan, 1e-30, 1 - 2.0**-24, np.inf, -np.inf, 0.5], np.float32))
+    check(be, x, u, min_p=np.array([0.0, -1.0, 1.0, 2.0, np.nan, 1e-30, 1 - 2.0**-24, np.inf, -np.inf, 0.5], np.float32))
+    check(be, x, u, top_k=np.array([0, -1, 1, 2, 4999, 5000, 5001, 2**31 - 1, -(2**31), 3], np.int32))
+    for at in (0.0, 1e-45, 1 - 2.0**-24, 1.0, 2.0, -1.0, np.nan, np.inf):
+        check(be, x, np.full(10, at, np.float32), top_k=np.full(10, 30, np.int32))
+        check(be, x, np.full(10, at, np.float32))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinities_and_nan(be, dtype):
+    rng = np.random.default_rng(6)
+    x = 3 * rng.normal(size=(9, 6000))
+    x[0] = -np.inf
+    x[1] = np.nan
+    x[2, rng.permutation(6000)[:5990]] = -np.inf
+    x[3, rng.permutation(6000)[:3000]] = np.nan
+    x[4, [5, 900, 5999]] = np.inf
+    x[5, :] = -np.inf
+    x[5, 4321] = -3e38
+    x[6, 10] = 3e38
+    x[7] = rng.choice([-3e38, 3e38, 0.0], 6000)
+    x[8, 0] = np.inf
+    x[8, 1] = np.nan
+    up = torch.from_numpy(x).cuda().to(dtype)
+    for u in (0.0, 0.4, 0.9999):
+        for rules in ({}, dict(top_k=np.full(9, 2, np.int32)), dict(top_p=np.full(9, 0.6, np.float32)), dict(min_p=np.full(9, 0.1, np.float32)), rules_of(9, rng, NAMES), dict(temperature=np.zeros(9, np.float32))):
+            check(be, up, np.full(9, u, np.float32), **rules)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_addresses(be, dtype):
+    rng = np.random.default_rng(7)
+    flat = torch.from_numpy(3 * rng.normal(size=1 + 5 * 5017)).cuda().to(dtype)
+    check(be, flat[: 5 * 5016].view(5, 5016)[:, :5000], rng.random(5).astype(np.float32), **rules_of(5, rng, NAMES))
+    check(be, flat[1:].view(5, 5017)[:, :5003], rng.random(5).astype(np.float32), **rules_of(5, rng, NAMES))
+
+
+def test_behind_the_logits_rules_by_a_recorded_plan(be):
+    """Rules, then the draw, recorded once; replays over other logits and random numbers are the eager results, and tokens that a mask takes away never come."""
+    rng = np.random.default_rng(8)
+    t, vocab = 6, 40000
+    x, out, u = torch.randn(t, vocab, device="cuda") * 3, torch.empty(t, vocab, device="cuda"), torch.rand(t, device="cuda")
+    allowed = torch.from_numpy(rng.integers(-2**31, 2**31, (t, vocab // 32)).astype(np.int32)).cuda()
+    rules = {k: torch.from_numpy(v).cuda() for k, v in rules_of(t, rng, NAMES).items()}
+    kept = []
+
+    def step():
+        be.adjust_logits(x, out=out, want_next=False, allowed=allowed)
+        kept.append(be.sample(out, u, **rules))
+
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        plan = be.plan_record(step)
+        held = kept[-1]
+        for i in range(8):
+            x.normal_(0, 3)
+            u.uniform_()
+            for a in held:
+                a.fill_(0)
+            plan.replay()
+            stream.synchronize()
+            got, logp = (a.clone() for a in held)
+            step()
+            stream.synchronize()
+            assert torch.equal(got, kept[-1][0]) and torch.equal(logp, kept[-1][1])
+            want, _ = sample(out.double().cpu().numpy(), u.cpu().numpy(), **{k: v.cpu().numpy() for k, v in rules.items()})
+            assert got.tolist() == want.tolist()
+            assert all(int(allowed[r, v // 32]) >> (v % 32) & 1 for r, v in enumerate(got.tolist()))
+    del plan
+
+
+def test_the_same_token_every_time(be):
+    rng = np.random.default_rng(9)
+    x = torch.from_numpy(2 * rng.normal(size=(16, 50000))).cuda().float()
+    u = torch.rand(16, device="cuda")
+    rules = {k: torch.from_numpy(v).cuda() for k, v in rules_of(16, rng, NAMES).items()}
+    a, la = be.sample(x, u, **rules)
+    for _ in range(20):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            b, lb = be.sample(x, u, **rules)
+            torch.cuda.current_stream().synchronize()
+        assert torch.equal(a, b) and torch.equal(la, lb)
+    assert be.sample(x, u, want_logp=False, **rules)[1] is None
+
+
+def test_the_bindings_refusals(be):
+    x, u = torch.randn(3, 100, device="cuda"), torch.rand(3, device="cuda")
+    i = torch.zeros(3, dtype=torch.int32, device="cuda")
+    for bad in (dict(logits=x.half()), dict(logits=x.cpu()), dict(u=u[:2]), dict(u=u.double()), dict(u=u.cpu()), dict(temperature=i), dict(top_k=u), dict(top_k=i[:2]), dict(top_p=u.double()), dict(min_p=u[:1]), dict(logits=x.t().contiguous().t())):
+        with pytest.raises((ValueError, RuntimeError)):
+            be.sample(**(dict(logits=x, u=u) | bad))
+    assert be.sample(x[:0], u[:0])[0].shape == (0,)

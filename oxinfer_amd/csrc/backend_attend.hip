@@ -311,7 +311,10 @@ int oxhip_dev_sample(oxhip_ctx* c, const void* logits, size_t stride, size_t row
     if (!rows) return 1;
     OnDevice on(c->device);
     if (!on.ok) return refuse(who, "hipSetDevice failed");
-    HIP_TRY(launch_sample(a, dtype == OXHIP_BF16, static_cast<hipStream_t>(stream)), "sample launch");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DecodeScratch* sc = parts(c, s, who);
+    if (!sc) return 0;
+    HIP_TRY(launch_sample(a, dtype == OXHIP_BF16, *sc, s), "sample launch");
     return 1;
 }
 

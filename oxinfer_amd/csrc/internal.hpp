@@ -299,7 +299,7 @@ hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const 
 struct LogitArgs;
 hipError_t launch_logits(const LogitArgs& a, bool bf16, hipStream_t s);
 struct SampleArgs;
-hipError_t launch_sample(const SampleArgs& a, bool bf16, hipStream_t s);
+hipError_t launch_sample(const SampleArgs& a, bool bf16, const DecodeScratch& sc, hipStream_t s);
 
 hipError_t launch_fill_zero(uint32_t* p, size_t n, hipStream_t s);  // n dwords, by a kernel on `s`
 

@@ -1,8 +1,24 @@
-// The arguments of the draw's launch (sample.hip).
+// The arguments of the draw's launches (sample.hip).
 #pragma once
 #include "internal.hpp"
 
 namespace oxhip {
+
+// Logits of a row that a workgroup takes, eight of each thread; slices that a row's sums are kept of.
+constexpr uint32_t SAMPLE_SLICE = 4096, SAMPLE_THREADS = 512, SAMPLE_SLICES = 256;
+// Steps of weight, a quarter of an octave each, that the first pass counts tokens by: past them a weight is 0.
+constexpr uint32_t SAMPLE_STEPS = 192;
+
+// What the first pass finds out about a row: see sample_scan_kernel.
+struct SampleRow {
+    float top, low, high;  // the largest logit; steps of the tokens among which a limit falls
+    uint32_t flags;
+};
+// What the second pass finds out about a slice.
+struct SampleSlice {
+    unsigned long long all, above, kept;  // weights: of all its tokens, of those above the limit's steps, of those of these that min-p leaves
+    uint32_t n_above, n;                  // tokens above; tokens in them
+};
 
 struct SampleArgs {
     const void* x;
@@ -13,7 +29,15 @@ struct SampleArgs {
     int32_t* next;
     float* logp;    // or none
     uint32_t unit;  // weights are whole numbers, 2^unit being the largest
-    uint32_t vec;
+    uint32_t slices, vec, row0;
+    // scratch
+    unsigned long long* step;    // [rows][slices][SAMPLE_STEPS]: tokens << 48 | weights in 2^-32
+    float* best;                 // [rows][slices]
+    SampleRow* row;              // [rows]
+    SampleSlice* slice;          // [rows][slices]
+    unsigned long long* token;   // [rows][slices][room]: order_of a logit << 32 | id
+    uint32_t room;
+    uint32_t* counters;  // one of each row, zero between launches
 };
 
 }  // namespace oxhip

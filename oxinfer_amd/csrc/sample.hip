@@ -14,10 +14,10 @@
 
 namespace oxhip {
 
-constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_FEW = 256, SAMPLE_HELD = 8192;
+constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_FEW = 2048, SAMPLE_HELD = 8192, SAMPLE_WITH = 256;
 constexpr uint32_t WAVES = SAMPLE_THREADS / 64;
 constexpr double LOG2E_D = 1.4426950408889634074;
-enum { ROW_GREEDY = 1, ROW_EMPTY = 2, ROW_WHOLE = 4, ROW_K = 8, ROW_P = 16, ROW_SUMS = 32, ROW_ALONE = 64 };
+enum { ROW_GREEDY = 1, ROW_EMPTY = 2, ROW_WHOLE = 4, ROW_K = 8, ROW_P = 16, ROW_SUMS = 32 };
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // in the same order, 0 and -0 alike
     const uint32_t b = __float_as_uint(x + 0.0f);
@@ -25,21 +25,39 @@ __device__ __forceinline__ uint32_t order_of(float x) {  // in the same order, 0
 }
 __device__ __forceinline__ float of_order(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
 
+// A value from another lane (0 from none), and sums over a wave's lanes: up to one's own, and of all.
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T lane_of(T v) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, true);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, true));
+    }
+}
 template <class T>
 __device__ __forceinline__ T wave_upto(T v) {
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (int y = 1; y < 64; y *= 2) {
-        const T o = __shfl_up(v, y);
-        v += lane >= (uint32_t)y ? o : (T)0;
-    }
+    v += lane_of<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v += lane_of<0x112, 0xF>(v);
+    v += lane_of<0x114, 0xF>(v);
+    v += lane_of<0x118, 0xF>(v);
+    v += lane_of<0x142, 0xA>(v);  // row_bcast:15, then :31
+    v += lane_of<0x143, 0xC>(v);
     return v;
 }
 template <class T>
+__device__ __forceinline__ T of_lane(T v, int lane) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(T, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane));
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+template <class T>
 __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int y = 32; y; y >>= 1) v += __shfl_xor(v, y);
-    return v;
+    return of_lane(wave_upto(v), 63);
 }
 template <class T>
 __device__ __forceinline__ void put(T* p, T v) {
@@ -161,11 +179,12 @@ __device__ __forceinline__ Weigher weigher(const SampleArgs& a, const Rules& r, 
 
 template <bool BF16>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs a) {
-    // (eight counts of a step side by side: tokens are many and steps few, and 64 lanes' additions to one place go one after the other)
+    // Tokens are counted for top-k, their weights summed for top-p alone, as whole numbers of 2^-32 of the slice's largest. (Eight sums of a step side by side: tokens are
+    // many and steps few, and 64 lanes' additions to one place go one after the other. One sum of a step, in f32, took 60 us of 64 rows of 151936, sixteen 47, these 11.)
     constexpr uint32_t COPIES = 8, GROUPS = 4;
-    __shared__ unsigned long long step_s[SAMPLE_STEPS][COPIES];
-    __shared__ float top_s[WAVES], best_s[SAMPLE_SLICES], down_s[SAMPLE_SLICES], mass_s[GROUPS][SAMPLE_STEPS];
-    __shared__ uint32_t count_s[GROUPS][SAMPLE_STEPS];
+    __shared__ __align__(16) unsigned long long step_s[SAMPLE_STEPS][COPIES];
+    __shared__ uint32_t sum_s[GROUPS][SAMPLE_STEPS];
+    __shared__ float top_s[WAVES], best_s[SAMPLE_SLICES], down_s[SAMPLE_SLICES];
     static_assert(GROUPS * (SAMPLE_STEPS / 2) <= SAMPLE_THREADS, "two steps a thread");
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slice = blockIdx.x / a.rows, at = blockIdx.x % a.rows, row = a.row0 + at;
     const Rules r = rules_of(a, row);
@@ -181,26 +200,26 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
         return v;
     };
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    for (uint32_t i = tid; i < SAMPLE_STEPS * COPIES; i += SAMPLE_THREADS) (&step_s[0][0])[i] = 0;
+    for (uint32_t i = 2 * tid; i < SAMPLE_STEPS * COPIES; i += 2 * SAMPLE_THREADS) *reinterpret_cast<uint4*>(&step_s[0][0] + i) = make_uint4(0, 0, 0, 0);
     top = largest(top);
     const float scale = step_scale(r.heat);
-    const bool sorted = !r.greedy && scale > 1e-30f && scale < 1e30f, limits = sorted && (r.k > 0 || r.p < 1.0f);
-    unsigned long long* steps = a.step + ((size_t)at * a.slices + slice) * SAMPLE_STEPS;
+    const bool sorted = !r.greedy && scale > 1e-30f && scale < 1e30f, number = r.k > 0, limits = sorted && (number || r.p < 1.0f);
+    uint32_t* steps = a.step + ((size_t)at * a.slices + slice) * SAMPLE_STEPS;
     if (limits) {
         const float high = step_of(top, scale);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float down = high - step_of(x[j], scale);  // (of infinite ones NaN or infinite)
             if (!(down < (float)SAMPLE_STEPS)) continue;
-            const float w = __builtin_amdgcn_exp2f((x[j] - top) * (0.25f * scale));
-            atomicAdd(&step_s[(int)down][lane % COPIES], 1ull << 48 | (uint32_t)(w * 4294967040.0f));
+            const uint32_t w = (uint32_t)(__builtin_amdgcn_exp2f((x[j] - top) * (0.25f * scale)) * 4294967040.0f);
+            atomicAdd(&step_s[(int)down][lane % COPIES], number ? 1ull : (unsigned long long)w);
         }
         __syncthreads();
         if (tid < SAMPLE_STEPS) {
             unsigned long long v = 0;
 #pragma unroll
             for (uint32_t c = 0; c < COPIES; c++) v += step_s[tid][(tid + c) % COPIES];
-            put(&steps[tid], v);
+            put(&steps[tid], number ? (uint32_t)v : __float_as_uint((float)v * 0x1p-32f));
         }
     }
     if (tid == 0) put(&a.best[(size_t)at * a.slices + slice], top);
@@ -228,22 +247,19 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
             float m[2] = {0.0f, 0.0f};
             for (uint32_t s = group; s < a.slices; s += GROUPS) {
                 const float down = down_s[s];
-                const unsigned long long* from = a.step + ((size_t)at * a.slices + s) * SAMPLE_STEPS;
+                const uint32_t* from = a.step + ((size_t)at * a.slices + s) * SAMPLE_STEPS;
 #pragma unroll
                 for (uint32_t h = 0; h < 2; h++) {
                     const uint32_t j = j0 + h * (SAMPLE_STEPS / 2);
                     if (down <= (float)j) {
-                        const unsigned long long v = get(&from[j - (uint32_t)down]);
-                        n[h] += (uint32_t)(v >> 48);
-                        m[h] += (float)(v & ((1ull << 48) - 1)) * 0x1p-32f * best_s[s];
+                        const uint32_t v = get(&from[j - (uint32_t)down]);
+                        n[h] += v;
+                        m[h] += __uint_as_float(v) * best_s[s];
                     }
                 }
             }
 #pragma unroll
-            for (uint32_t h = 0; h < 2; h++) {
-                count_s[group][j0 + h * (SAMPLE_STEPS / 2)] = n[h];
-                mass_s[group][j0 + h * (SAMPLE_STEPS / 2)] = m[h];
-            }
+            for (uint32_t h = 0; h < 2; h++) sum_s[group][j0 + h * (SAMPLE_STEPS / 2)] = number ? n[h] : __float_as_uint(m[h]);
         }
         __syncthreads();
         if (tid < 64) {  // PER steps a lane
@@ -257,8 +273,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
                 m_to[j] = j ? m_to[j ? j - 1 : 0] : 0.0f;
 #pragma unroll
                 for (uint32_t g = 0; g < GROUPS; g++) {
-                    n_to[j] += count_s[g][PER * lane + j];
-                    m_to[j] += mass_s[g][PER * lane + j];
+                    n_to[j] += sum_s[g][PER * lane + j];
+                    m_to[j] += __uint_as_float(sum_s[g][PER * lane + j]);
                 }
             }
             const uint32_t n_before = wave_upto(n_to[PER - 1]) - n_to[PER - 1];
@@ -268,8 +284,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
                 n_to[j] += n_before;
                 m_to[j] += m_before;
             }
-            const uint32_t n_all = __shfl(n_to[PER - 1], 63);
-            const float m_all = __shfl(m_to[PER - 1], 63);
+            const uint32_t n_all = of_lane(n_to[PER - 1], 63);
+            const float m_all = of_lane(m_to[PER - 1], 63);
             constexpr int NONE = 100000;
             auto first = [&](auto reached) {  // the first step j with reached(j)
                 int at = NONE;
@@ -280,22 +296,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
                 }
                 return at;
             };
-            auto upto = [&](auto (&v), int step) {  // v up to and with a step
-                auto r = v[0];
-#pragma unroll
-                for (uint32_t j = 1; j < PER; j++) r = (uint32_t)step % PER == j ? v[j] : r;
-                return __shfl(r, step / (int)PER);
-            };
             constexpr float NEAR = 4e-5f;  // (weights in f32, cut off at 2^-32 of a slice's largest; the slices' sums in f32)
-            int k_at = NONE, p_lo = NONE, p_hi = NONE;
-            const bool k_on = r.k > 0 && (uint32_t)r.k < n_all;
+            int k_at = NONE, p_lo = 0, p_hi = SAMPLE_STEPS - 1;
+            const bool k_on = number && (uint32_t)r.k < n_all;
             if (k_on) k_at = first([&](uint32_t j) { return n_to[j] >= (uint32_t)r.k; });
-            const float sum_least = !k_on ? m_all : k_at ? upto(m_to, k_at - 1) : 0.0f, sum_most = k_on ? upto(m_to, k_at) : m_all;
             bool p_on = r.p < 1.0f;
-            if (p_on) {
-                const float p = fmaxf(r.p, 0.0f), lo = p * sum_least * (1.0f - NEAR), hi = p * sum_most * (1.0f + NEAR);
-                p_lo = first([&](uint32_t j) { return m_to[j] >= lo; });
-                p_hi = min(first([&](uint32_t j) { return m_to[j] >= hi; }), (int)SAMPLE_STEPS - 1);
+            if (p_on && !number) {
+                const float want = fmaxf(r.p, 0.0f) * m_all;
+                p_lo = first([&](uint32_t j) { return m_to[j] >= want * (1.0f - NEAR); });
+                p_hi = min(first([&](uint32_t j) { return m_to[j] >= want * (1.0f + NEAR); }), (int)SAMPLE_STEPS - 1);
                 p_lo = min(p_lo, p_hi);
             }
             // Tokens that min-p leaves lie within so many steps of the best: limits below them are none.
@@ -307,10 +316,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
             if (k_in || p_on) {
                 int from = p_on ? p_lo : k_at, to = p_on ? p_hi : k_at;
                 if (k_in && p_on) from = 0, to = k_at;  // (top-p of what top-k leaves: all of that is looked at)
-                if (upto(n_to, to) <= SAMPLE_FEW) from = 0;
                 out.low = high - (float)to;
                 out.high = from == 0 ? __builtin_inff() : high - (float)from;
-                out.flags = (k_in ? ROW_K : 0u) | (p_on ? ROW_P : 0u) | (k_in ? 0u : ROW_SUMS) | (from == 0 ? ROW_ALONE : 0u);
+                out.flags = (k_in ? ROW_K : 0u) | (p_on ? ROW_P : 0u) | (k_in ? 0u : ROW_SUMS);
             }
         }
     }
@@ -319,16 +327,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
 
 // ---- what finds a limit, and a draw ---------------------------------------------------------------------------------------------------------
 
-struct Narrowing {
-    uint32_t count[SAMPLE_BINS];
-    unsigned long long weight[SAMPLE_BINS];
-};
-struct DrawShared {
+struct alignas(16) DrawShared {
     union {
-        Narrowing bins;
+        unsigned long long bins[SAMPLE_BINS];
         struct {
-            unsigned long long weight[SAMPLE_FEW];
-            uint32_t order[SAMPLE_FEW], rank[SAMPLE_FEW];
+            unsigned long long token[SAMPLE_FEW], weight[SAMPLE_FEW + 1];
+            uint32_t start[SAMPLE_BINS + 1];
         } few;
     };
     unsigned long long slice[SAMPLE_SLICES], sums[WAVES], found[3];
@@ -342,17 +346,27 @@ struct Cut {
 };
 
 // The first tokens, in the order of their logits, that come to `want` by number or by weight, of the tokens that each(f) gives to f(logits, ids) by eight a thread
-// (-infinity: none), those of cut.order and above, `above` lying above them all. By parts of the range from_v .. to_v (falling) of logits first, then by parts of the range of order_of's numbers that is left,
-// until a part is one number. False: all together do not come to it.
-template <class Each>
+// (-infinity: none), those of cut.order and above, `above` lying above them all; from_v .. to_v (falling): about where their logits lie. By parts of a range of
+// order_of's numbers, until a part is one number; where the range is wide, by parts of the range of the logits themselves first. False: all together do not come
+// to it.
+template <bool BF16, class Each>
 __device__ __forceinline__ bool narrow(DrawShared& sh, const Weigher& weight, Each each, bool number, uint64_t want, uint64_t above, double from_v, double to_v, Cut& cut) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    constexpr uint32_t PER = SAMPLE_BINS / SAMPLE_THREADS;
+    constexpr uint32_t PER = SAMPLE_BINS / SAMPLE_THREADS, ONE = BF16 ? 16 : 0;  // (a bf16 has 16 bits: that many numbers of order_of are one value)
     const double wide = from_v - to_v, scale = wide > 0.0 && wide < 1e300 ? (double)(SAMPLE_BINS - 1) / wide : 0.0;
-    uint32_t shift = 0, part0 = 0, low = 0, high = 0xFFFFFFFFu;
     const uint32_t least = cut.order;
-    for (int level = 0;; level++) {
-        for (uint32_t i = tid; i < SAMPLE_BINS; i += SAMPLE_THREADS) sh.bins.count[i] = 0, sh.bins.weight[i] = 0;
+    auto order_near = [&](double v, double room) { return v + room < -3.4e38 ? 0u : v + room > 3.4e38 ? 0xFFFFFFFFu : order_of((float)(v + room)); };
+    const double room0 = 1e-6 * (fabs(from_v) + fabs(to_v));
+    uint32_t low = order_near(to_v, -room0), high = order_near(from_v, room0), shift = 0, part0 = 0;
+    bool values = !(high > low && (high - low) >> 22 == 0);  // (two rounds of 2048 parts of numbers do otherwise)
+    bool open = !values, of_part = false;  // what lies outside of low .. high counts to its ends; only logits of the part part0 of the first round count
+    auto settle = [&]() {
+        const uint32_t width = high - low;
+        shift = max(ONE, width >= SAMPLE_BINS ? 21u - (uint32_t)__builtin_clz(width) : 0u);
+    };
+    settle();
+    for (;;) {
+        for (uint32_t i = 2 * tid; i < SAMPLE_BINS; i += 2 * SAMPLE_THREADS) *reinterpret_cast<ulonglong2*>(&sh.bins[i]) = ulonglong2{0, 0};
         __syncthreads();
         each([&](const float (&x)[8], const uint32_t (&)[8]) {
             uint32_t p[8];
@@ -360,9 +374,13 @@ __device__ __forceinline__ bool narrow(DrawShared& sh, const Weigher& weight, Ea
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const uint32_t o = order_of(x[j]);
-                const double d = (from_v - (double)x[j]) * scale;
-                p[j] = d > 0.0 ? (uint32_t)fmin(d, (double)(SAMPLE_BINS - 1)) : 0u;
-                if (level) p[j] = p[j] != part0 || o < low || o > high ? SAMPLE_BINS : (high - o) >> shift;
+                uint32_t v = 0;
+                if (values || of_part) {
+                    const double d = (from_v - (double)x[j]) * scale;
+                    v = d > 0.0 ? (uint32_t)fmin(d, (double)(SAMPLE_BINS - 1)) : 0u;
+                }
+                const bool out = of_part && v != part0;
+                p[j] = values ? v : open ? (o >= high ? 0u : min((high - o) >> shift, SAMPLE_BINS - 1)) : out || o < low || o > high ? SAMPLE_BINS : (high - o) >> shift;
                 if (o < least || !(x[j] > -__builtin_inff())) p[j] = SAMPLE_BINS;
                 any = any || p[j] < SAMPLE_BINS;
             }
@@ -371,16 +389,13 @@ __device__ __forceinline__ bool narrow(DrawShared& sh, const Weigher& weight, Ea
             weight.of(x, w);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (p[j] < SAMPLE_BINS && w[j]) {
-                    atomicAdd(&sh.bins.count[p[j]], 1u);
-                    if (!number) atomicAdd(&sh.bins.weight[p[j]], (unsigned long long)w[j]);
-                }
+                if (p[j] < SAMPLE_BINS && w[j]) atomicAdd(&sh.bins[p[j]], number ? 1ull : (unsigned long long)w[j]);
         });
         __syncthreads();
         unsigned long long v[PER], mine = 0;
 #pragma unroll
         for (uint32_t j = 0; j < PER; j++) {
-            v[j] = number ? sh.bins.count[PER * tid + j] : sh.bins.weight[PER * tid + j];
+            v[j] = sh.bins[PER * tid + j];
             mine += v[j];
         }
         const unsigned long long upto = wave_upto(mine);
@@ -394,35 +409,39 @@ __device__ __forceinline__ bool narrow(DrawShared& sh, const Weigher& weight, Ea
             if (before < want && before + v[j] >= want) {
                 sh.found[0] = PER * tid + j;
                 sh.found[1] = before;
-                sh.found[2] = sh.bins.count[PER * tid + j];
+                sh.found[2] = v[j];
             }
             before += v[j];
         }
         __syncthreads();
-        const uint32_t in = (uint32_t)sh.found[0], in_it = (uint32_t)sh.found[2];
+        const uint32_t in = (uint32_t)sh.found[0];
         if (in >= SAMPLE_BINS) return false;
         above = sh.found[1];
-        if (level == 0) {
+        if (values) {
             part0 = in;
             // The logits of the part, a little more on both sides; at the ends, and where they reach past what f32 holds, to the end.
             const double from = from_v - (double)in / scale, to = from_v - (double)(in + 1) / scale, room = 1e-6 * (fabs(from_v) + fabs(from) + fabs(to));
-            high = in == 0 || !(scale > 0.0) || !(from + room < 3.4e38) ? 0xFFFFFFFFu : order_of((float)(from + room));
-            low = in + 1 == SAMPLE_BINS || !(scale > 0.0) || !(to - room > -3.4e38) ? 0u : order_of((float)(to - room));
-            low = min(low, high);
+            high = in == 0 || !(scale > 0.0) ? 0xFFFFFFFFu : order_near(from, room);
+            low = in + 1 == SAMPLE_BINS || !(scale > 0.0) ? 0u : min(high, order_near(to, -room));
+            values = false;
+            of_part = true;
         } else {
-            const uint32_t h = high - (in << shift);
-            low = h - low >= (1u << shift) ? h - ((1u << shift) - 1) : low;
-            high = h;
-            if (!shift) {
-                const uint64_t wt = weight(of_order(h)), left = want - above;
-                cut.order = h;
-                cut.ties = (uint32_t)(number ? left : (left + wt - 1) / wt);
-                cut.all_ties = cut.ties >= in_it;
+            const uint32_t h = high - (in << shift), span = (1u << shift) - 1, l = h - low >= span || open ? h - min(h, span) : low;
+            const bool end = open && (in == 0 || in + 1 == SAMPLE_BINS);
+            if (shift <= ONE && !end) {
+                // the one value of the part
+                const uint32_t o = !BF16 ? h : h & 0x80000000u ? h & 0xFFFF0000u : ((h + 1) & 0xFFFF0000u) - 1;
+                const uint64_t wt = number ? 1 : weight(of_order(o)), left = want - above;
+                cut.order = o;
+                cut.ties = (uint32_t)((left + wt - 1) / wt);
+                cut.all_ties = cut.ties >= sh.found[2] / wt;
                 return true;
             }
+            low = open && in + 1 == SAMPLE_BINS ? 0u : l;
+            high = open && in == 0 ? 0xFFFFFFFFu : h;
+            open = false;
         }
-        const uint32_t width = high - low;
-        shift = width >= SAMPLE_BINS ? 21 - __builtin_clz(width) : 0;
+        settle();
         __syncthreads();
     }
 }
@@ -500,10 +519,11 @@ __device__ __forceinline__ uint64_t share_of(float u, uint64_t all) {
     return want < (double)all ? (uint64_t)want + 1 : all;
 }
 
-// The limits of a row and its draw, by a workgroup: the tokens among which the limits fall are given by each(f) (all of the row's: `everything`); sh.slice has the kept weights of all
+// The limits of a row and its draw, by a workgroup: the tokens among which the limits fall are given by each(f), and by by_slices(sums, f), which adds f(logits, ids) up for each
+// slice (all of the row's: `everything`); sh.slice has the kept weights of all
 // others, by slices of `per` ids. `all` and `above`: the weights of all tokens, and of those above; n_above: the number of these.
-template <bool BF16, class Each>
-__device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32_t row, const Rules& r, const Weigher& weight, uint32_t flags, Each each, bool everything, uint32_t slices, uint32_t per,
+template <bool BF16, class Each, class BySlices>
+__device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32_t row, const Rules& r, const Weigher& weight, uint32_t flags, Each each, BySlices by_slices, bool everything, uint32_t slices, uint32_t per,
                                      uint64_t all, uint64_t above, uint32_t n_above, double from_v, double to_v) {
     const uint32_t tid = threadIdx.x;
     Cut cut{0, 0, true};
@@ -511,7 +531,7 @@ __device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32
     if (flags & ROW_GREEDY) {
         cut = Cut{order_of(weight.top_f), 1, false};
     } else {
-        if (flags & ROW_K) limited = narrow(sh, weight, each, true, (uint64_t)(uint32_t)r.k, n_above, from_v, to_v, cut);
+        if (flags & ROW_K) limited = narrow<BF16>(sh, weight, each, true, (uint64_t)(uint32_t)r.k, n_above, from_v, to_v, cut);
         if (flags & ROW_P) {
             if (limited) {
                 uint64_t v = 0;
@@ -525,20 +545,21 @@ __device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32
             }
             const uint64_t want = max((uint64_t)ceil(fmax((double)r.p, 0.0) * (double)all), (uint64_t)1);
             if (above >= want) return false;  // (the first launch's sums were further off than it allows for)
-            if (!narrow(sh, weight, each, false, want, above, from_v, to_v, cut) && !limited) return false;
+            if (!narrow<BF16>(sh, weight, each, false, want, above, from_v, to_v, cut) && !limited) return false;
         }
     }
     const double least = r.least > 0.0f ? fmin((double)r.least, 1.0) * (double)(1ull << a.unit) : 0.0;
     uint32_t tie_end = 0xFFFFFFFFu;  // ids at the cut are kept up to this one
     if (cut.order && !cut.all_ties) {
-        unsigned long long* n = sh.bins.weight;  // (the slices' numbers of ties, in the place of the bins)
+        unsigned long long* n = sh.bins;  // (the slices' numbers of ties, in the place of the bins)
         __syncthreads();
         for (uint32_t s = tid; s < slices; s += SAMPLE_THREADS) n[s] = 0;
         __syncthreads();
-        each([&](const float (&x)[8], const uint32_t (&i)[8]) {
+        by_slices(n, [&](const float (&x)[4], const uint32_t (&)[4]) {
+            uint64_t v = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (order_of(x[j]) == cut.order) atomicAdd(&n[i[j] / per], 1ull);
+            for (int j = 0; j < 4; j++) v += order_of(x[j]) == cut.order ? 1 : 0;
+            return v;
         });
         __syncthreads();
         uint64_t left = cut.ties;
@@ -554,15 +575,14 @@ __device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32
         return (o > cut.order || (o == cut.order && i <= tie_end)) && (double)w >= least ? w : 0;
     };
     __syncthreads();
-    if (cut.order || flags & (ROW_K | ROW_P) || everything) each([&](const float (&x)[8], const uint32_t (&i)[8]) {
-        uint64_t w[8];
-        weight.of(x, w);
+    if (cut.order || everything)
+        by_slices(sh.slice, [&](const float (&x)[4], const uint32_t (&i)[4]) {
+            uint64_t w[4], v = 0;
+            weight.of(x, w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint64_t v = left(x[j], i[j], w[j]);
-            if (v) atomicAdd(&sh.slice[i[j] / per], (unsigned long long)v);
-        }
-    });
+            for (int j = 0; j < 4; j++) v += left(x[j], i[j], w[j]);
+            return v;
+        });
     __syncthreads();
     uint64_t total = 0;
     for (uint32_t s = tid; s < slices; s += SAMPLE_THREADS) total += sh.slice[s];
@@ -582,62 +602,108 @@ __device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32
     }
     return true;
 }
-// The same of a few tokens that are all that may be kept, in LDS (sh.few.order, ids in the order of places): by their ranks.
-__device__ __forceinline__ void draw_few(const SampleArgs& a, DrawShared& sh, uint32_t row, const Rules& r, const Weigher& weight, uint32_t flags, uint32_t n, uint64_t all, uint32_t id, uint32_t order) {
-    const uint32_t tid = threadIdx.x;
-    const bool live = tid < n;
-    const uint64_t w = live ? weight(of_order(order)) : 0;
-    uint32_t rank = 0;
-    if (tid < SAMPLE_FEW) {
-        for (uint32_t j = 0; j < n; j++) {
-            const uint32_t o = sh.few.order[j];
-            rank += o > order || (o == order && j < tid) ? 1u : 0u;
+// The same of n tokens (order_of << 32 | id, by ids) that are all that may be kept, four a thread: by their ranks. A token's rank is the number of tokens in the higher
+// ones of 2048 parts of the range top .. to_v, and of those of its own part that come before it.
+template <bool BF16>
+__device__ __forceinline__ void draw_few(const SampleArgs& a, DrawShared& sh, uint32_t row, const Rules& r, const Weigher& weight, uint32_t flags, const unsigned long long* tokens, uint32_t n,
+                                         uint64_t all, float to_v) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr uint32_t PER = SAMPLE_FEW / SAMPLE_THREADS, BINS = SAMPLE_BINS / SAMPLE_THREADS;
+    static_assert(PER == 4 && BINS == 4, "four tokens and four parts a thread");
+    const float scale = (float)(SAMPLE_BINS - 1) / fmaxf(weight.top_f - to_v, 1e-30f);
+    float x[PER];
+    uint32_t id[PER], part[PER], slot[PER], rank[PER];
+    for (uint32_t i = tid; i <= SAMPLE_BINS; i += SAMPLE_THREADS) sh.few.start[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+        const uint32_t k = PER * tid + j;
+        const unsigned long long t = tokens[min(k, n - 1)];
+        x[j] = k < n ? of_order((uint32_t)(t >> 32)) : -__builtin_inff();
+        id[j] = (uint32_t)t;
+        part[j] = (uint32_t)fminf((weight.top_f - x[j]) * scale, (float)(SAMPLE_BINS - 1));
+        if (k < n) slot[j] = atomicAdd(&sh.few.start[part[j]], 1u);
+    }
+    __syncthreads();
+    // sums over the workgroup, up to a thread's own
+    auto upto = [&](auto v, auto& total) {
+        const auto u = wave_upto(v);
+        __syncthreads();
+        if (lane == 63) sh.sums[wave] = u;
+        __syncthreads();
+        auto before = u - v;
+        total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; w++) {
+            const auto s = (decltype(v))sh.sums[w];
+            if (w < wave) before += s;
+            total += s;
         }
-        if (live) sh.few.weight[rank] = w;
-    }
-    __syncthreads();
-    // weights before each rank: four waves' scans
-    unsigned long long by_rank = tid < n ? sh.few.weight[tid] : 0;
-    const unsigned long long upto = wave_upto(by_rank);
-    if ((tid & 63) == 63) sh.sums[tid >> 6] = upto;
-    __syncthreads();
-    uint64_t before = upto - by_rank;
-    for (uint32_t v = 0; v < tid >> 6; v++) before += sh.sums[v];
-    if (tid < n) sh.few.weight[tid] = before;
-    if (tid == 0) sh.found[0] = 0;
-    __syncthreads();
-    bool keep = live && w;
-    if (flags & ROW_K) {
-        keep = keep && rank < (uint32_t)r.k;
-        if (live && rank == (uint32_t)r.k) sh.found[0] = sh.few.weight[rank];  // (what top-k keeps)
-        else if (tid == 0 && n <= (uint32_t)r.k) sh.found[0] = ~0ull;
-    }
-    __syncthreads();
-    if (flags & ROW_P) {
-        if (flags & ROW_K) {
-            all = sh.found[0];
-            if (all == ~0ull) {
-                all = 0;
-                for (uint32_t v = 0; v < WAVES; v++) all += sh.sums[v];
-            }
+        return before;
+    };
+    {
+        uint32_t c[BINS], mine = 0, total;
+#pragma unroll
+        for (uint32_t j = 0; j < BINS; j++) mine += c[j] = sh.few.start[BINS * tid + j];
+        uint32_t before = upto(mine, total);
+#pragma unroll
+        for (uint32_t j = 0; j < BINS; j++) {
+            sh.few.start[BINS * tid + j] = before;
+            before += c[j];
         }
-        const uint64_t want = max((uint64_t)ceil(fmax((double)r.p, 0.0) * (double)all), (uint64_t)1);
-        keep = keep && sh.few.weight[rank] < want;
+        if (tid == 0) sh.few.start[SAMPLE_BINS] = n;
     }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++)
+        if (PER * tid + j < n) sh.few.token[sh.few.start[part[j]] + slot[j]] = (unsigned long long)order_of(x[j]) << 32 | (0xFFFFFFFFu - id[j]);
+    __syncthreads();
+    uint64_t w[PER];
+    weight.of(x, w);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+        if (PER * tid + j >= n) continue;
+        const unsigned long long mine = (unsigned long long)order_of(x[j]) << 32 | (0xFFFFFFFFu - id[j]);
+        const uint32_t from = sh.few.start[part[j]], to = sh.few.start[part[j] + 1];
+        rank[j] = from;
+        for (uint32_t i = from; i < to; i++) rank[j] += sh.few.token[i] > mine ? 1u : 0u;
+        sh.few.weight[rank[j]] = w[j];
+    }
+    __syncthreads();
+    // the weights before each rank
+    {
+        unsigned long long c[PER], mine = 0, total;
+#pragma unroll
+        for (uint32_t j = 0; j < PER; j++) mine += c[j] = PER * tid + j < n ? sh.few.weight[PER * tid + j] : 0;
+        unsigned long long before = upto(mine, total);
+#pragma unroll
+        for (uint32_t j = 0; j < PER; j++) {
+            if (PER * tid + j < n) sh.few.weight[PER * tid + j] = before;
+            before += c[j];
+        }
+        if (tid == 0) sh.few.weight[n] = total;
+    }
+    __syncthreads();
+    const uint32_t k = flags & ROW_K ? min((uint32_t)r.k, n) : n;
+    if (flags & ROW_K) all = sh.few.weight[k];
+    const uint64_t want = flags & ROW_P ? max((uint64_t)ceil(fmax((double)r.p, 0.0) * (double)all), (uint64_t)1) : ~0ull;
     const double least = r.least > 0.0f ? fmin((double)r.least, 1.0) * (double)(1ull << a.unit) : 0.0;
-    const unsigned long long kept = keep && (double)w >= least ? w : 0, to = wave_upto(kept);
-    __syncthreads();
-    if ((tid & 63) == 63) sh.sums[tid >> 6] = to;
-    __syncthreads();
-    uint64_t from = to - kept, total = 0;
-    for (uint32_t v = 0; v < WAVES; v++) {
-        if (v < tid >> 6) from += sh.sums[v];
-        total += sh.sums[v];
+    unsigned long long kept[PER], mine = 0, total;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+        kept[j] = 0;
+        if (PER * tid + j < n && rank[j] < k && sh.few.weight[rank[j]] < want && (double)w[j] >= least) kept[j] = w[j];
+        mine += kept[j];
     }
+    unsigned long long before = upto(mine, total);
     const uint64_t target = share_of(r.u, total);
-    if (from < target && from + kept >= target) {
-        a.next[row] = (int32_t)id;
-        if (a.logp) a.logp[row] = (float)log((double)w / (double)total);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; j++) {
+        if (before < target && before + kept[j] >= target) {
+            a.next[row] = (int32_t)id[j];
+            if (a.logp) a.logp[row] = (float)log((double)kept[j] / (double)total);
+        }
+        before += kept[j];
     }
 }
 
@@ -648,6 +714,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     __shared__ unsigned long long sums_s[WAVES][3];
     __shared__ uint32_t counts_s[WAVES][2];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slice = blockIdx.x / a.rows, at = blockIdx.x % a.rows, row = a.row0 + at;
+    float x[8];
+    load_eight<BF16>(a, row, slice * SAMPLE_SLICE + 8 * tid, x);
     const SampleRow info = a.row[at];
     const Rules r = rules_of(a, row);
     if (info.flags & (ROW_EMPTY | ROW_GREEDY | ROW_WHOLE)) return;
@@ -655,10 +723,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
     const float scale = step_scale(r.heat);
     const bool limits = info.flags & (ROW_K | ROW_P);
     const double least = r.least > 0.0f ? fmin((double)r.least, 1.0) * (double)(1ull << a.unit) : 0.0;
-    float x[8];
-    load_eight<BF16>(a, row, slice * SAMPLE_SLICE + 8 * tid, x);
     unsigned long long all = 0, above = 0, kept = 0;
-    uint32_t n_above = 0, named = 0, higher = 0;  // tokens of the thread among which the limits fall, and those above, a bit each
+    uint32_t named = 0, higher = 0;  // tokens of the thread among which the limits fall, and those above, a bit each
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float o = limits ? step_of(x[j], scale) : 0.0f;
@@ -674,41 +740,50 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
             all += w[j];
             if (higher >> j & 1) {
                 above += w[j];
-                n_above += w[j] ? 1 : 0;
                 kept += (double)w[j] >= least ? w[j] : 0;
             }
         }
     }
-    const uint32_t n = __popc(named), n_upto = wave_upto(n);
-    all = wave_sum(all);
-    above = wave_sum(above);
+    // (where those above are few, they are set apart with the others: a row that has few of both is done by their ranks)
+    if (!limits) higher = 0;
+    const uint32_t n = __popc(named), n_upto = wave_upto(n), both = __popc(named | higher), both_upto = wave_upto(both);
     kept = wave_sum(kept);
-    n_above = wave_sum(n_above);
+    if (limits) {
+        all = wave_sum(all);
+        above = wave_sum(above);
+    }
     if (lane == 63) {
         sums_s[wave][0] = all;
         sums_s[wave][1] = above;
         sums_s[wave][2] = kept;
-        counts_s[wave][0] = n_above;
+        counts_s[wave][0] = both_upto;
         counts_s[wave][1] = n_upto;
     }
     __syncthreads();
-    uint32_t to = n_upto - n;
-    for (uint32_t w = 0; w < wave; w++) to += counts_s[w][1];
+    uint32_t n_both = 0, n_named = 0, both_before = 0, named_before = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) {
+        if (w == wave) both_before = n_both, named_before = n_named;
+        n_both += counts_s[w][0];
+        n_named += counts_s[w][1];
+    }
+    const bool with = n_both - n_named <= SAMPLE_WITH;
+    const uint32_t set = with ? named | higher : named;
+    uint32_t to = with ? both_before + both_upto - both : named_before + n_upto - n;
     const size_t place = (size_t)at * a.slices + slice;
 #pragma unroll
     for (int j = 0; j < 8; j++)
-        if (named >> j & 1) {
+        if (set >> j & 1) {
             if (to < a.room) a.token[place * a.room + to] = (unsigned long long)order_of(x[j]) << 32 | (slice * SAMPLE_SLICE + 8 * tid + j);
             to++;
         }
     if (tid == 0) {
-        SampleSlice o{0, 0, 0, 0, 0};
+        SampleSlice o{0, 0, 0, n_both - n_named, with ? n_both : n_named};
+#pragma unroll
         for (uint32_t w = 0; w < WAVES; w++) {
             o.all += sums_s[w][0];
             o.above += sums_s[w][1];
             o.kept += sums_s[w][2];
-            o.n_above += counts_s[w][0];
-            o.n += counts_s[w][1];
         }
         a.slice[place] = o;
     }
@@ -771,11 +846,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
     const Weigher weight = weigher(a, r, info.top);
     uint64_t all = 0, above = 0;
     uint32_t n_above = 0, total = 0;
-    bool whole = WHOLE || (info.flags & ROW_WHOLE);
+    bool whole = WHOLE || (info.flags & ROW_WHOLE), with = false;  // (all tokens above the limits' steps are set apart as well)
     const bool limits = info.flags & (ROW_K | ROW_P);
     const unsigned long long* tokens = a.token + (size_t)at * a.slices * a.room;
     if (!whole) {  // what the slices have, together
-        bool over = false;
+        bool over = false, without = false;
         for (uint32_t s = tid; s < a.slices; s += SAMPLE_THREADS) {
             const SampleSlice p = a.slice[(size_t)at * a.slices + s];
             all += p.all;
@@ -784,8 +859,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
             sh.slice[s] = p.kept;
             sh.offset[s] = p.n;
             over = over || p.n > a.room;
+            without = without || p.n_above > SAMPLE_WITH;
         }
         whole = __syncthreads_or(over);
+        with = !__syncthreads_or(without);
         if (wave == 0) {  // the slices' tokens, one behind the other
             uint32_t from = 0;
             for (uint32_t s0 = 0; s0 < a.slices; s0 += 64) {
@@ -810,16 +887,19 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
             for (uint32_t i = lane; i < many; i += 64) held_s[from + i] = tokens[(size_t)s * a.room + i];
         }
         __syncthreads();
-        if ((info.flags & ROW_ALONE) && total <= SAMPLE_FEW) {
-            const unsigned long long t = tid < total ? held_s[tid] : 0;
-            if (tid < SAMPLE_FEW) sh.few.order[tid] = (uint32_t)(t >> 32);
-            __syncthreads();
-            draw_few(a, sh, row, r, weight, info.flags, total, all, (uint32_t)t, (uint32_t)(t >> 32));
+        if (limits && with && total <= SAMPLE_FEW) {
+            draw_few<BF16>(a, sh, row, r, weight, info.flags, held_s, total, all, info.low / step_scale(r.heat));
             return;
         }
     }
     const uint32_t pieces = (a.vocab + SAMPLE_SLICE - 1) / SAMPLE_SLICE, per = WHOLE ? (pieces + SAMPLE_SLICES - 1) / SAMPLE_SLICES * SAMPLE_SLICE : SAMPLE_SLICE;
     const uint32_t slices = (uint32_t)(((uint64_t)a.vocab + per - 1) / per);
+    // (tokens above the limits' steps that are set apart with them are known to be kept: their weights are in the slices' sums)
+    auto token = [&](unsigned long long t, bool here, float& x, uint32_t& id) {
+        x = of_order((uint32_t)(t >> 32));
+        id = (uint32_t)t;
+        if (!here || step_of(x, step_scale(r.heat)) > info.high) x = -__builtin_inff();
+    };
     // The tokens among which the limits fall: held here, where the second pass has left them, or the whole row where it is.
     auto each = [&](auto f) {
         float x[8];
@@ -837,9 +917,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const uint32_t k = i + j * SAMPLE_THREADS + tid;
-                    const unsigned long long t = held_s[min(k, total - 1)];
-                    x[j] = k < total ? of_order((uint32_t)(t >> 32)) : -__builtin_inff();
-                    id[j] = (uint32_t)t;
+                    token(held_s[min(k, total - 1)], k < total, x[j], id[j]);
                 }
                 f(x, id);
             }
@@ -850,12 +928,43 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const uint32_t k = i + j * 64 + lane;
-                        const unsigned long long t = tokens[(size_t)s * a.room + min(k, many - 1)];
-                        x[j] = k < many ? of_order((uint32_t)(t >> 32)) : -__builtin_inff();
-                        id[j] = (uint32_t)t;
+                        token(tokens[(size_t)s * a.room + min(k, many - 1)], k < many, x[j], id[j]);
                     }
                     f(x, id);
                 }
+            }
+        }
+    };
+    auto by_slices = [&](unsigned long long* sums, auto f) {
+        float x[4];
+        uint32_t id[4];
+        if (whole) {
+            for (uint32_t p = 0; p < 2 * pieces; p++) {  // (half of what each takes at a time)
+                const uint32_t i = p / 2 * SAMPLE_SLICE + 8 * tid;
+                float y[8];
+                load_eight<BF16>(a, row, i, y);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[j] = p & 1 ? y[4 + j] : y[j];
+                    id[j] = i + (p & 1) * 4 + j;
+                }
+                const unsigned long long v = wave_sum((unsigned long long)f(x, id));
+                if (lane == 0 && v) atomicAdd(&sums[p / 2 * SAMPLE_SLICE / per], v);
+            }
+        } else {
+            for (uint32_t s = wave; s < slices; s += WAVES) {
+                const uint32_t from = sh.offset[s], many = sh.offset[s + 1] - from;
+                unsigned long long v = 0;
+                for (uint32_t i = 0; i < many; i += 4 * 64) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t k = i + j * 64 + lane, at = min(k, many - 1);
+                        token(total <= SAMPLE_HELD ? held_s[from + at] : tokens[(size_t)s * a.room + at], k < many, x[j], id[j]);
+                    }
+                    v += f(x, id);
+                }
+                v = wave_sum(v);
+                if (lane == 0) sums[s] += v;
             }
         }
     };
@@ -882,7 +991,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
                 all = sum_of(sh, all);
             }
         }
-        if (draw<BF16>(a, sh, row, r, weight, flags, each, whole, slices, per, all, above, n_above, from_v, to_v) || whole) return;
+        if (draw<BF16>(a, sh, row, r, weight, flags, each, by_slices, whole, slices, per, all, above, n_above, from_v, to_v) || whole) return;
         whole = true;
     }
 }
@@ -896,7 +1005,7 @@ static hipError_t launch(SampleArgs a, const DecodeScratch& sc, hipStream_t s) {
     // As many rows at a time as the scratch holds, with room for 256 tokens of a slice at least.
     constexpr size_t LEAST = SAMPLE_SLICE / 16;
     const uint32_t rows = a.rows;
-    const size_t bytes = sc.partial_floats * 4, fixed = sizeof(SampleRow) + (size_t)a.slices * (SAMPLE_STEPS * 8 + sizeof(float) + sizeof(SampleSlice)) + 64;
+    const size_t bytes = sc.partial_floats * 4, fixed = sizeof(SampleRow) + (size_t)a.slices * (SAMPLE_STEPS * 4 + sizeof(float) + sizeof(SampleSlice)) + 64;
     uint32_t most = (uint32_t)(bytes / (fixed + a.slices * LEAST * 8));
     if (most > sc.ncounters / CTR_STRIDE) most = (uint32_t)(sc.ncounters / CTR_STRIDE);
     if (!most) return hipErrorInvalidValue;
@@ -909,7 +1018,7 @@ static hipError_t launch(SampleArgs a, const DecodeScratch& sc, hipStream_t s) {
         p += (n + 15) / 16 * 16;
         return q;
     };
-    a.step = reinterpret_cast<unsigned long long*>(take((size_t)most * a.slices * SAMPLE_STEPS * 8));
+    a.step = reinterpret_cast<uint32_t*>(take((size_t)most * a.slices * SAMPLE_STEPS * 4));
     a.slice = reinterpret_cast<SampleSlice*>(take((size_t)most * a.slices * sizeof(SampleSlice)));
     a.best = reinterpret_cast<float*>(take((size_t)most * a.slices * sizeof(float)));
     a.row = reinterpret_cast<SampleRow*>(take((size_t)most * sizeof(SampleRow)));

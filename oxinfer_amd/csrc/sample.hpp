@@ -31,7 +31,7 @@ struct SampleArgs {
     uint32_t unit;  // weights are whole numbers, 2^unit being the largest
     uint32_t slices, vec, row0;
     // scratch
-    unsigned long long* step;    // [rows][slices][SAMPLE_STEPS]: tokens << 48 | weights in 2^-32
+    uint32_t* step;              // [rows][slices][SAMPLE_STEPS]: numbers of tokens, or (f32) their weights
     float* best;                 // [rows][slices]
     SampleRow* row;              // [rows]
     SampleSlice* slice;          // [rows][slices]

@@ -430,7 +430,7 @@ int oxhip_dev_kv_summary_read(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const ox
 int oxhip_dev_kv_select(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, const void* q, size_t q_stride, size_t n_q, int dtype,
                         size_t count, size_t first, size_t last, int32_t* chosen, void* stream);
 /* oxhip_dev_attend over the spans alone that `chosen` [rows, n_kv, count] names for a row and key head (of those keys, what the rules let the row see). Numbers that are
- * negative, past the row's own span, or not above the one before them name nothing. */
+ * negative, past the row's own span, or not above the one before them name nothing; a span that comes again behind a lower number counts again. */
 int oxhip_dev_attend_selected(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const int32_t* chosen, size_t count, size_t span, const void* q, size_t q_stride,
                               size_t n_q, int dtype, float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
 

@@ -161,6 +161,8 @@ __device__ __forceinline__ void load_query(const void* q, size_t at, bool vec, f
 constexpr uint32_t PROMPT_ENTRIES = 128;
 // What the launches of one call have alike; whether the kernels with rules are to run.
 AttendArgs attend_args(const KvView& kv, const KvBatchView& b, const AttendCall& call, const DecodeScratch& sc, bool* rules);
+// The attention over chosen spans (a.chosen), a wave a row and key head: a.units of them.
+hipError_t launch_attend_rows(const AttendArgs& a, bool bf16, bool rules, hipStream_t s);
 hipError_t launch_attend_prompt(const AttendArgs& a, bool bf16, bool rules, hipStream_t s);
 
 }  // namespace oxhip

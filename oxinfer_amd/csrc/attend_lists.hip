@@ -41,12 +41,23 @@ hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const Sh
     return e != hipSuccess ? e : go<SHARED>(a, call.bf16, rules, grid, s);
 }
 
+constexpr uint64_t ROW_UNITS = 2048, ROW_ROWS = 32;
+
 hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const ChosenView& chosen, const AttendCall& call, const DecodeScratch& sc, hipStream_t s) {
     bool rules;
     AttendArgs a = attend_args(kv, b, call, sc, &rules);
     a.chosen = chosen.chosen;
     a.count = chosen.count;
     while ((1u << a.span_shift) < chosen.span_blocks) a.span_shift++;
+    // A wave a row and key head where these fill the chip and have a sequence's codes in common, so that they are bound by the L2 and by their own instructions
+    // (64 spans of 64 of a prompt of 16384, 8 key heads of 128 with 4 heads each, bf16: 256 rows 126 us, 145 with a workgroup a row and key head, 512 rows 226 and 272, 2048 833 and
+    // 1001; 128 rows 78 and 78). Rows of sequences of their own are bound by memory, and eight waves a list have more on its way (256 of them 236 and 209).
+    const uint64_t units = (uint64_t)b.rows * kv.n_kv;
+    if (a.g <= 8 && b.row_start && units >= ROW_UNITS && b.rows >= (uint64_t)b.n_seqs * ROW_ROWS) {
+        if (!kv_launch_fits(units + 64, 64)) return hipErrorInvalidValue;
+        a.units = (uint32_t)units;
+        return launch_attend_rows(a, call.bf16, rules, s);
+    }
     unsigned grid;
     const hipError_t e = spread(a, sc, false, std::min<uint64_t>((uint64_t)chosen.count << a.span_shift, (uint64_t)b.max_pages << kv.shift), 256 * split_places((int)kv.d / 32), &grid);
     return e != hipSuccess ? e : go<CHOSEN>(a, call.bf16, rules, grid, s);

@@ -242,7 +242,7 @@ int oxhip_dev_kv_select(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_b
     if (q_stride && q_stride < width) return refuse(who, "rows lie at least a row apart");
     if (!count || count > SELECT_SPANS || first > count || last > count - first) return refuse(who, "1 to 16384 spans of a row, the first and the last ones among them");
     if (b->max_pages > SELECT_SPANS / (kv->page_tokens / sum->span)) return refuse(who, "a sequence's table has room for 16384 spans at most");
-    if (!kv_launch_fits((uint64_t)b->rows * kv->n_kv, 512)) return refuse(who, "more rows or heads than one launch takes");
+    if (!kv_launch_fits((b->row_start ? kv_places(b->rows, b->n_seqs, 1, 1) : b->n_seqs) * kv->n_kv, 1024)) return refuse(who, "more rows, sequences or heads than one launch takes");
     if (!c) return refuse(who, "null context");
     if (!b->rows) return 1;
     a.code = sum->code;

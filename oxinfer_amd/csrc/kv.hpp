@@ -31,6 +31,7 @@ struct SelectArgs {
     size_t q_stride;
     int32_t* out;  // [rows][n_kv][count]
     uint32_t span_shift, g, count, first, last;
+    uint32_t rows_of, places, spans;  // rows of a sequence that a workgroup takes; workgroups of a key head; spans that a sequence's table may hold
 };
 // The spans that a sequence's table may hold: their scores lie in LDS.
 constexpr uint32_t SELECT_SPANS = 16384;

@@ -25,12 +25,12 @@ class Shared(kv_ref.World):
         return [np.concatenate([a[:common], b[common:]])[: self.lens[s]] for a, b in zip(super().sequence(leader), own)]
 
 
-def named(chosen, pos, span):
-    """The tokens that a list of spans names for a row at `pos`."""
-    sees, before = np.zeros(pos + 1, bool), -1
+def named(chosen, pos, span, length=None):
+    """How often a list of spans names each token (of `length`) for a row at `pos`."""
+    sees, before = np.zeros(pos + 1 if length is None else length, int), -1
     for c in chosen.tolist():
-        if before < c <= pos // span:
-            sees[c * span : (c + 1) * span] = True
+        if before < c and 0 <= c <= pos // span:
+            sees[c * span : (c + 1) * span] += 1
         before = c
     return sees
 
@@ -46,19 +46,20 @@ def attend_selected(w, q, g, scale, chosen, span, half=False, **rules):
             if pos < 0:
                 continue
             for h in range(w.n_kv * g):
-                sees = named(chosen[r, h // g], pos, span)
-                j = np.arange(pos + 1)
-                rule = np.ones(pos + 1, bool)
+                sees = named(chosen[r, h // g], pos, span, len(k))
+                j = np.arange(len(k))
+                rule = j <= pos
                 if rules.get("window"):
                     rule &= j > pos - rules["window"]
                 if rules.get("first") is not None:
                     rule &= j >= rules["first"][r]
                 if rules.get("prefix") is not None:
                     rule |= j < rules["prefix"][s]
-                sees &= rule
+                often = sees[sees * rule > 0]
+                sees = sees * rule > 0
                 if not sees.any():
                     continue
-                x, kh, vh = q[r, h], k[: pos + 1, h // g][sees], v[: pos + 1, h // g][sees]
+                x, kh, vh = q[r, h], k[:, h // g][sees], v[:, h // g][sees]
                 score = scale * (kh @ x)
                 # (the terms of kv_ref.attend's bound)
                 ds = (w.d + 8) * u * abs(scale) * (np.abs(kh) @ np.abs(x))
@@ -72,7 +73,7 @@ def attend_selected(w, q, g, scale, chosen, span, half=False, **rules):
                     score = score - bias
                     ds = ds + 4 * u * np.abs(bias)
                 ds = ds + 8 * u * (np.abs(score) + 84)
-                p = np.exp(score - score.max())
+                p = often * np.exp(score - score.max())
                 o = p @ vh / p.sum()
                 rel = 2 * ds + (2.0**-11 if half else 2.0**-21) + (64 + len(p) / 128) * 2 * u
                 e = (p * rel) @ np.abs(vh) / p.sum() + (p * rel).sum() / p.sum() * np.abs(o) + 2.0**-36 * len(p) * np.abs(vh).max() / p.sum()

@@ -278,6 +278,82 @@ def test_attention_with_masks_caps_and_biases(be, rules, dtype):
     check(be, w, 3, 32, lists(w, 6, 32, rng, full=True), dtype, loud=4.0, **rules)
 
 
+# ---- batches of many rows of a sequence, a wave a row and key head: 32 rows of a sequence and 2048 of these waves at least ----
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", range(32, 257, 32))
+def test_many_rows_of_every_head_size(be, d, dtype):
+    w = kv_ref.World([1397, 365], 32, d, page=64, seed=d, n=[60, 7])
+    check(be, w, 2, 64, lists(w, 7, 64, np.random.default_rng(d)), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("g", [1, 3, 4, 5, 8, 9])
+def test_many_rows_of_groups_of_heads(be, g, dtype):
+    w = kv_ref.World([470, 833, 64], 32, 64, page=32, seed=g, n=[60, 35, 5])
+    check(be, w, g, 32, lists(w, 9, 32, np.random.default_rng(g)), dtype, strided=True)
+
+
+@pytest.mark.parametrize("span,page,count", [(32, 32, 1), (32, 256, 2), (32, 64, 65), (64, 64, 33), (128, 256, 16), (1024, 1024, 3), (32, 32, 130)])
+def test_many_rows_of_spans_and_pages(be, span, page, count):
+    """Lists that end at, before and behind each set's turn and each 64 blocks; rows before the first token, rows behind the last sequence."""
+    w = kv_ref.World([5000, 31, 1025], 24, 64, page=page, seed=span, n=[60, 40, 6])
+    check(be, w, 2, span, lists(w, count, span, np.random.default_rng(count), full=True), ragged=True)
+    w = kv_ref.World([3000], 32, 32, page=page, seed=span, n=[64])
+    check(be, w, 5, span, lists(w, count, span, np.random.default_rng(count)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("g", [3, 6])
+@pytest.mark.parametrize("rules", RULES, ids=str)
+def test_many_rows_with_masks_caps_and_biases(be, rules, g, dtype):
+    rules = dict(rules)
+    rng = np.random.default_rng(8)
+    w = kv_ref.World([190, 350], 32, 64, page=32, seed=9, n=[46, 20])
+    if rules.get("slopes"):
+        rules["slopes"] = np.exp2(-8 * np.arange(1, 32 * g + 1) / (32 * g)).astype(np.float32)
+    if "prefix" in rules:
+        rules["prefix"] = np.array(rules["prefix"][:2], np.int32)
+    if "first" in rules:
+        rules["first"] = (positions(w) * rng.integers(0, 5, w.rows) // 4).astype(np.int32)
+    check(be, w, g, 32, lists(w, 6, 32, rng, full=True), dtype, loud=4.0, **rules)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 30.0])
+def test_many_rows_of_other_scales(be, scale):
+    w = kv_ref.World([400, 300], 32, 64, page=64, seed=3, n=[60, 5])
+    check(be, w, 3, 32, lists(w, 6, 32, np.random.default_rng(1)), scale=scale)
+
+
+def test_many_rows_of_scales_at_their_ends(be):
+    """Scales of zero, the least and the largest, in blocks of one set and of several."""
+    w = kv_ref.World([800, 700], 32, 64, page=32, seed=6, n=[60, 9])
+    for page, value in ((0, 0.0), (1, 2.0**-60), (2, 0.0), (3, 2.0**60), (4, 0.0), (9, 2.0**59), (10, 0.0)):
+        w.vs[w.table[:, page]] = value
+    w.ks[w.table[0, 3]] = w.ks[w.table[1, 4]] = 0.0
+    check(be, w, 3, 32, lists(w, 14, 32, np.random.default_rng(2), full=True))
+
+
+def test_many_rows_with_pages_outside_the_cache_and_lists_that_are_not_sound(be):
+    from oxinfer_amd import hip
+    w = kv_ref.World([300, 280], 32, 64, page=32, seed=3, n=[60, 30])
+    chosen = np.random.default_rng(2).integers(-3, 12, (w.rows, 32, 6)).astype(np.int32)
+    check(be, w, 2, 32, chosen)
+    q = torch.randn(w.rows, 64 * 64, device="cuda")
+    cache, batch = w.tensors(hip)
+    up = torch.from_numpy(chosen).cuda()
+    want = be.attend_selected(cache, batch, q, up, 32).view(w.rows, 32, 2, 64)
+    seq, pos = np.repeat([0, 1], w.n), positions(w)
+    for s, entry in ((0, 2), (1, 0), (1, 8)):
+        pages = batch.pages.clone()
+        pages[s, entry] = -1
+        got = be.attend_selected(cache, hip.KvBatch(batch.kv_len, pages, rows=w.rows, row_start=batch.row_start), q, up, 32).view(w.rows, 32, 2, 64)
+        sees = np.array([[seq[r] == s and lists_ref.named(chosen[r, h], int(pos[r]), 32)[entry * 32 : entry * 32 + 32].any() for h in range(32)] for r in range(w.rows)])
+        sees = torch.from_numpy(sees).cuda()
+        assert sees.any() and got[sees].isnan().all() and torch.equal(got[~sees], want[~sees])
+
+
 def test_lists_that_are_not_sound(be):
     """Numbers that do not ascend, come twice, are negative or lie past the row's own span name nothing; a row without any gives zeros."""
     w = kv_ref.World([200, 200, 200, 200, 200], 1, 64, page=32, seed=3)

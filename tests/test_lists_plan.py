@@ -122,7 +122,7 @@ def test_calls_of_more_than_one_launch_takes(lib):  # noqa: F811
         return said(lib, calls(lib, hip, *s)[which]())
 
     for good, bad in ((ask(batch(8 * m, 32 * m - 8, True), 0), ask(batch(8 * m, 32 * m, True), 0)), (ask(batch(8 * m - 1), 1), ask(batch(8 * m), 1)), (ask(batch(m, 32 * m, True), 1), ask(batch(8 * m, 5, True), 1)),
-                      (ask(batch(16 * m), 2), ask(batch(16 * m, d=128), 2)), (ask(batch(4 * m - 1), 3), ask(batch(4 * m), 3)), (ask(batch(4 * m - 1), 4), ask(batch(4 * m), 4))):
+                      (ask(batch(16 * m), 2), ask(batch(16 * m, d=128), 2)), (ask(batch(2 * m - 1), 3), ask(batch(2 * m), 3)), (ask(batch(m, m - 1, True), 3), ask(batch(m, m, True), 3)), (ask(batch(4 * m - 1), 4), ask(batch(4 * m), 4))):
         assert "null context" in good and "one launch" in bad, (good, bad)
 
 

@@ -249,7 +249,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES, KD <= 4 ? 2 : 1) void attend_rows_k
             if (b + 1 < SLOTS) request(a.kv.v, wheres[b + 1 < SLOTS ? b + 1 : b], vq[(b + 1) & 1]);
             else request(a.kv.k, where_of(i + SLOTS), kq[0]);  // (past the last block: some block, or the cache's first)
             const half8 nothing = {0, 0, 0, 0, 0, 0, 0, 0};
-            const half8 wh = slot == (uint32_t)b ? ph : nothing, wl = slot == (uint32_t)b ? pl : nothing;
+            const half8 wh = slot == (uint32_t)b ? ph : nothing;
+            half8 wl;
+            if constexpr (F32) wl = slot == (uint32_t)b ? pl : nothing;
 #pragma unroll
             for (int c = 0; c < KD; c++) {
                 const uint4 u = vq[b & 1][c];

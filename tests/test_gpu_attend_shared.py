@@ -234,6 +234,211 @@ def test_unsound_numbers_stay_inside_the_arrays(be):
         assert torch.equal(be.attend_shared(cache, batch, shared, q)[:6], want)
 
 
+# ---- groups of many entries, in tables with room for thousands of tokens: several tiles a group, several parts a tile ----
+
+
+def broad(w):
+    """w with tables for 8192 tokens at least, no page of the cache in what is added."""
+    add = max(0, 8192 // w.page - w.table.shape[1])
+    w.table = np.concatenate([w.table, np.full((len(w.lens), add), w.n_pages, np.int32)], 1)
+    return w
+
+
+def crowd(n_seqs, common, *args, n=None, starts=None, seed=0, **kwargs):
+    rng = np.random.default_rng(seed)
+    starts, common = ([0, n_seqs] if starts is None else starts), np.atleast_1d(common)
+    least = np.zeros(n_seqs, int)
+    for i, c in enumerate(common):
+        least[starts[i] : starts[i + 1]] = c
+    lens = least + rng.integers(0, 70, n_seqs) + (1 if n is None else np.asarray(n))
+    return broad(Shared(lens, starts, common, *args, n=n, seed=seed, **kwargs))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", range(32, 257, 32))
+def test_many_entries_of_head_sizes(be, d, dtype):
+    check(be, crowd(37, 360, 2, d, page=64, seed=d), 4, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("g", [1, 2, 3, 5, 7, 8, 12, 16, 17, 33])
+def test_many_entries_of_groups_of_heads(be, g, dtype):
+    n = 130 // g + 3
+    check(be, crowd(n, 67, 3, 64, page=32, seed=g), g, dtype)
+    check(be, crowd(n, 130, 1, 64, page=32, seed=g, n=np.random.default_rng(g).integers(1, 4, n)), g, dtype)
+
+
+@pytest.mark.parametrize("common", [0, 1, 31, 32, 33, 64, 511, 512, 513, 1300])
+def test_many_entries_and_lengths_of_the_prefix(be, common):
+    check(be, crowd(33, common, 1, 64, page=128, seed=common), 4)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_entries_of_several_groups(be, dtype):
+    """Groups that end inside a tile and between tiles, groups of one sequence or without shared tokens, sequences of no group."""
+    for starts, common in (([0, 20, 70, 101], [50, 90, 33]), ([3, 4, 9, 90], [64, 0, 70]), ([0, 64, 96], [100, 40]), ([0, 1, 2, 3, 101], [9, 9, 70, 69])):
+        check(be, crowd(101, common, 2, 64, page=32, seed=4, starts=starts), 4, dtype)
+        n = np.random.default_rng(len(starts)).integers(0, 9, 101)
+        check(be, crowd(101, common, 1, 96, page=64, seed=4, starts=starts, n=n), 1 if dtype == "f32" else 3, dtype, ragged=True)
+
+
+def test_many_entries_of_groups_of_a_row(be):
+    """Many groups of a row each, beside a group of many sequences."""
+    starts = [*range(64), 200, 9000]
+    check(be, broad(Shared(60 + np.arange(200), starts, [40 + i % 20 for i in range(64)] + [3], 1, 32, page=32, seed=5)), 50)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rules", RULES, ids=str)
+@pytest.mark.parametrize("n", [1, 3], ids=["one", "many"])
+def test_many_entries_with_masks_caps_and_biases(be, rules, n, dtype):
+    rules = dict(rules)
+    rng = np.random.default_rng(8)
+    w = crowd(60, [101, 75], 2, 64, page=32, seed=9, starts=[0, 36, 60], n=None if n == 1 else rng.integers(0, 7, 60))
+    g = 5
+    if rules.get("slopes"):
+        rules["slopes"] = np.exp2(-np.arange(1, 11)).astype(np.float32)
+    if "prefix" in rules:
+        rules["prefix"] = np.tile(np.array(rules["prefix"], np.int32), 12)
+    pos = positions(w)
+    if rules.get("first") == "docs":
+        rules["first"] = (pos * rng.integers(0, 5, w.rows) // 4).astype(np.int32)
+    elif rules.get("first") == "none":
+        rules["first"] = np.where(np.arange(w.rows) % 2, 0, np.where(np.arange(w.rows) % 4, pos + 1, 2**31 - 1)).astype(np.int32)
+    check(be, w, g, dtype, loud=4.0, **rules)
+
+
+def test_many_entries_and_more_rows_than_tokens(be):
+    n = [4, 7, 2, 60, 70]
+    got = check(be, broad(Shared([40, 3, 0, 90, 65], [0, 5], [2], 2, 64, seed=1, n=n)), 2, ragged=True)
+    assert (got[4:8] == 0).all() and (got[11:13] == 0).all() and (got[73:78] == 0).all()
+
+
+def test_many_entries_of_a_long_prefix(be):
+    """More than 64 blocks of a wave."""
+    w = broad(Shared([40100, 40040, 40037, 40020], [0, 4], [40003], 16, 32, page=256, seed=3, n=[20, 16, 12, 16]))
+    from oxinfer_amd import hip
+    cache, batch, shared = handles(w, hip)
+    for dtype, half in ((torch.float32, False), (torch.bfloat16, True)):
+        q = (2 * torch.randn(w.rows, 128 * 32, device="cuda")).to(dtype)
+        heads = [0, 60, 127]
+        want, tol = kv_ref.attend(w, q.double().cpu().numpy().reshape(w.rows, 128, 32), 8, 32**-0.5, heads=heads, half=half)
+        off = np.abs(be.attend_shared(cache, batch, shared, q).double().cpu().numpy().reshape(want.shape) - want)[:, heads]
+        assert (off <= tol[:, heads]).all(), f"{np.max(off / np.maximum(tol[:, heads], 1e-300)):.2f} times the bound"
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 4.0])
+def test_many_entries_and_scales(be, scale):
+    check(be, crowd(33, 90, 2, 64, seed=2), 4, scale=scale, window=30)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_entries_with_strides_and_addresses(be, dtype):
+    for n in (None, [4] * 44):
+        w = crowd(44, 50, 2, 96, seed=3, n=n)
+        check(be, w, 3, dtype, strided=True)
+        check(be, w, 3, dtype, strided=True, odd=True)
+
+
+@pytest.mark.parametrize("n", [1, 5])
+def test_many_entries_with_scales_of_zero_and_values_far_apart(be, n):
+    w = broad(Shared([190] + [175 + i for i in range(47)], [0, 48], [160], 2, 64, page=32, seed=6, n=[n] * 48))
+    for s, page, value in ((0, 0, 0.0), (0, 1, 2.0**60), (0, 2, 2.0**-60), (0, 4, 0.0), (1, 5, 0.0), (2, 5, 2.0**-60), (3, 5, 2.0**60)):
+        w.vs[w.table[s, page]] = value
+    w.ks[w.table[0, 3]] = w.ks[w.table[4, 5]] = 0.0
+    check(be, w, 3)
+
+
+def test_many_entries_with_pages_outside_the_cache(be):
+    from oxinfer_amd import hip
+    n = np.array([2] * 40)
+    w = broad(Shared(140 + np.arange(40), [0, 30, 40], [97, 20], 2, 64, page=32, seed=3, n=n))
+    q = torch.randn(w.rows, 16 * 64, device="cuda")
+    cache, batch, shared = handles(w, hip)
+    want = be.attend_shared(cache, batch, shared, q, window=60)
+    assert want.isfinite().all()
+    pos, seq = positions(w), np.repeat(np.arange(40), 2)
+    for s, entry, sees in ((0, 2, (seq < 30) & (pos - 59 <= 95)), (1, 3, (seq == 1) & (pos >= 97)), (0, 3, (seq < 30) & (pos >= 96) & (pos - 59 <= np.where(seq == 0, 127, 96))), (30, 0, (seq >= 30) & (pos - 59 <= np.where(seq == 30, 31, 19))), (5, 0, pos < 0)):
+        pages = batch.pages.clone()
+        pages[s, entry] = w.n_pages
+        got = be.attend_shared(cache, hip.KvBatch(batch.kv_len, pages, rows=w.rows, row_start=batch.row_start), shared, q, window=60)
+        assert got[torch.from_numpy(sees).cuda()].isnan().all()
+        assert torch.equal(got[torch.from_numpy(~sees).cuda()], want[torch.from_numpy(~sees).cuda()]), (s, entry)
+
+
+def test_many_entries_and_queries_that_are_no_numbers(be):
+    from oxinfer_amd import hip
+    w = crowd(40, 70, 2, 64, seed=6)
+    q = torch.randn(40, 2 * 4 * 64, device="cuda")
+    cache, batch, shared = handles(w, hip)
+    want = be.attend_shared(cache, batch, shared, q)
+    bad = q.clone()
+    bad[1, 70] = float("nan")
+    bad[33, 5] = float("inf")
+    got = be.attend_shared(cache, batch, shared, bad)
+    same = torch.ones(40, 8, dtype=torch.bool)
+    same[1, 1] = same[33, 0] = False
+    assert torch.equal(got.view(40, 8, 64)[same], want.view(40, 8, 64)[same])
+    assert got.view(40, 8, 64)[1, 1].isnan().all() and got.view(40, 8, 64)[33, 0].isnan().all()
+
+
+def test_many_entries_and_unsound_numbers(be):
+    from oxinfer_amd import hip
+    w = broad(Shared([64, 64, 64], [0, 3], [40], 1, 64, seed=3, wild=False, n=[20, 10, 30]))
+    cache, batch, shared = handles(w, hip, True)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.randn(62, 5 * 64, device="cuda")
+    out = torch.full((70, 5 * 64), 7.0, device="cuda")
+    want = be.attend_shared(cache, batch, shared, q)[:60].clone()
+    zeros = torch.zeros_like(batch.pages)
+    big = 2**31 - 1
+    for lens, start, groups, common in (((big, 64, -5), (0, 20, 30, 60), (0, 3), (40,)), ((64, 64, 64), (0, 20, 30, 9000), (0, 3), (40,)), ((64, 64, 64), (-7, 20, 30, 60), (0, 3), (40,)), ((64, 64, 64), (60, 30, 20, 0), (0, 3), (40,)),
+                                        ((64, 64, 64), (0, 0, 0, 0), (0, 3), (40,)), ((64, 64, 64), (0, 20, 30, 60), (-4, 99), (big,)), ((64, 64, 64), (0, 20, 30, 60), (3, 0), (big,)), ((64, 3, 64), (0, 20, 30, 60), (1, 3), (big,)),
+                                        ((64, 64, 64), (0, 20, 30, 60), (0, 3), (-(2**31),)), ((0, 0, 0), (0, 20, 30, 60), (0, 3), (64,))):
+        b = hip.KvBatch(i32(*lens), zeros, rows=60, row_start=i32(*start))
+        be.attend_shared(cache, b, hip.KvShared(i32(*groups), i32(*common)), q[:60], out=out[4:64])
+        torch.cuda.synchronize()
+        assert (out[:4] == 7).all() and (out[64:] == 7).all()
+        assert torch.equal(be.attend_shared(cache, batch, shared, q)[:60], want)
+
+
+def test_many_entries_give_the_same_bits_every_time(be):
+    from oxinfer_amd import hip
+    w = crowd(40, 6000, 2, 128, page=64, seed=3)
+    cache, batch, shared = handles(w, hip)
+    q = torch.randn(40, 8 * 128, device="cuda")
+    want = be.attend_shared(cache, batch, shared, q).clone()
+    for _ in range(20):
+        assert torch.equal(be.attend_shared(cache, batch, shared, q), want)
+
+
+def test_many_entries_in_a_recorded_plan(be):
+    """The lengths and the shared tokens are the device's at each replay, down to none; eager calls on another stream run beside it."""
+    from oxinfer_amd import hip
+    w = crowd(40, 5000, 2, 128, page=64, seed=3)
+    cache, batch, shared = handles(w, hip)
+    q, out = torch.randn(40, 8 * 128, device="cuda"), torch.zeros(40, 8 * 128, device="cuda")
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        be.attend_shared(cache, batch, shared, q, out=out)
+        stream.synchronize()
+        plan = be.plan_record(lambda: be.attend_shared(cache, batch, shared, q, out=out))
+        full = batch.kv_len.clone()
+        for common in (5000, 37, 0, 5000, 4097):
+            shared.common.fill_(common)
+            batch.kv_len.copy_(torch.minimum(full, torch.full_like(full, max(common, 1))) if common < 5000 else full)
+            q.normal_()
+            out.fill_(7)
+            stream.synchronize()
+            plan.replay()
+            with torch.cuda.stream(other):
+                want = be.attend_shared(cache, batch, shared, q)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), common
+    del plan
+
+
 def test_tables_that_name_the_shared_pages_fit_both_calls(be):
     """As appending sequences have them: whole shared pages in all tables. The results are attend's within both calls' bounds."""
     from oxinfer_amd import hip

@@ -485,6 +485,17 @@ def test_the_same_bits_on_any_stream(be):
             assert torch.equal(again, chosen) and torch.equal(got, want)
 
 
+def test_recording_without_scratch_is_refused(be):
+    from oxinfer_amd import hip
+    w = kv_ref.World([300, 310], 1, 64, seed=3)
+    cache, batch = w.tensors(hip)
+    chosen = torch.zeros((2, 1, 3), dtype=torch.int32, device="cuda")
+    q, out = torch.randn(2, 64, device="cuda"), torch.empty(2, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(RuntimeError, match="plan"):
+        be.plan_record(lambda: be.attend_selected(cache, batch, q, chosen, 32, out=out))
+
+
 def test_the_bindings_refusals(be):
     from oxinfer_amd import hip
     w = kv_ref.World([200, 200], 2, 64, page=64, seed=3)

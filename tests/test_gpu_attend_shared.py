@@ -530,6 +530,16 @@ def test_streams_and_threads(be):
     assert not wrong
 
 
+def test_recording_without_scratch_is_refused(be):
+    from oxinfer_amd import hip
+    w = Shared([300, 310], [0, 2], [200], 1, 64, seed=3)
+    cache, batch, shared = handles(w, hip)
+    q, out = torch.randn(2, 64, device="cuda"), torch.empty(2, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(RuntimeError, match="plan"):
+        be.plan_record(lambda: be.attend_shared(cache, batch, shared, q, out=out))
+
+
 def test_the_bindings_refusals(be):
     from oxinfer_amd import hip
     w = Shared([64, 50], [0, 2], [40], 2, 64, seed=3)

@@ -22,8 +22,9 @@ def rules_of(t, rng, names):
 
 
 def check(be, x, u, strided=False, **rules):
-    """x: a torch tensor of logits on the device. logp: weights are off by 2^-(62 - log2 vocab) of the largest at most, their sums by as many; then one
-    rounding to f32, and one of the logarithm's argument."""
+    """x: a torch tensor of logits on the device. logp: a weight is a whole number of 2^-unit of the largest (unit = 62 - log2 vocab, 46 at most), made of a series that is
+    off by 2^-42 of it; so a share is off by 2^-41 of itself and, for itself and for the sum, by vocab such units, which are more of a small share; then
+    one rounding to f32."""
     t, vocab = x.shape
     up = {k: torch.from_numpy(v).cuda() for k, v in rules.items()}
     got, logp = be.sample(x, torch.from_numpy(u).cuda(), **up)
@@ -32,10 +33,10 @@ def check(be, x, u, strided=False, **rules):
     logp = logp.double().cpu().numpy()
     live = want >= 0
     assert (logp[~live] == -np.inf).all()
-    bits = max(1, (vocab - 1).bit_length())
+    unit = min(46, 62 - (vocab - 1).bit_length())
     with np.errstate(over="ignore"):
-        share = 2.0 ** (bits - 61) * (1 + np.exp(-logs[live]))  # (the token's own weight may be small beside the largest)
-    assert (np.abs(logp[live] - logs[live]) <= 2.0**-24 * np.abs(logs[live]) + vocab * share + 2.0**-50).all()
+        share = 2.0**-unit * (1 + np.exp(-logs[live]))
+    assert (np.abs(logp[live] - logs[live]) <= 2.0**-24 * np.abs(logs[live]) + vocab * share + 2.0**-41).all()
     return got
 
 
@@ -203,6 +204,65 @@ def test_the_same_token_every_time(be):
             torch.cuda.current_stream().synchronize()
         assert torch.equal(a, b) and torch.equal(la, lb)
     assert be.sample(x, u, want_logp=False, **rules)[1] is None
+
+
+def test_a_vocabulary_past_a_million(be):
+    """More slices than sums are kept of."""
+    rng = np.random.default_rng(12)
+    x = torch.from_numpy(3 * rng.normal(size=(3, 1_100_003))).cuda().float()
+    for names in ((), ("top_k",), ("top_p",), NAMES):
+        check(be, x, rng.random(3).astype(np.float32), **rules_of(3, rng, names))
+    check(be, x.bfloat16(), rng.random(3).astype(np.float32), top_k=np.array([1_000_000, 5, 0], np.int32), top_p=np.array([0.999, 1.0, 0.5], np.float32))
+
+
+def test_more_rows_than_the_workspace_holds(be):
+    """What a row draws is no matter of the rows beside it, nor of how many of them a launch takes."""
+    rng = np.random.default_rng(13)
+    x = 3 * torch.randn(900, 151936, device="cuda").bfloat16()
+    u = torch.rand(900, device="cuda")
+    rules = {k: torch.from_numpy(v).cuda() for k, v in rules_of(900, rng, NAMES).items()}
+    got, logp = be.sample(x, u, **rules)
+    for lo, hi in ((0, 1), (1, 40), (40, 170), (500, 570), (895, 900)):
+        a, b = be.sample(x[lo:hi], u[lo:hi].contiguous(), **{k: v[lo:hi].contiguous() for k, v in rules.items()})
+        assert torch.equal(a, got[lo:hi]) and torch.equal(b, logp[lo:hi])
+    some = [0, 133, 450, 899]
+    want, _ = sample(x[some].double().cpu().numpy(), u[some].cpu().numpy(), **{k: v[some].cpu().numpy() for k, v in rules.items()})
+    assert got[some].tolist() == want.tolist()
+
+
+def test_recording_without_scratch_is_refused(be):
+    x, u = torch.randn(2, 300, device="cuda"), torch.rand(2, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(RuntimeError, match="plan"):
+        be.plan_record(lambda: be.sample(x, u))
+
+
+def test_threads_on_streams_of_their_own(be):
+    import threading
+    rng = np.random.default_rng(14)
+    made = []
+    for i in range(4):
+        x, u = 3 * torch.randn(3 + 5 * i, 30000 + 7000 * i, device="cuda"), torch.rand(3 + 5 * i, device="cuda")
+        rules = {k: torch.from_numpy(v).cuda() for k, v in rules_of(len(u), rng, NAMES).items()}
+        made.append((x, u, rules, be.sample(x, u, **rules)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def go(i):
+        x, u, rules, want = made[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = be.sample(x, u, **rules)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_the_bindings_refusals(be):

@@ -245,18 +245,25 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
         if (group < GROUPS) {
             uint32_t n[2] = {0, 0};
             float m[2] = {0.0f, 0.0f};
-            for (uint32_t s = group; s < a.slices; s += GROUPS) {
-                const float down = down_s[s];
-                const uint32_t* from = a.step + ((size_t)at * a.slices + s) * SAMPLE_STEPS;
+            constexpr uint32_t AHEAD = 8;  // (slices asked for at once: they lie in memory, past the L2)
+            for (uint32_t s0 = group; s0 < a.slices; s0 += GROUPS * AHEAD) {
+                uint32_t v[AHEAD][2];
+                auto slice_of = [&](uint32_t i) { return min(s0 + GROUPS * i, a.slices - 1); };
 #pragma unroll
-                for (uint32_t h = 0; h < 2; h++) {
-                    const uint32_t j = j0 + h * (SAMPLE_STEPS / 2);
-                    if (down <= (float)j) {
-                        const uint32_t v = get(&from[j - (uint32_t)down]);
-                        n[h] += v;
-                        m[h] += __uint_as_float(v) * best_s[s];
+                for (uint32_t i = 0; i < AHEAD; i++)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++) {
+                        const uint32_t j = j0 + h * (SAMPLE_STEPS / 2), s = slice_of(i);
+                        v[i][h] = get(a.step + ((size_t)at * a.slices + s) * SAMPLE_STEPS + (j - (uint32_t)fminf(down_s[s], (float)j)));
                     }
-                }
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; i++)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++) {
+                        const bool on = s0 + GROUPS * i < a.slices && down_s[slice_of(i)] <= (float)(j0 + h * (SAMPLE_STEPS / 2));
+                        n[h] += on ? v[i][h] : 0;
+                        m[h] += on ? __uint_as_float(v[i][h]) * best_s[slice_of(i)] : 0.0f;
+                    }
             }
 #pragma unroll
             for (uint32_t h = 0; h < 2; h++) sum_s[group][j0 + h * (SAMPLE_STEPS / 2)] = number ? n[h] : __float_as_uint(m[h]);

@@ -22,7 +22,7 @@ struct AttendArgs {
     int32_t power;     // the call's scale's
     uint32_t g, window, cols, vec, quantum, many, least, prompt;  // cols: entries of a tile that may be in use; vec: q by 16 bytes, out by 16 bytes
     // of a shared prefix, and of chosen spans (attend_lists.hip): tiles x key heads, parts of one at most
-    uint32_t units, parts;
+    uint32_t units, parts, tile_rows;  // (rows of the batch that a tile has)
     const int32_t *group_start, *common;
     uint32_t n_groups;
     const int32_t* chosen;

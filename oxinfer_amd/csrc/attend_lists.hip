@@ -12,8 +12,8 @@ namespace oxhip {
 // How many tiles a batch has, and parts of each: `target` workgroups in all, where lists of `blocks` blocks at most have parts of a.least blocks for them.
 static hipError_t spread(AttendArgs& a, const DecodeScratch& sc, bool several, uint64_t blocks, uint32_t target, unsigned* grid) {
     const uint64_t units = kv_row_tiles(a.b.rows, a.g, several) * a.kv.n_kv;
-    a.cols = several ? 16u : std::min(16u, a.g);
-    a.least = a.kv.d > 128 ? KV_LEAST / 2 : KV_LEAST;
+    a.tile_rows = several && a.g < 16 ? 16 / a.g : 1;
+    a.cols = std::min(16u, a.tile_rows * a.g);
     const uint64_t room = std::min<uint64_t>(sc.partial_floats / ((uint64_t)a.cols * (a.kv.d + 2)), sc.ncounters / CTR_STRIDE);  // parts that the scratch holds
     uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>((target + units - 1) / units, (blocks + a.least - 1) / a.least));
     parts = std::min<uint64_t>(parts, MOST_SPLITS);
@@ -33,11 +33,16 @@ static hipError_t go(const AttendArgs& a, bool bf16, bool rules, unsigned grid, 
 hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const SharedView& shared, const AttendCall& call, const DecodeScratch& sc, hipStream_t s) {
     bool rules;
     AttendArgs a = attend_args(kv, b, call, sc, &rules);
+    a.least = kv.d > 128 ? KV_LEAST / 2 : KV_LEAST;
     a.group_start = shared.group_start;
     a.common = shared.common;
     a.n_groups = shared.n_groups;
     unsigned grid;
-    const hipError_t e = spread(a, sc, true, (uint64_t)b.max_pages << kv.shift, 256 * split_places((int)kv.d / 32), &grid);
+    // Rows share what they read where there is more of it than the chip takes at once. Fewer have tiles of their own, whose lists are shorter and whose workgroups have fewer entries
+    // to join (8 key heads of 128, 4 heads each, f32: 4 sequences behind 700 tokens 11.1 us, 14.1 of four rows a tile; 32 of them 11.1 and 14.3; 8 behind 3000 tokens 16.2 and 20.4; and from the
+    // border on 64 behind 700 tokens 16.2 and 14.5; 16 behind 3000 21.7 and 20.6; 16 behind 12000 43.0 and 27.7).
+    const uint64_t blocks = (uint64_t)b.max_pages << kv.shift, alone = kv_row_tiles(b.rows, a.g, false) * kv.n_kv * ((blocks + a.least - 1) / a.least);
+    const hipError_t e = spread(a, sc, alone > 256, blocks, 256 * split_places((int)kv.d / 32), &grid);
     return e != hipSuccess ? e : go<SHARED>(a, call.bf16, rules, grid, s);
 }
 
@@ -46,6 +51,7 @@ constexpr uint64_t ROW_UNITS = 2048, ROW_ROWS = 32;
 hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const ChosenView& chosen, const AttendCall& call, const DecodeScratch& sc, hipStream_t s) {
     bool rules;
     AttendArgs a = attend_args(kv, b, call, sc, &rules);
+    a.least = kv.d > 128 ? KV_LEAST / 2 : KV_LEAST;
     a.chosen = chosen.chosen;
     a.count = chosen.count;
     while ((1u << a.span_shift) < chosen.span_blocks) a.span_shift++;

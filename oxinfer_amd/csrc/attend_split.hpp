@@ -128,13 +128,13 @@ __global__ __launch_bounds__(64 * split_waves(KD), 2 * split_places(KD)) void at
         i = live ? divide(e0 + n, g) : 0u;
         head = head0 + (live ? e0 + n - i * g : 0u);
     } else {
-        // Tiles of 16 / g rows of the batch (of one row, or 16 heads of its group, where g is larger or KIND is CHOSEN), each in a.parts parts at most.
+        // Tiles of a.tile_rows rows of the batch (of one row, or 16 heads of its group, where KIND is CHOSEN), each in a.parts parts at most.
         const uint32_t unit = blockIdx.x % a.units, heads = (g + 15) / 16;
         part = blockIdx.x / a.units;
         kvh = unit % a.kv.n_kv;
         const uint32_t tile = unit / a.kv.n_kv / heads, h16 = unit / a.kv.n_kv % heads;
         per = min(16u, g - 16 * h16);
-        const uint32_t rows_of = KIND == SHARED && g < 16 ? 16 / g : 1, row0 = tile * rows_of, rows = min(rows_of, a.b.rows - row0);
+        const uint32_t rows_of = KIND == SHARED ? a.tile_rows : 1, row0 = tile * rows_of, rows = min(rows_of, a.b.rows - row0);
         first_row = row0;
         e0 = 0;
         head0 = kvh * g + 16 * h16;

@@ -400,7 +400,7 @@ typedef struct {
     const int32_t* common;      /* [n_groups] */
     size_t n_groups;
 } oxhip_kv_shared;
-/* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence:
+/* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for up to 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence:
  * token j < common of a sequence lies in the page that the table of its group's FIRST sequence names, any other in its own table's. (Tables that all name
  * the shared pages, as appending sequences' do, fit both calls.) Everything else is oxhip_dev_attend's: rules, types, rows that see nothing, pages outside the cache;
  * rows that are no sequence's (also of row numbers that do not ascend) are left as they are. For batches of few rows a sequence: a prompt's are
@@ -471,7 +471,8 @@ int oxhip_dev_logits(oxhip_ctx* ctx, const void* logits, size_t stride, void* ou
  *   min_p: tokens with w >= min_p (above 1: as 1; 0 and below, or NaN: all).
  * next: the first id up to which what remains, in the order of the ids, weighs more than u times all of it, u in [0, 1) being the row's random number (what is
  * below 0 or NaN is 0, 1 and above gives the last one); -1 where nothing weighs. logp (or NULL): the logarithm of the token's share of what remains (-infinity for -1).
- * Weights are held as whole numbers of 2^-(62 - ceil(log2 vocab)) of the largest: their sums are exact, the same numbers draw the same token. */
+ * Weights are made in f64 and held as whole numbers of 2^-unit of the largest, unit = min(46, 62 - ceil(log2 vocab)): their sums are exact, the same numbers draw the
+ * same token. */
 typedef struct {
     const float* temperature;
     const int32_t* top_k;

@@ -6,6 +6,10 @@
 //   score(span) = max over the heads of the group of (sum of products of bytes) * s_span * s_query:
 // the sum is exact (int8 matrix instructions, 32-bit sums), the product of the three is formed in f64, so that which spans are chosen does not depend on the
 // order of any sum. A span costs d + 4 bytes to score, 1 / (2 span) of what its keys and values take.
+//
+// What has to be read is little (2.3 MB for a token over 131072, 14 for 64 sequences of up to 32768): the choice is bound by the chain from page numbers to scores to counts, and
+// takes 18 and 14 us of the 24 and 20 that the mean keys, reading back and the choice take together; 1018 rows over 20001 tokens 24 of 29, of which the instructions
+// that turn sums into scores and count them are the larger part.
 #include <algorithm>
 
 #include "kv.hpp"

@@ -10,6 +10,9 @@
 // look at to find the limit: a few by their ranks, many by counting them, in parts of a range that shrinks to one value. Then it knows every slice's sum of
 // what is kept, the slice that the draw falls into, and reads that one again. Tokens that do not fit the room set apart for them (steps that hold much of
 // the vocabulary), and rows whose weights no f32 sorts (infinite logits, temperatures at the ends of f32), are looked at where they are, by a whole row's passes.
+//
+// One row of 128256 f32 takes 21 us (7.8 + 4.9 + 8.8 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 50 (17.4 + 23.4 + 12.1: counting in LDS,
+// the f64 series, the third launch's chain). A workgroup of 512 threads with eight logits each: of 256 with sixteen they took 24.8 and 51.2.
 #include "sample.hpp"
 
 namespace oxhip {
@@ -133,7 +136,7 @@ __device__ __forceinline__ float step_of(float x, float scale) { return floorf(x
 
 // Weights: 2^y of y = (l - top) log2 e / temperature, in 2^-unit. 2^y by its Taylor series around the nearest whole number, 10 terms of |f ln 2| <= 0.35: the next is 2^-42
 // of it. An addition of 2^52 rounds to a whole number. Of eight logits at a time, so that the series' numbers are brought once for eight (one by one, with
-// a branch each, the second launch took 28 us of 64 rows of 151936, so 10).
+// a branch each, the second launch took 26.9 us of 64 rows of 151936, so 23.9).
 struct Weigher {
     double top, by;
     float top_f;
@@ -180,7 +183,8 @@ __device__ __forceinline__ Weigher weigher(const SampleArgs& a, const Rules& r, 
 template <bool BF16>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs a) {
     // Tokens are counted for top-k, their weights summed for top-p alone, as whole numbers of 2^-32 of the slice's largest. (Eight sums of a step side by side: tokens are
-    // many and steps few, and 64 lanes' additions to one place go one after the other. One sum of a step, in f32, took 60 us of 64 rows of 151936, sixteen 47, these 11.)
+    // many and steps few, and 64 lanes' additions to one place go one after the other. The launch takes 17 us of 64 rows of 151936, 9 where no row has a limit; with one sum of
+    // a step, in f32, 69, with sixteen 66: additions of floats in LDS are slow.)
     constexpr uint32_t COPIES = 8, GROUPS = 4;
     __shared__ __align__(16) unsigned long long step_s[SAMPLE_STEPS][COPIES];
     __shared__ uint32_t sum_s[GROUPS][SAMPLE_STEPS];

@@ -11,13 +11,15 @@
 // what is kept, the slice that the draw falls into, and reads that one again. Tokens that do not fit the room set apart for them (steps that hold much of
 // the vocabulary), and rows whose weights no f32 sorts (infinite logits, temperatures at the ends of f32), are looked at where they are, by a whole row's passes.
 //
-// One row of 128256 f32 takes 21 us (7.8 + 4.9 + 8.8 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 50 (17.4 + 23.4 + 12.1: counting in LDS,
+// One row of 128256 f32 takes 21 us (7.8 + 4.9 + 8.8 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 47 (17.4 + 23.4 + 8.7: counting in LDS,
 // the f64 series, the third launch's chain). A workgroup of 512 threads with eight logits each: of 256 with sixteen they took 24.8 and 51.2.
 #include "sample.hpp"
 
 namespace oxhip {
 
-constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_FEW = 2048, SAMPLE_HELD = 8192, SAMPLE_WITH = 256;
+// (Tokens held in LDS: as many as fit beside the rest. A CU then has one of the third launch's workgroups; with 8192 two of them may meet on one, and 64 rows of
+// 151936 took 49.1 us instead of 46.1.)
+constexpr uint32_t SAMPLE_BINS = 2048, SAMPLE_FEW = 2048, SAMPLE_HELD = 14336, SAMPLE_WITH = 256;
 constexpr uint32_t WAVES = SAMPLE_THREADS / 64;
 constexpr double LOG2E_D = 1.4426950408889634074;
 enum { ROW_GREEDY = 1, ROW_EMPTY = 2, ROW_WHOLE = 4, ROW_K = 8, ROW_P = 16, ROW_SUMS = 32 };

@@ -14,13 +14,18 @@
 
 namespace oxhip {
 
-// How many tiles a batch has, and parts of each: `target` workgroups in all, where lists of `blocks` blocks at most have parts of a.least blocks for them.
-static hipError_t spread(AttendArgs& a, const DecodeScratch& sc, bool several, uint64_t blocks, uint32_t target, unsigned* grid) {
+// How many tiles a batch has, and parts of each: `target` workgroups in all, where lists of `blocks` blocks at most (even: all as long) have parts of a.least blocks for them.
+static hipError_t spread(AttendArgs& a, const DecodeScratch& sc, bool several, bool even, uint64_t blocks, uint32_t target, unsigned* grid) {
     const uint64_t units = kv_row_tiles(a.b.rows, a.g, several) * a.kv.n_kv;
     a.tile_rows = several && a.g < 16 ? 16 / a.g : 1;
     a.cols = std::min(16u, a.tile_rows * a.g);
     const uint64_t room = std::min<uint64_t>(sc.partial_floats / ((uint64_t)a.cols * (a.kv.d + 2)), sc.ncounters / CTR_STRIDE);  // parts that the scratch holds
-    uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>((target + units - 1) / units, (blocks + a.least - 1) / a.least));
+    // A few workgroups more than the chip takes at once are a second round of them, so there are fewer then, and longer ones: of chosen spans, lists of one length, up to an eighth too many
+    // (24 rows of 4 key heads of d = 256: 288 workgroups on 256 places 47.1 us, 192 of them 36.0; but 640 on 512 58.2, 320 of them 61.9). Of shared prefixes lists differ, and some have
+    // fewer parts, so only where the fewer ones fill the chip all the same (288 34.9 us, 252 of them 27.8; 560 on 512 39.5, 480 of them 30.5; but 260 33.1, 208 of them 37.1).
+    const uint64_t wanted = (target + units - 1) / units, fewer = std::max<uint64_t>(1, target / units);
+    const bool round = even ? units * wanted * 8 <= target * 9 : units * fewer * 16 >= target * 15;
+    uint64_t parts = std::max<uint64_t>(1, std::min<uint64_t>(round ? fewer : wanted, (blocks + a.least - 1) / a.least));
     parts = std::min<uint64_t>(parts, MOST_SPLITS);
     if (units * parts > room) parts = std::max<uint64_t>(1, room / units);
     if (!kv_launch_fits(units * parts, 64 * split_waves((int)a.kv.d / 32))) return hipErrorInvalidValue;
@@ -47,7 +52,7 @@ hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const Sh
     // to join (8 key heads of 128, 4 heads each, f32: 4 sequences behind 700 tokens 11.1 us, 14.1 of four rows a tile; 32 of them 11.1 and 14.3; 8 behind 3000 tokens 16.2 and 20.4; and from the
     // border on 64 behind 700 tokens 16.2 and 14.5; 16 behind 3000 21.7 and 20.6; 16 behind 12000 43.0 and 27.7).
     const uint64_t blocks = (uint64_t)b.max_pages << kv.shift, alone = kv_row_tiles(b.rows, a.g, false) * kv.n_kv * ((blocks + a.least - 1) / a.least);
-    const hipError_t e = spread(a, sc, alone > 256, blocks, 256 * split_places((int)kv.d / 32), &grid);
+    const hipError_t e = spread(a, sc, alone > 256, false, blocks, 256 * split_places((int)kv.d / 32), &grid);
     return e != hipSuccess ? e : go<SHARED>(a, call.bf16, rules, grid, s);
 }
 
@@ -70,7 +75,7 @@ hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const 
         return launch_attend_rows(a, call.bf16, rules, s);
     }
     unsigned grid;
-    const hipError_t e = spread(a, sc, false, std::min<uint64_t>((uint64_t)chosen.count << a.span_shift, (uint64_t)b.max_pages << kv.shift), 256 * split_places((int)kv.d / 32), &grid);
+    const hipError_t e = spread(a, sc, false, true, std::min<uint64_t>((uint64_t)chosen.count << a.span_shift, (uint64_t)b.max_pages << kv.shift), 256 * split_places((int)kv.d / 32), &grid);
     return e != hipSuccess ? e : go<CHOSEN>(a, call.bf16, rules, grid, s);
 }
 

@@ -479,7 +479,8 @@ typedef struct {
     const float* top_p;
     const float* min_p;
 } oxhip_sample_rules;
-/* logits [rows, vocab] of `dtype`, rows `stride` values apart (0 = dense); a vocabulary has 2^31 - 4096 ids at most. */
+/* logits [rows, vocab] of `dtype`, rows `stride` values apart (0 = dense); a vocabulary has 2^31 - 4096 ids at most, a call fewer than 2^22 rows; scratch as
+ * oxhip_dev_attend's. */
 int oxhip_dev_sample(oxhip_ctx* ctx, const void* logits, size_t stride, size_t rows, size_t vocab, int dtype, const oxhip_sample_rules* rules, const float* u, int32_t* next,
                      float* logp, void* stream);
 

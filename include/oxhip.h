@@ -402,11 +402,17 @@ typedef struct {
 } oxhip_kv_shared;
 /* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for up to 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence:
  * token j < common of a sequence lies in the page that the table of its group's FIRST sequence names, any other in its own table's. (Tables that all name
- * the shared pages, as appending sequences' do, fit both calls.) Everything else is oxhip_dev_attend's: rules, types, rows that see nothing, pages outside the cache;
+ * the shared pages, as those of sequences that share whole pages may, fit both calls.) Everything else is oxhip_dev_attend's: rules, types, rows that see nothing, pages outside the cache;
  * rows that are no sequence's (also of row numbers that do not ascend) are left as they are. For batches of few rows a sequence: a prompt's are
  * oxhip_dev_attend's. */
 int oxhip_dev_attend_shared(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_shared* shared, const void* q, size_t q_stride, size_t n_q,
                             int dtype, float scale, const oxhip_attend_rules* rules, void* out, size_t out_stride, void* stream);
+/* oxhip_dev_kv_append of such a batch. The shared tokens are those that the group's first sequence holds: of another one's rows before `common` the queries are rotated,
+ * and nothing is stored. Its own tokens go into its own table's pages, and where they begin inside a block, that block begins with them, whatever scale and codes the cache has
+ * there. (oxhip_dev_kv_append takes the places before them in the block for tokens of the sequence, and its scale for theirs.) Shared and own tokens may lie in one
+ * block of the first sequence alone. */
+int oxhip_dev_kv_append_shared(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_shared* shared, const void* k, size_t k_stride, const void* v,
+                               size_t v_stride, const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream);
 
 /* Attention over the parts of a long cache that matter to a row: mean keys of its spans, a choice among them by a cheap score, the attention over the choice.
  * A span is `span` tokens (a power of two, 32 at least and a page at most); a summary holds, for every span of the cache and key head, the mean m of
@@ -416,7 +422,8 @@ typedef struct {
     float* scale; /* [n_pages, n_kv, page_tokens / span] */
     size_t span;
 } oxhip_kv_summary;
-/* The spans that the batch's rows touch (after their append), over the tokens that the cache then holds of them. Keys whose scale is under 2^-60 count as 0. A
+/* The spans that the batch's rows touch (after their append), over the tokens that the cache then holds of them, all in the sequence's own table (a span whose first tokens
+ * another sequence's page holds has no mean key). Keys whose scale is under 2^-60 count as 0. A
  * span of a page outside the cache is left out. A page that a call appended to stands once in one table, as for the append. */
 int oxhip_dev_kv_summarize(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, void* stream);
 /* The mean keys that the last `count` spans of every sequence stand for, out [n_seqs, count, n_kv, d] f32 at a multiple of 16 bytes; places before a sequence's

@@ -84,6 +84,14 @@ const char* check_attend(const oxhip_kv_cache* kv, const oxhip_kv_batch* b, cons
     call->bf16 = dtype == OXHIP_BF16;
     return nullptr;
 }
+// The groups of a batch whose sequences share first tokens: nullptr, or what is wrong.
+const char* check_shared(const oxhip_kv_shared* shared, SharedView* v) {
+    if (!shared || !shared->group_start || !shared->common) return "null argument";
+    if (!aligned(shared->group_start, 4) || !aligned(shared->common, 4)) return "an array of 4-byte values at an odd address";
+    if (!shared->n_groups || shared->n_groups > ((size_t)1 << 24)) return "1 to 2^24 groups";
+    *v = SharedView{shared->group_start, shared->common, (uint32_t)shared->n_groups};
+    return nullptr;
+}
 // A summary of a cache, or nullptr and what is wrong.
 const char* check_summary(const oxhip_kv_cache* kv, const oxhip_kv_summary* sum, uint32_t* span_shift) {
     if (!sum || !sum->code || !sum->scale) return "null argument";
@@ -94,13 +102,8 @@ const char* check_summary(const oxhip_kv_cache* kv, const oxhip_kv_summary* sum,
     return nullptr;
 }
 
-}  // namespace
-
-extern "C" {
-
-int oxhip_dev_kv_append(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
-                        size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream) {
-    const char* who = "kv_append";
+int append(const char* who, oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const SharedView& shared, const void* k, size_t k_stride, const void* v, size_t v_stride,
+           const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream) {
     KvView kvv;
     KvBatchView bv;
     if (!k || !v) return refuse(who, "null argument");
@@ -126,10 +129,27 @@ int oxhip_dev_kv_append(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_b
     if (!b->rows) return 1;
     OnDevice on(c->device);
     if (!on.ok) return refuse(who, "hipSetDevice failed");
-    HIP_TRY(launch_kv_append(kvv, bv, r, k, k_stride ? k_stride : width, v, v_stride ? v_stride : width, q, q_stride ? q_stride : q_width, q_out, q_out_stride ? q_out_stride : q_width,
+    HIP_TRY(launch_kv_append(kvv, bv, shared, r, k, k_stride ? k_stride : width, v, v_stride ? v_stride : width, q, q_stride ? q_stride : q_width, q_out, q_out_stride ? q_out_stride : q_width,
                              (uint32_t)n_q, dtype == OXHIP_BF16, static_cast<hipStream_t>(stream)),
             "kv_append launch");
     return 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+int oxhip_dev_kv_append(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
+                        size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream) {
+    return append("kv_append", c, kv, b, SharedView{}, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride, n_q, dtype, rope, stream);
+}
+
+int oxhip_dev_kv_append_shared(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_shared* shared, const void* k, size_t k_stride, const void* v,
+                               size_t v_stride, const void* q, size_t q_stride, void* q_out, size_t q_out_stride, size_t n_q, int dtype, const oxhip_rope* rope, void* stream) {
+    const char* who = "kv_append_shared";
+    SharedView sv{};
+    if (const char* why = check_shared(shared, &sv)) return refuse(who, why);
+    return append(who, c, kv, b, sv, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride, n_q, dtype, rope, stream);
 }
 
 int oxhip_dev_kv_read(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, size_t count, void* k_out, void* v_out, int dtype, void* stream) {
@@ -179,9 +199,8 @@ int oxhip_dev_attend_shared(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_
     KvBatchView bv;
     AttendCall call{};
     if (const char* why = check_attend(kv, b, q, q_stride, n_q, dtype, scale, rules, out, out_stride, &kvv, &bv, &call)) return refuse(who, why);
-    if (!shared || !shared->group_start || !shared->common) return refuse(who, "null argument");
-    if (!aligned(shared->group_start, 4) || !aligned(shared->common, 4)) return refuse(who, "an array of 4-byte values at an odd address");
-    if (!shared->n_groups || shared->n_groups > ((size_t)1 << 24)) return refuse(who, "1 to 2^24 groups");
+    SharedView sv{};
+    if (const char* why = check_shared(shared, &sv)) return refuse(who, why);
     if (!kv_launch_fits(kv_row_tiles(b->rows, n_q / kv->n_kv, true) * kv->n_kv, 512)) return refuse(who, "more rows or heads than one launch takes");
     if (!c) return refuse(who, "null context");
     if (!b->rows) return 1;
@@ -190,7 +209,7 @@ int oxhip_dev_attend_shared(oxhip_ctx* c, const oxhip_kv_cache* kv, const oxhip_
     hipStream_t s = static_cast<hipStream_t>(stream);
     DecodeScratch* sc = parts(c, s, who);
     if (!sc) return 0;
-    HIP_TRY(launch_attend_shared(kvv, bv, SharedView{shared->group_start, shared->common, (uint32_t)shared->n_groups}, call, *sc, s), "attend_shared launch");
+    HIP_TRY(launch_attend_shared(kvv, bv, sv, call, *sc, s), "attend_shared launch");
     return 1;
 }
 

@@ -270,7 +270,12 @@ hipError_t launch_moe_bf16_down(const WeightView& w, const GroupView& g, uint32_
 struct KvView;
 struct KvBatchView;
 struct RopeView;
-hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
+// The sequences whose first tokens are the same: those of group i are group_start[i] .. group_start[i + 1] - 1, and they share common[i] tokens.
+struct SharedView {
+    const int32_t *group_start, *common;
+    uint32_t n_groups;
+};
+hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const SharedView& shared, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
                             size_t q_stride, void* q_out, size_t q_out_stride, uint32_t n_q, bool bf16, hipStream_t s);
 hipError_t launch_kv_read(const KvView& kv, const KvBatchView& b, size_t count, void* k_out, void* v_out, bool bf16, hipStream_t s);
 struct AttendCall {
@@ -284,11 +289,6 @@ struct AttendCall {
     bool bf16;
 };
 hipError_t launch_attend(const KvView& kv, const KvBatchView& b, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
-// The sequences whose first tokens are the same: those of group i are group_start[i] .. group_start[i + 1] - 1, and they share common[i] tokens.
-struct SharedView {
-    const int32_t *group_start, *common;
-    uint32_t n_groups;
-};
 hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const SharedView& shared, const AttendCall& call, const DecodeScratch& sc, hipStream_t s);
 // The spans of `span_blocks` blocks that were chosen for each row and key head: [rows][n_kv][count].
 struct ChosenView {

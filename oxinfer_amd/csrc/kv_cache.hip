@@ -1,5 +1,7 @@
 // Filling the 8-bit key / value cache and reading it back: the rotation of queries and keys, the quantization per block of 32 tokens and
 // head, and the blocks' layout (kv_plan.hpp).
+#include <type_traits>
+
 #include "kv.hpp"
 
 namespace oxhip {
@@ -151,7 +153,25 @@ struct AppendArgs {
     size_t k_stride, v_stride, q_stride, q_out_stride;
     uint32_t vec, even;  // k, v, q and q_out by 16 bytes; whole runs of 8 channels rotate alike
     uint32_t tasks;      // heads of a sequence: keys, values, queries
+    SharedView shared;   // or none (group_start nullptr)
 };
+
+// The first position that is sequence s's own, by one wave: of the tokens before it, which its group's first sequence holds, nothing is stored, and what the
+// cache has in front of it in the same block is no token of this sequence's.
+__device__ __forceinline__ int32_t first_own(const SharedView& shared, int32_t s) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t base = 0, n = shared.n_groups + 1;  // the last of the groups' borders at s or before it; up to 64 of them take one request
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64;
+        const uint64_t m = __ballot(lane * step < n && shared.group_start[min(base + lane * step, shared.n_groups)] <= s);
+        const uint32_t at = m ? 63u - (uint32_t)__builtin_clzll(m) : 0u;
+        base += at * step;
+        n = min(step, n - at * step);
+    }
+    if (base >= shared.n_groups) return 0;
+    const int32_t leader = shared.group_start[base];
+    return leader >= 0 && leader < s ? max(shared.common[base], 0) : 0;
+}
 
 // One block of 32 positions (those of them that the call's rows take) of one head per workgroup: blockIdx.y below n_kv its keys, below
 // 2 n_kv its values, behind them a query head of the same rows.
@@ -161,8 +181,8 @@ struct AppendArgs {
 // nothing and grows to what is needed.)
 // The bound is memory: rows read once, a byte a value written. A block that is new, or most of it, goes out as whole 16-byte lines through an
 // image in LDS (a value operand's tokens lie 1 byte apart, its channels 16); single tokens are stored as they lie.
-// MOST: runs of eight channels a thread holds, d / 64.
-template <bool BF16, int MOST>
+// MOST: runs of eight channels a thread holds, d / 64. SHARED: the batch's sequences share first tokens.
+template <bool BF16, int MOST, bool SHARED>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     __shared__ double top_s[4];
     __shared__ __align__(16) uint8_t image[KV_BLOCK * 64 * MOST];
@@ -176,13 +196,23 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     const int32_t before = q.len - q.n;  // (negative: rows before the sequence's first token are left out)
     const int32_t from = max(before, 0);
     const int32_t block = from / (int32_t)KV_BLOCK + place, p0 = block * (int32_t)KV_BLOCK;
-    const int32_t lo = max(p0, from), hi = min(p0 + (int32_t)KV_BLOCK, q.len);  // positions of this block that are new
+    int32_t lo = max(p0, from);
+    const int32_t hi = min(p0 + (int32_t)KV_BLOCK, q.len);  // positions of this block that are new
     if (place < 0 || hi <= lo || q.n <= 0) return;
+    int32_t own = 0;
+    const bool query = blockIdx.y >= 2 * a.kv.n_kv;
+    if constexpr (SHARED) {
+        if (!query) {
+            own = first_own(a.shared, s);
+            lo = max(lo, own);
+            if (hi <= lo) return;
+        }
+    }
     const uint32_t per = d / 8, units = (uint32_t)(hi - lo) * per;  // eight channels of a token each
     const size_t first = (size_t)(q.row0 + (lo - before));
 
     double x[MOST][8];
-    if (blockIdx.y >= 2 * a.kv.n_kv) {
+    if (query) {
         const size_t head = (size_t)(blockIdx.y - 2 * a.kv.n_kv) * d;
 #pragma unroll
         for (int i = 0; i < MOST; i++) {
@@ -205,7 +235,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     const size_t index = kv_block_index(a.kv, page, head, (uint32_t)block);
     uint8_t* codes = (values ? a.kv.v : a.kv.k) + index * KV_BLOCK * d;
     float* scale_at = (values ? a.kv.v_scale : a.kv.k_scale) + index;
-    const bool old = lo > p0;  // the block holds tokens of earlier calls
+    const bool old = lo > max(p0, own);  // the block holds tokens of earlier calls
     const float held = old ? *scale_at : KV_SCALE_MIN;
 
     double top = 0.0;
@@ -270,16 +300,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         for (uint32_t i = tid; i < KV_BLOCK * d / 16; i += 256) *reinterpret_cast<uint4*>(codes + 16 * i) = *reinterpret_cast<const uint4*>(image + 16 * i);
         return;
     }
-    // a block without older tokens: what lies behind the last new one is nobody's yet, and becomes zeros
+    // a block without older tokens: what lies behind the last new one is nobody's yet, and becomes zeros (so do the places in front of the sequence's first own token)
     for (uint32_t i = tid; i < KV_BLOCK * d / 16; i += 256) {
         uint4 u = *reinterpret_cast<const uint4*>(image + 16 * i);
-        if (hi - p0 < (int32_t)KV_BLOCK) {
+        if (hi - lo < (int32_t)KV_BLOCK) {
             const uint32_t g = i * 16 % 1024 / 256, n = i % 16;
             uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (uint32_t k = 0; k < 16; k++) {
                 const uint32_t t = values ? k % 8 / 4 * 16 + 4 * g + k % 4 : k / 8 * 16 + n;
-                if (t >= (uint32_t)(hi - p0)) w[k / 4] = (w[k / 4] & ~(0xFFu << (8 * (k % 4)))) | 128u << (8 * (k % 4));
+                if (t >= (uint32_t)(hi - p0) || (SHARED && t < (uint32_t)(lo - p0))) w[k / 4] = (w[k / 4] & ~(0xFFu << (8 * (k % 4)))) | 128u << (8 * (k % 4));
             }
             u = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -289,7 +319,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 
 // The same for one new token a sequence (row_start NULL): a wave takes one head's keys, values or query, four channels a lane, and needs no other
 // wave. A step of 64 sequences, 32 query heads over 8 of 128 channels: 11.9 us with the kernel above, a workgroup to a head, 5.7 here.
-template <bool BF16>
+template <bool BF16, bool SHARED>
 __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendArgs a) {
     const uint32_t d = a.kv.d, lane = threadIdx.x & 63, c = 4 * lane;
     const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), s = task / a.tasks, what = task % a.tasks;  // (a sequence's heads: keys, values, queries)
@@ -315,13 +345,19 @@ __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendArgs a) {
         if (live) store_run<BF16, 4>(a.q_out, (size_t)s * a.q_out_stride + (size_t)head * d + c, a.vec & 8, x);
         return;
     }
+    int32_t own = 0;
+    if constexpr (SHARED) {
+        own = first_own(a.shared, (int32_t)s);
+        if (pos < own) return;
+    }
     const uint32_t block = (uint32_t)pos / KV_BLOCK, t = (uint32_t)pos % KV_BLOCK;
+    const bool old = t && (!SHARED || pos > own);  // the block holds tokens of earlier calls
     const int32_t page = kv_page(a.b, a.kv, (int32_t)s, block);
     if (page < 0) return;
     const size_t index = kv_block_index(a.kv, page, head, block);
     uint8_t* codes = (key ? a.kv.k : a.kv.v) + index * KV_BLOCK * d;
     float* scale_at = (key ? a.kv.k_scale : a.kv.v_scale) + index;
-    const float was = t ? sound_scale(*scale_at) : KV_SCALE_MIN;
+    const float was = old ? sound_scale(*scale_at) : KV_SCALE_MIN;
     double top = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -331,7 +367,7 @@ __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendArgs a) {
 #pragma unroll
     for (int m = 32; m; m >>= 1) top = fmax(top, __shfl_xor(top, m));
     const float scale = grown_scale(was, top);
-    if (t && scale != was) {  // the codes that are there, first
+    if (old && scale != was) {  // the codes that are there, first
         for (uint32_t i = lane; i < KV_BLOCK * d / 16; i += 64) {
             uint4 u = *reinterpret_cast<const uint4*>(codes + 16 * i);
             const float ratio = was / scale;
@@ -343,7 +379,7 @@ __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendArgs a) {
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the token's own bytes go there behind them)
     }
-    if (lane == 0 && (!t || scale != was)) *scale_at = scale;
+    if (lane == 0 && (!old || scale != was)) *scale_at = scale;
     if (!live) return;
     const double inv = 1.0 / (double)scale;
     uint32_t code[4];
@@ -437,24 +473,30 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
     }
 }
 
-hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
+hipError_t launch_kv_append(const KvView& kv, const KvBatchView& b, const SharedView& shared, const RopeView& rope, const void* k, size_t k_stride, const void* v, size_t v_stride, const void* q,
                             size_t q_stride, void* q_out, size_t q_out_stride, uint32_t n_q, bool bf16, hipStream_t s) {
-    AppendArgs a{kv, b, rope, k, v, q, q_out, k_stride, v_stride, q_stride, q_out_stride, 0, 0, 2 * kv.n_kv + n_q};
+    AppendArgs a{kv, b, rope, k, v, q, q_out, k_stride, v_stride, q_stride, q_out_stride, 0, 0, 2 * kv.n_kv + n_q, shared};
     const size_t size = bf16 ? 2 : 4;
     auto vec = [&](const void* p, size_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; };
     a.vec = (vec(k, k_stride) ? 1u : 0u) | (vec(v, v_stride) ? 2u : 0u) | (vec(q, q_stride) ? 4u : 0u) | (vec(q_out, q_out_stride) ? 8u : 0u);
     a.even = rope.half % 8 == 0;
     if (!b.row_start) {
         const unsigned grid = (unsigned)kv_append_workgroups(false, b.rows, b.n_seqs, a.tasks);
-        if (bf16) kv_append_step_kernel<true><<<grid, 256, 0, s>>>(a);
-        else kv_append_step_kernel<false><<<grid, 256, 0, s>>>(a);
+        auto step = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
+        if (shared.group_start) bf16 ? step(kv_append_step_kernel<true, true>) : step(kv_append_step_kernel<false, true>);
+        else bf16 ? step(kv_append_step_kernel<true, false>) : step(kv_append_step_kernel<false, false>);
         return hipGetLastError();
     }
     const dim3 grid((unsigned)kv_append_workgroups(true, b.rows, b.n_seqs, a.tasks), a.tasks);
     auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
-    if (kv.d <= 64) bf16 ? go(kv_append_kernel<true, 1>) : go(kv_append_kernel<false, 1>);
-    else if (kv.d <= 128) bf16 ? go(kv_append_kernel<true, 2>) : go(kv_append_kernel<false, 2>);
-    else bf16 ? go(kv_append_kernel<true, 4>) : go(kv_append_kernel<false, 4>);
+    auto of = [&](auto sharing) {
+        constexpr bool SHARED = decltype(sharing)::value;
+        if (kv.d <= 64) bf16 ? go(kv_append_kernel<true, 1, SHARED>) : go(kv_append_kernel<false, 1, SHARED>);
+        else if (kv.d <= 128) bf16 ? go(kv_append_kernel<true, 2, SHARED>) : go(kv_append_kernel<false, 2, SHARED>);
+        else bf16 ? go(kv_append_kernel<true, 4, SHARED>) : go(kv_append_kernel<false, 4, SHARED>);
+    };
+    if (shared.group_start) of(std::true_type{});
+    else of(std::false_type{});
     return hipGetLastError();
 }
 

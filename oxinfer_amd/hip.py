@@ -155,6 +155,7 @@ def load_library():
         "oxhip_dev_kv_read": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), sz, vp, vp, C.c_int, vp]),
         "oxhip_dev_attend": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
         "oxhip_dev_logits": (C.c_int, [vp, vp, sz, vp, sz, sz, sz, C.c_int, C.POINTER(LogitRulesC), vp, vp]),
+        "oxhip_dev_kv_append_shared": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSharedC), vp, sz, vp, sz, vp, sz, vp, sz, sz, C.c_int, C.POINTER(RopeC), vp]),
         "oxhip_dev_attend_shared": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSharedC), vp, sz, sz, C.c_int, C.c_float, C.POINTER(AttendRulesC), vp, sz, vp]),
         "oxhip_dev_kv_summarize": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSummaryC), vp]),
         "oxhip_dev_kv_summary_read": (C.c_int, [vp, C.POINTER(KvCacheC), C.POINTER(KvBatchC), C.POINTER(KvSummaryC), sz, vp, vp]),
@@ -697,10 +698,11 @@ class HipBackend:
         scales = [torch.zeros((n_pages, n_kv, per), dtype=torch.float32, device=dev) for _ in range(2)]
         return KvCache(*codes, *scales, page_tokens, d)
 
-    def kv_append(self, cache, batch, k, v, q=None, rope=None, q_out=None):
+    def kv_append(self, cache, batch, k, v, q=None, rope=None, q_out=None, shared=None):
         """The rows' keys and values [rows, n_kv * d] (f32 or bf16; any row stride) into the cache; the keys, and the queries [rows, n_q * d],
         rotated by `rope`. Returns the rotated queries (`q_out`, which may be q) or None. Rows behind the last sequence, and rows before a
-        sequence's first token, are left as `q_out` has them: in a new one they may hold anything."""
+        sequence's first token, are left as `q_out` has them: in a new one they may hold anything. `shared` (`KvShared`): the sequences' first tokens
+        are their group's first one's, and each one's own begin behind them, also inside a block."""
         self._held(cache, batch)
         dev, rows, width = self.device, batch.rows, cache.n_kv * cache.d
         kp, ks, kd = _rows("k", k, width, rows, dev)
@@ -723,8 +725,14 @@ class HipBackend:
             raise ValueError("q, q_out, k and v have one type")
         if rope is not None and rope.device != dev:
             raise ValueError(f"rope: wanted on cuda:{dev}")
-        if rows and not self.lib.oxhip_dev_kv_append(self.ctx, cache.ref, batch.ref, kp, ks, vp, vs, qp, qs, op, os_, n_q, kd, rope.ref if rope is not None else None,
-                                                     self._stream_here()):
+        rest = kp, ks, vp, vs, qp, qs, op, os_, n_q, kd, rope.ref if rope is not None else None, self._stream_here()
+        if shared is None:
+            done = not rows or self.lib.oxhip_dev_kv_append(self.ctx, cache.ref, batch.ref, *rest)
+        else:
+            if shared.device != dev:
+                raise ValueError(f"shared: wanted on cuda:{dev}")
+            done = not rows or self.lib.oxhip_dev_kv_append_shared(self.ctx, cache.ref, batch.ref, shared.ref, *rest)
+        if not done:
             raise RuntimeError(self.last_error())
         return q_out
 

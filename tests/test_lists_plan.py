@@ -137,3 +137,25 @@ def test_the_bindings_own_checks():
     with pytest.raises(ValueError, match="wanted"):
         hip.KvSummary(z(3, 2, 64, t=torch.int8), z(3, 2, t=torch.float32), 32)
     assert os.path.exists(hip.library_path())
+
+
+def test_appends_behind_shared_tokens_that_are_refused(lib):  # noqa: F811
+    """What oxhip_dev_kv_append refuses, and groups that are none."""
+    from oxinfer_amd import hip
+
+    def append(s, of=(P, P, 2), k=P, ks=0, q=P, n_q=4, dtype=0, rope=None, null=False):
+        r = C.byref(hip.RopeC(*rope)) if rope else None
+        return said(lib, lib.oxhip_dev_kv_append_shared(None, C.byref(s[0]), C.byref(s[1]), None if null else C.byref(hip.KvSharedC(*of)), k, ks, P, 0, q, 0, q, 0, n_q, dtype, r, None))
+
+    good = structs(hip)
+    for kw in (dict(), dict(q=None, n_q=0), dict(dtype=1, k=P + 2), dict(ks=130), dict(rope=(P, 100, 32, 0))):
+        assert "null context" in append(good, **kw), kw
+    for kw in (dict(null=True), dict(of=(None, P, 2)), dict(of=(P, None, 2)), dict(of=(P, P, 0)), dict(of=(P, P, 2**25)), dict(of=(P + 2, P, 2)), dict(of=(P, P + 1, 2)), dict(k=None), dict(k=P + 2), dict(ks=1), dict(q=None),
+               dict(n_q=0), dict(dtype=2), dict(rope=(P, 0, 32, 0)), dict(rope=(None, 4, 32, 0))):
+        assert "null context" not in append(good, **kw), kw
+        assert lib.oxhip_last_error().decode().startswith("kv_append_shared: ")
+    for kv, b in OF_KV:
+        assert "null context" not in append(structs(hip, kv, b))
+    m = 2**20
+    ragged = lambda rows: append(structs(hip, {}, dict(n_seqs=7 * m, rows=rows, row_start=P)), q=None, n_q=0)  # noqa: E731
+    assert "null context" in ragged(5) and "one launch" in ragged(2**28)

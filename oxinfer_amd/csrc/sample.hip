@@ -588,7 +588,7 @@ __device__ __forceinline__ bool draw(const SampleArgs& a, DrawShared& sh, uint32
         return (o > cut.order || (o == cut.order && i <= tie_end)) && (double)w >= least ? w : 0;
     };
     __syncthreads();
-    if (cut.order || everything)
+    if (cut.order || everything || (flags & ROW_K))  // (also of a top-k past all tokens that weigh anything, which keeps those set apart)
         by_slices(sh.slice, [&](const float (&x)[4], const uint32_t (&i)[4]) {
             uint64_t w[4], v = 0;
             weight.of(x, w);

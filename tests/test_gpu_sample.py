@@ -272,3 +272,15 @@ def test_the_bindings_refusals(be):
         with pytest.raises((ValueError, RuntimeError)):
             be.sample(**(dict(logits=x, u=u) | bad))
     assert be.sample(x[:0], u[:0])[0].shape == (0,)
+
+
+def test_top_k_behind_the_last_weight(be):
+    """More tokens are asked for than weigh anything, and the last ones that do share a step of weight with some that do not: none is left out of the sum."""
+    x = np.full((1, 9000), -1e4, np.float32)
+    best = 0.5 / (4 / np.log(2))  # (in the middle of a step, as is then the weight of half a unit, 2^-47)
+    at = lambda octaves: np.float32(best - octaves * np.log(2))  # noqa: E731
+    x[0, :3000] = at(46.95)  # one unit
+    x[0, 5100:8100] = at(47.05)  # none
+    x[0, [5000, 8500]] = best
+    # the middle of the whole lies between the two best ones, 1500 units before the end of the first
+    assert check(be, torch.from_numpy(x).cuda(), np.array([0.5], np.float32), top_k=np.array([4000], np.int32)).tolist() == [5000]

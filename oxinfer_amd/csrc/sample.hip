@@ -239,7 +239,14 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
     if (top == -__builtin_inff()) out.flags = ROW_EMPTY;
     else if (r.greedy) out.flags = ROW_GREEDY;
     else if (!sorted || !(fabsf(top * scale) < 1e30f)) out.flags = ROW_WHOLE;
-    else if (limits) {
+    else if (limits && fabsf(step_of(top, scale)) >= 0x1p23f) {
+        // Steps are whole numbers below 2^23 only: past that a token's may lie some ulps of them off (2^-23 of `high`, for it and the best one together), also past the last
+        // one that is counted. What weighs anything is all looked at then: neighbouring logits are a step apart and more, so that it is of few different values.
+        const float high = step_of(top, scale);
+        out.low = high - (float)SAMPLE_STEPS - fabsf(high) * 0x1p-21f;
+        out.high = __builtin_inff();
+        out.flags = (number ? ROW_K : 0u) | (r.p < 1.0f ? ROW_P : 0u);
+    } else if (limits) {
         // the row's steps from the slices', which begin each at its own largest logit
         const float high = step_of(top, scale);
         for (uint32_t s = tid; s < a.slices; s += SAMPLE_THREADS) {
@@ -320,10 +327,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_scan_kernel(SampleArgs 
                 p_hi = min(first([&](uint32_t j) { return m_to[j] >= want * (1.0f + NEAR); }), (int)SAMPLE_STEPS - 1);
                 p_lo = min(p_lo, p_hi);
             }
-            // Tokens that min-p leaves lie within so many steps of the best: limits below them are none.
+            // Tokens that min-p leaves lie within so many steps of the best: limits below them are none. (Four steps for a weight of half a unit, held as one; two for both steps' roundings.)
             bool k_in = k_on;
             if (r.least > 0.0f) {
-                const int reach = (int)fminf(-4.0f * __builtin_amdgcn_logf(fminf(r.least, 1.0f)) + 2.5f, 10000.0f);
+                const int reach = (int)fminf(-4.0f * __builtin_amdgcn_logf(fminf(r.least, 1.0f)) + 6.5f, 10000.0f);
                 if ((!p_on || p_lo > reach) && (!k_in || k_at > reach)) p_on = k_in = false;
             }
             if (k_in || p_on) {

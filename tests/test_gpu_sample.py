@@ -274,6 +274,55 @@ def test_the_bindings_refusals(be):
     assert be.sample(x[:0], u[:0])[0].shape == (0,)
 
 
+def below(top, ulps):
+    """The f32 value so many steps of f32 below `top`."""
+    for _ in range(ulps):
+        top = np.nextafter(np.float32(top), np.float32(-np.inf))
+    return top
+
+
+def test_small_temperatures_pass_no_limit_over(be):
+    """Best logits over the temperature of 2^23 and more, where neighbouring f32 logits weigh what the limits tell apart."""
+    x = np.full((2, 5000), -1e4, np.float32)
+    top = np.float32(15.160547)
+    x[:, 40] = top
+    x[:, [10, 20, 30]] = below(top, 2)  # 0.148 of the best: top-p keeps one of them, and so does top-k
+    up = torch.from_numpy(x).cuda()
+    u, heat, least = np.full(2, 0.2, np.float32), np.full(2, 1e-6, np.float32), np.full(2, 0.1388, np.float32)
+    assert check(be, up, u, temperature=heat, min_p=least, top_p=np.full(2, 0.75, np.float32)).tolist() == [40, 40]
+    assert check(be, up, u, temperature=heat, min_p=least, top_k=np.full(2, 2, np.int32)).tolist() == [40, 40]
+    # 2^-37 of the best: with top-k 2 one of them is left, and the random number lies between it and the next
+    x[:] = -1e4
+    top = np.float32(14.092963218688965)
+    x[:, 3] = top
+    x[:, :3] = below(top, 4)
+    up = torch.from_numpy(x).cuda()
+    heat = np.full(2, 1.4791656610668724e-07, np.float32)
+    assert check(be, up, np.full(2, 600 * 2.0**-46, np.float32), temperature=heat, top_k=np.full(2, 2, np.int32)).tolist() == [3, 3]
+
+
+def test_neighbouring_logits_at_any_temperature(be):
+    rng = np.random.default_rng(21)
+    t, vocab = 400, 6000
+    heat = (10 ** rng.uniform(-8, -4, t)).astype(np.float32)
+    x = np.full((t, vocab), -1e4, np.float32)
+    least = np.zeros(t, np.float32)
+    for r in range(t):
+        top = np.float32(rng.uniform(1, 40) * rng.choice([1, 1, -1]))
+        ids = rng.permutation(vocab)
+        at = 0
+        for ulps in (0, 1, 2, 3):
+            n = int(rng.integers(1, 7)) if ulps else int(rng.integers(1, 3))
+            x[r, ids[at : at + n]] = below(top, ulps)
+            at += n
+        w = np.exp((float(below(top, int(rng.integers(0, 4)))) - float(top)) / float(heat[r]))
+        least[r] = w * rng.uniform(0.3, 0.98)
+    up = torch.from_numpy(x).cuda()
+    u, p, k = rng.uniform(0.001, 0.999, t).astype(np.float32), rng.uniform(0.2, 0.999, t).astype(np.float32), rng.integers(1, 12, t).astype(np.int32)
+    for rules in (dict(top_p=p), dict(top_k=k), dict(min_p=least), dict(top_p=p, min_p=least), dict(top_k=k, min_p=least), dict(top_p=p, top_k=k), dict(top_p=p, top_k=k, min_p=least)):
+        check(be, up, u, temperature=heat, **rules)
+
+
 def test_top_k_behind_the_last_weight(be):
     """More tokens are asked for than weigh anything, and the last ones that do share a step of weight with some that do not: none is left out of the sum."""
     x = np.full((1, 9000), -1e4, np.float32)

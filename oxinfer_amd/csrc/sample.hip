@@ -127,6 +127,7 @@ __device__ __forceinline__ Rules rules_of(const SampleArgs& a, uint32_t row) {
     r.heat = a.temperature ? a.temperature[row] : 1.0f;
     r.greedy = !(r.heat > 0.0f);
     r.k = a.top_k ? a.top_k[row] : 0;
+    if (r.k > 0 && (uint32_t)r.k >= a.vocab) r.k = 0;  // (none: top-p then has its steps' weights, which are not summed where tokens are counted for top-k)
     r.p = a.top_p ? a.top_p[row] : 1.0f;
     r.least = a.min_p ? a.min_p[row] : 0.0f;
     r.u = a.u[row];

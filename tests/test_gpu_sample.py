@@ -333,3 +333,23 @@ def test_top_k_behind_the_last_weight(be):
     x[0, [5000, 8500]] = best
     # the middle of the whole lies between the two best ones, 1500 units before the end of the first
     assert check(be, torch.from_numpy(x).cuda(), np.array([0.5], np.float32), top_k=np.array([4000], np.int32)).tolist() == [5000]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_top_k_of_the_whole_vocabulary_is_none(be, dtype):
+    """Bit for bit what no top-k gives, beside rows that have one; of one token less the last of equal ones is left out."""
+    rng = np.random.default_rng(16)
+    x = (3 * torch.randn(12, 40003, device="cuda")).to(dtype)
+    u = torch.rand(12, device="cuda")
+    for names in ((), ("top_p",), ("min_p",), ("temperature", "top_p", "min_p")):
+        rules = {k: torch.from_numpy(v).cuda() for k, v in rules_of(12, rng, names).items()}
+        none = be.sample(x, u, **rules)
+        for k in (40003, 40004, 2**31 - 1):
+            got = be.sample(x, u, top_k=torch.full((12,), k, dtype=torch.int32, device="cuda"), **rules)
+            assert all(torch.equal(a, b) for a, b in zip(got, none))
+        some = torch.tensor([k for _ in range(4) for k in (40003, 7, 0)], dtype=torch.int32, device="cuda")
+        got = be.sample(x, u, top_k=some, **rules)
+        assert all(torch.equal(a[some != 7], b[some != 7]) for a, b in zip(got, none))
+    flat = torch.zeros(2, 5000, device="cuda", dtype=dtype)
+    assert check(be, flat, np.full(2, 0.99999, np.float32), top_k=np.array([4999, 5000], np.int32)).tolist() == [4998, 4999]
+    assert check(be, flat[:, :1], np.zeros(2, np.float32), top_k=np.array([1, 5], np.int32)).tolist() == [0, 0]

@@ -765,7 +765,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
             }
         }
     }
-    // (where those above are few, they are set apart with the others: a row that has few of both is done by their ranks)
+    // (where those above are few, they are set apart with the others, if all of them fit: a row that has few of both is done by their ranks)
     if (!limits) higher = 0;
     const uint32_t n = __popc(named), n_upto = wave_upto(n), both = __popc(named | higher), both_upto = wave_upto(both);
     kept = wave_sum(kept);
@@ -788,7 +788,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
         n_both += counts_s[w][0];
         n_named += counts_s[w][1];
     }
-    const bool with = n_both - n_named <= SAMPLE_WITH;
+    const bool with = n_both - n_named <= SAMPLE_WITH && n_both <= a.room;
     const uint32_t set = with ? named | higher : named;
     uint32_t to = with ? both_before + both_upto - both : named_before + n_upto - n;
     const size_t place = (size_t)at * a.slices + slice;
@@ -799,7 +799,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_sums_kernel(SampleArgs 
             to++;
         }
     if (tid == 0) {
-        SampleSlice o{0, 0, 0, n_both - n_named, with ? n_both : n_named};
+        SampleSlice o{0, 0, 0, (uint16_t)(n_both - n_named), (uint16_t)(with ? n_both : n_named), with};
 #pragma unroll
         for (uint32_t w = 0; w < WAVES; w++) {
             o.all += sums_s[w][0];
@@ -880,7 +880,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
             sh.slice[s] = p.kept;
             sh.offset[s] = p.n;
             over = over || p.n > a.room;
-            without = without || p.n_above > SAMPLE_WITH;
+            without = without || !p.with;
         }
         whole = __syncthreads_or(over);
         with = !__syncthreads_or(without);

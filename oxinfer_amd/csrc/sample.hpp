@@ -17,7 +17,8 @@ struct SampleRow {
 // What the second pass finds out about a slice.
 struct SampleSlice {
     unsigned long long all, above, kept;  // weights: of all its tokens, of those above the limit's steps, of those of these that min-p leaves
-    uint32_t n_above, n;                  // tokens above; tokens in them
+    uint16_t n_above, n;                  // tokens above; tokens that are set apart
+    uint32_t with;                        // those above are among these
 };
 
 struct SampleArgs {

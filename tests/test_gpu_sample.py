@@ -353,3 +353,24 @@ def test_a_top_k_of_the_whole_vocabulary_is_none(be, dtype):
     flat = torch.zeros(2, 5000, device="cuda", dtype=dtype)
     assert check(be, flat, np.full(2, 0.99999, np.float32), top_k=np.array([4999, 5000], np.int32)).tolist() == [4998, 4999]
     assert check(be, flat[:, :1], np.zeros(2, np.float32), top_k=np.array([1, 5], np.int32)).tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("rows", [1, 64, 170, 256])
+def test_tokens_set_apart_and_the_room_for_them(be, rows):
+    """Slices of 4096 with 180 to 250 tokens above the limit's step and 10 to 300 in it, in launches of few rows and of as many as leave a slice room for about 256."""
+    rng = np.random.default_rng(rows)
+    vocab = 100_000
+    v = np.arange(vocab) % 4096
+    x = (0.02 * rng.normal(size=(rows, vocab))).astype(np.float32)
+    above, at = rng.integers(180, 251, rows), rng.integers(10, 301, rows)
+    x += np.where(v < above[:, None], 8, np.where(v < (above + at)[:, None], 7, 0)).astype(np.float32)
+    up, u = torch.from_numpy(x).cuda(), rng.random(rows).astype(np.float32)
+    w = np.exp(np.array([8.0, 7.0]))
+    p = ((above * w[0] + at * w[1] * rng.uniform(0.1, 0.9, rows)) / (above * w[0] + at * w[1] + (4096 - above - at))).astype(np.float32)  # (falls among those of 7)
+    k = ((above + (at * rng.uniform(0.1, 0.9, rows)).astype(int)) * (vocab // 4096)).astype(np.int32)
+    least = np.exp(rng.uniform(-1.1, -0.9, rows)).astype(np.float32)
+    for rules in (dict(top_p=p), dict(top_k=k), dict(top_p=p, min_p=least), dict(top_k=k, min_p=least), dict(top_k=k, top_p=p)):
+        some = np.unique(rng.integers(0, rows, 12))
+        got, logp = be.sample(up, torch.from_numpy(u).cuda(), **{n: torch.from_numpy(a).cuda() for n, a in rules.items()})
+        few = check(be, up[torch.from_numpy(some).cuda()], u[some], **{n: a[some] for n, a in rules.items()})
+        assert few.tolist() == got[torch.from_numpy(some).cuda()].tolist()

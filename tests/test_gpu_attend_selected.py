@@ -517,3 +517,59 @@ def test_the_bindings_refusals(be):
         be.kv_summarize(other, batch, held)
     with pytest.raises(ValueError):
         hip.KvSummary(held.code.float(), held.scale, 64)
+
+
+# ---- the choice over tables as large as they may be (scores of more LDS than a launch has unasked), by sixteen waves and by eight ------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 300])
+def test_choice_over_the_largest_table(be, n, dtype):
+    """16384 spans' room, one row (sixteen waves) and as many as eight waves each take."""
+    w = kv_ref.World([524027], 1, 32, page=256, seed=n, n=[n])
+    assert w.table.shape[1] * 256 // 32 == 16384
+    for count, last in ((100, 1), (1, 0), (16000, 7)) if n == 1 else ((64, 2),):
+        check_choice(be, w, 2, 32, count, first=min(count - 1, 3), last=last, dtype=dtype, ragged=n > 1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("spans", [4094, 4095, 4096, 4100])
+def test_choice_where_scores_outgrow_a_launchs_own_lds(be, spans, dtype):
+    """4096 spans' room in a table is 32 KiB of scores. One row and drafted ones."""
+    for n in ([1], [6]):
+        w = kv_ref.World([32 * spans - 7], 1, 64, page=32, seed=spans, n=n)
+        check_choice(be, w, 3, 32, 40, dtype=dtype, ragged=n != [1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,lens", [(64, [32700, 33000, 20]), (64, [60000, 65000, 40000]), (96, [100000, 131000, 90]), (256, [33000, 32900, 40])])
+def test_choice_for_drafted_rows_over_long_caches(be, d, lens, dtype):
+    """Sixteen waves over up to four rows of a sequence each, heads of any size."""
+    for n, g in (([5, 3, 1], 2), ([1, 9, 2], 5), ([2, 2, 2], 16)):
+        check_choice(be, kv_ref.World(lens, 1, d, page=64, seed=d, n=n), g, 32, 33, last=2, dtype=dtype, ragged=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [160, 192, 224, 256])
+def test_choice_of_wide_heads_for_one_token_of_a_long_cache(be, d, dtype):
+    check_choice(be, kv_ref.World([33500], 2, d, page=128, seed=d), 4, 32, 50, dtype=dtype)
+
+
+def test_choice_over_the_largest_table_by_a_recorded_plan(be):
+    from oxinfer_amd import hip
+    w = kv_ref.World([524027], 1, 32, page=256, seed=2)
+    cache, batch = w.tensors(hip)
+    held, code, scale = summary(be, w, hip, cache, 32, np.random.default_rng(1))
+    q, out = torch.zeros(1, 64, device="cuda"), torch.empty((1, 1, 90), dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        plan = be.plan_record(lambda: be.kv_select(cache, batch, held, q, 90, out=out))
+        for length in (524027, 400000, 200, 524032):
+            batch.kv_len.fill_(length)
+            q.normal_()
+            plan.replay()
+            torch.cuda.current_stream().synchronize()
+            w.lens = np.array([length])
+            want = lists_ref.select(w, q.cpu().numpy().reshape(1, 2, 32), 2, 32, code, scale, 90, 1, 1)
+            assert np.array_equal(out.cpu().numpy(), want)
+    del plan

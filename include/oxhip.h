@@ -400,7 +400,9 @@ typedef struct {
     const int32_t* common;      /* [n_groups] */
     size_t n_groups;
 } oxhip_kv_shared;
-/* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for up to 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence:
+/* oxhip_dev_attend of such a batch, the shared tokens of a group being read once for up to 16 / g of its rows (g = n_q / n_kv) instead of once for each sequence (where the
+ * rows, their heads and the tables' room, max_pages, come to more than the chip takes at once: smaller batches read them for each row, which is faster there. The host goes by
+ * max_pages, not by the lengths, so a table no wider than its step needs has the form that fits):
  * token j < common of a sequence lies in the page that the table of its group's FIRST sequence names, any other in its own table's. (Tables that all name
  * the shared pages, as those of sequences that share whole pages may, fit both calls.) Everything else is oxhip_dev_attend's: rules, types, rows that see nothing, pages outside the cache;
  * rows that are no sequence's (also of row numbers that do not ascend) are left as they are. For batches of few rows a sequence: a prompt's are
@@ -433,7 +435,8 @@ int oxhip_dev_kv_summary_read(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const ox
  * the others those of the highest score, of equal ones the lower; ascending, -1 behind the last (all spans, where there are no more than count). The score of
  * a span is max over the key head's query heads of (sum of products of bytes) * its scale * the query's, the query being made bytes as a mean
  * key is (its scale max |q| times the f32 nearest to 1 / 127; NaN as 0, infinity as the largest value); the sum is exact and the products are formed in f64. A span of a page outside the cache has the lowest score.
- * q [rows, n_q, d] as oxhip_dev_attend's. A sequence's table has room for 16384 spans at most (max_pages * page_tokens / span). */
+ * q [rows, n_q, d] as oxhip_dev_attend's. A sequence's table has room for 16384 spans at most (max_pages * page_tokens / span); rows of a sequence that share
+ * a workgroup's reading of its mean keys are min(16 / g, 8, 4096 / room) at most. */
 int oxhip_dev_kv_select(oxhip_ctx* ctx, const oxhip_kv_cache* kv, const oxhip_kv_batch* b, const oxhip_kv_summary* sum, const void* q, size_t q_stride, size_t n_q, int dtype,
                         size_t count, size_t first, size_t last, int32_t* chosen, void* stream);
 /* oxhip_dev_attend over the spans alone that `chosen` [rows, n_kv, count] names for a row and key head (of those keys, what the rules let the row see). Numbers that are

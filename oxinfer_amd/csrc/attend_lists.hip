@@ -6,7 +6,7 @@
 //
 // Shared: 64 sequences behind 8192 tokens and up to 1024 of their own, 8 key heads of 128 with 4 heads each, bf16, 40 us (68 MB from memory 13; `attend` over tables that
 // name the shared pages 120); 128 behind 32768, f32, 197 (the products, twice for two planes, 117; `attend` 625). A block that 16 tiles of a key head take each comes from the L2
-// all but once (93 % hits of the longer case), at 10 to 12 TB/s; a wave's step of 240 vector and 16 matrix instructions (32 of f32 rows) is a chain that four waves a SIMD do not quite
+// all but once (93 % hits of the longer case), at 10 to 12 TB/s (the rate seen: that the L2 gives no more is not shown); a wave's step of 240 vector and 16 matrix instructions (32 of f32 rows) is a chain that four waves a SIMD do not quite
 // fill. Chosen: 64 sequences, 64 spans of 64 each, 88 us: memory, 5.4 TB/s.
 #include <cmath>
 
@@ -50,7 +50,8 @@ hipError_t launch_attend_shared(const KvView& kv, const KvBatchView& b, const Sh
     unsigned grid;
     // Rows share what they read where there is more of it than the chip takes at once. Fewer have tiles of their own, whose lists are shorter and whose workgroups have fewer entries
     // to join (8 key heads of 128, 4 heads each, f32: 4 sequences behind 700 tokens 11.1 us, 14.1 of four rows a tile; 32 of them 11.1 and 14.3; 8 behind 3000 tokens 16.2 and 20.4; and from the
-    // border on 64 behind 700 tokens 16.2 and 14.5; 16 behind 3000 21.7 and 20.6; 16 behind 12000 43.0 and 27.7).
+    // border on 64 behind 700 tokens 16.2 and 14.5; 16 behind 3000 21.7 and 20.6; 16 behind 12000 43.0 and 27.7). The host knows the tables' room alone: four answers behind 700 tokens in
+    // tables for 131072 share tiles, and take 13.8 us.
     const uint64_t blocks = (uint64_t)b.max_pages << kv.shift, alone = kv_row_tiles(b.rows, a.g, false) * kv.n_kv * ((blocks + a.least - 1) / a.least);
     const hipError_t e = spread(a, sc, alone > 256, false, blocks, 256 * split_places((int)kv.d / 32), &grid);
     return e != hipSuccess ? e : go<SHARED>(a, call.bf16, rules, grid, s);
@@ -67,7 +68,7 @@ hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const 
     while ((1u << a.span_shift) < chosen.span_blocks) a.span_shift++;
     // A wave a row and key head where these fill the chip and have a sequence's codes in common, so that they are bound by the L2 and by their own instructions
     // (64 spans of 64 of a prompt of 16384, 8 key heads of 128 with 4 heads each, bf16: 256 rows 126 us, 145 with a workgroup a row and key head, 512 rows 226 and 272, 2048 833 and
-    // 1001; 128 rows 78 and 78). Rows of sequences of their own are bound by memory, and eight waves a list have more on its way (256 of them 236 and 209).
+    // 1001; 128 rows 78 and 78; dense attention of the same rows 163, 267, 598). Rows of sequences of their own are bound by memory, and eight waves a list have more on its way (256 of them 236 and 209).
     const uint64_t units = (uint64_t)b.rows * kv.n_kv;
     if (a.g <= 8 && b.row_start && units >= ROW_UNITS && b.rows >= (uint64_t)b.n_seqs * ROW_ROWS) {
         if (!kv_launch_fits(units + 64, 64)) return hipErrorInvalidValue;

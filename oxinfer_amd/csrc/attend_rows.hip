@@ -6,7 +6,7 @@
 // block's values get the weights of its set alone, zeros elsewhere. The sets meet behind the last block, by lane shifts. The mathematics is attend.hip's.
 //
 // 1018 rows of two sequences, 48 spans of 32 each, 4 key heads of 96 with 3 heads each, f32, capped, distance bias: 115 us, 150 by attend_split.hpp's kernel. What the rows read,
-// 1.1 GB, comes from the L2 (93 % hits) at 10 TB/s; of about 160 vector instructions a block 96 turn codes into f16 values, for 3 entries of 16.
+// 1.1 GB, comes from the L2 (93 % hits) at 10 TB/s (the rate seen; not shown to be a limit); of about 160 vector instructions a block 96 turn codes into f16 values, for 3 entries of 16.
 #include <cmath>
 #include <type_traits>
 

@@ -9,7 +9,8 @@
 // forms the weights' exact sums, for each slice, and sets the tokens of these steps apart, in the order of their ids. The third, a workgroup a row, has but these to
 // look at to find the limit: a few by their ranks, many by counting them, in parts of a range that shrinks to one value. Then it knows every slice's sum of
 // what is kept, the slice that the draw falls into, and reads that one again. Tokens that do not fit the room set apart for them (steps that hold much of
-// the vocabulary), and rows whose weights no f32 sorts (infinite logits, temperatures at the ends of f32), are looked at where they are, by a whole row's passes.
+// the vocabulary), and rows whose weights no f32 sorts (infinite logits, temperatures at the ends of f32), are looked at where they are, by a whole row's passes. (64 rows of 151936 bf16, normal
+// logits of deviation 2, top-p 0.95: 90 us; 256 of them, whose slices have room for 256 tokens each, 915.)
 //
 // One row of 128256 f32 takes 21 us (7.8 + 4.9 + 8.8 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 47 (17.4 + 23.4 + 8.7: counting in LDS,
 // the f64 series, the third launch's chain). A workgroup of 512 threads with eight logits each: of 256 with sixteen they took 24.8 and 51.2.

@@ -68,7 +68,7 @@ hipError_t launch_attend_selected(const KvView& kv, const KvBatchView& b, const 
     while ((1u << a.span_shift) < chosen.span_blocks) a.span_shift++;
     // A wave a row and key head where these fill the chip and have a sequence's codes in common, so that they are bound by the L2 and by their own instructions
     // (64 spans of 64 of a prompt of 16384, 8 key heads of 128 with 4 heads each, bf16: 256 rows 126 us, 145 with a workgroup a row and key head, 512 rows 226 and 272, 2048 833 and
-    // 1001; 128 rows 78 and 78; dense attention of the same rows 163, 267, 598). Rows of sequences of their own are bound by memory, and eight waves a list have more on its way (256 of them 236 and 209).
+    // 1001; 128 rows 78 and 78; dense attention of 256, 512 and 2048 rows 163, 267 and 598). Rows of sequences of their own are bound by memory, and eight waves a list have more on its way (256 of them 236 and 209).
     const uint64_t units = (uint64_t)b.rows * kv.n_kv;
     if (a.g <= 8 && b.row_start && units >= ROW_UNITS && b.rows >= (uint64_t)b.n_seqs * ROW_ROWS) {
         if (!kv_launch_fits(units + 64, 64)) return hipErrorInvalidValue;

@@ -12,7 +12,7 @@
 // the vocabulary), and rows whose weights no f32 sorts (infinite logits, temperatures at the ends of f32), are looked at where they are, by a whole row's passes. (64 rows of 151936 bf16, normal
 // logits of deviation 2, top-p 0.95: 90 us; 256 of them, whose slices have room for 256 tokens each, 915.)
 //
-// One row of 128256 f32 takes 21 us (7.8 + 4.9 + 8.8 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 47 (17.4 + 23.4 + 8.7: counting in LDS,
+// One row of 128256 f32 takes 21.6 us (8.0 + 5.2 + 9.5 traced: chains of loads, barriers and arrivals), 64 rows of 151936 bf16, 19 MB, 47 (17.5 + 24.0 + 8.7: counting in LDS,
 // the f64 series, the third launch's chain). A workgroup of 512 threads with eight logits each: of 256 with sixteen they took 24.8 and 51.2.
 #include "sample.hpp"
 
